@@ -33,6 +33,9 @@
  *                                 (qwen3_fused.cpp:502-503), which of its 8 KiB blocks lie near
  *                                 which side of the GPU package; llmi_mha_args.workspace_side
  *   llmi_hip_mha_decode_static    (new) llmi_hip_mha_decode without a caller's workspace
+ *   llmi_hip_mha_decode_tree, llmi_hip_qk_norm_rope_append_tree, llmi_hip_verify_tree,
+ *   llmi_hip_kv_commit_tree       (new) one step of speculative decoding: several drafted tokens
+ *                                 checked in one pass of the model
  *   llmi_pool_* / llmi_hip_pool_* base::CUDADeviceAllocator::allocate / release
  *                                 code/source/base/alloc_cu.cpp:7-119
  *   llmi_hip_memcpy / memset_zero base::DeviceAllocator::memcpy / memset_zero
@@ -302,6 +305,113 @@ int llmi_hip_sincos_table(float* sin_cache, float* cos_cache, int32_t head_dim,
 int llmi_hip_kv_restride(const void* src_pos_major, void* dst_head_major, int32_t layer_num,
                          int32_t max_seq_len, int32_t kv_dim, int32_t head_dim, int32_t num_pos,
                          void* stream);
+
+/* ---- drafted tokens: a tree of them through the model in one pass ------------
+ * No counterpart in the reference, which decodes one token per step. A tree of up to LLMI_TREE_MAX_NODES nodes: node 0
+ * (the root) is the newest certain token, every other node a drafted one whose parent has a smaller index; a chain is the tree
+ * in which node i follows node i - 1. With `pos` positions in the cache node i's K and V rows lie in slot pos + i of
+ * every layer. Per layer: llmi_hip_qk_norm_rope_append_tree, llmi_hip_mha_decode_tree; after the last one
+ * llmi_hip_verify_tree on the nodes' logits, then llmi_hip_kv_commit_tree for all layers: the accepted nodes' rows move to slots
+ * pos, pos + 1, ..., and the next step's root is the token that llmi_hip_verify_tree chose, at position pos + number of
+ * accepted nodes. Position, path and count may stay in device memory throughout, so the whole step can be captured once. */
+#define LLMI_TREE_MAX_NODES 64
+
+typedef struct llmi_mha_tree_args {
+    llmi_mha_args mha;          /* as for llmi_hip_mha_decode, except: query, output and output_f32 hold node_num rows of
+                                   head_num*128, pos is the number of cached positions (= the slot of node 0, and the bound of
+                                   *pos_device), force_path and waves_per_group are 0, workspace_side is ignored         */
+    const uint64_t* tree_mask;  /* device [node_num]: bit j of word i = node i sees node j; bits from node_num on are ignored.
+                                   NULL: a chain, node i sees nodes 0..i                                                  */
+    int32_t node_num;           /* 1 .. LLMI_TREE_MAX_NODES                                                              */
+} llmi_mha_tree_args;
+
+/* Attention of all nodes of one layer: for node i and query head h the softmax-weighted sum of V rows as in
+ * llmi_hip_mha_decode, over the cached positions 0..pos-1 and the nodes its word names (slots pos..pos+node_num-1, written
+ * before). A node with no key at all (an empty word and nothing cached) gets zeros; what stands in the K and V rows a node does
+ * not see leaves no trace in its output, NaN and infinities included. Allocates nothing; safe under stream capture; the workspace needs
+ * no initialisation, and two calls that share one must not overlap in time. */
+int llmi_hip_mha_decode_tree(const llmi_mha_tree_args* args);
+/* What llmi_hip_mha_decode_tree would launch (no HIP call): path, num_splits, rows_per_split, waves_per_group and
+ * workspace_needed as for llmi_hip_mha_plan; group_pad is the query rows (node x head) of a KV head that one workgroup takes. */
+int llmi_hip_mha_tree_plan(const llmi_mha_tree_args* args, llmi_mha_plan* plan);
+/* Bytes of workspace that are enough for any pos and num_splits 0. A smaller one limits the splits. */
+size_t llmi_hip_mha_tree_workspace_bytes(int32_t head_num, int32_t head_dim, int32_t node_num);
+
+typedef struct llmi_qk_norm_rope_tree_args {
+    llmi_qk_norm_rope_args row; /* as for llmi_hip_qk_norm_rope_append, with the rows of node_num nodes behind every row pointer;
+                                   pos is the slot of node 0 (and the bound of *pos_device); value_new and value_cache are required,
+                                   all row pointers 16-byte aligned                                                        */
+    const int32_t* depth;       /* device [node_num]: node i is rotated for position pos + depth[i], held within the tables (0 ..
+                                   max_seq_len-1). NULL: a chain, depth[i] = i                                            */
+    const int32_t* pos_device;  /* optional, device int32: the position read at run time, clamped to 0..row.pos            */
+    int32_t node_num;           /* 1 .. LLMI_TREE_MAX_NODES                                                              */
+    /* elements between one node's row and the next; multiples of 8; 0 = rows lie one behind the other */
+    int64_t query_stride, query_src_stride, key_new_stride, value_new_stride;
+} llmi_qk_norm_rope_tree_args;
+
+/* llmi_hip_qk_norm_rope_append for all nodes of a tree in one launch: node i's K and V rows go to slot pos + i. Same
+ * arithmetic, same bits. key_new must not lie in the slots that are written (the raw rows are read while slots are written),
+ * except row by row: a node's key_new may be its own slot. */
+int llmi_hip_qk_norm_rope_append_tree(const llmi_qk_norm_rope_tree_args* args);
+
+enum { LLMI_LOGITS_F32 = 0, LLMI_LOGITS_BF16 = 1 };
+
+typedef struct llmi_verify_tree_args {
+    const void* target_logits;  /* device [node_num][vocab]: row i is the target's logits behind node i                   */
+    const void* draft_logits;   /* device [node_num][vocab] or NULL: row i is what node i + 1's token was sampled from, in a
+                                   chain (parents NULL) at the same temperature; the last row is not read                 */
+    const int32_t* tokens;      /* device [node_num]; tokens[0] is not read                                               */
+    const int32_t* parents;     /* device [node_num], parents[i] < i (parents[0] is not read), or NULL: a chain           */
+    const float* uniform;       /* device [node_num], in [0, 1): uniform[i] decides node i, uniform[0] the token behind the path */
+    int32_t* path;              /* device [node_num]: the accepted nodes from the root (0) on, then -1                    */
+    int32_t* result;            /* device [2]: number of accepted nodes (the root among them), the token that follows      */
+    void* workspace;            /* device, llmi_hip_verify_tree_workspace_bytes(); needs no initialisation                */
+    size_t workspace_bytes;
+    int32_t node_num;
+    int32_t vocab;
+    int32_t logits_type;        /* LLMI_LOGITS_*, of both                                                                */
+    float temperature;          /* > 0; 0 = greedy                                                                        */
+    int64_t target_stride;      /* elements between rows; 0 = vocab                                                       */
+    int64_t draft_stride;
+    void* stream;
+} llmi_verify_tree_args;
+
+/* Which drafted tokens the target accepts, and the token behind them. p = softmax(target row / temperature).
+ * Greedy (temperature 0): a child is accepted if its token is its parent's likeliest one (the lowest index of equals); the
+ * following token is the last accepted node's likeliest; uniform is not read (and may be NULL), draft_logits must be NULL.
+ * Otherwise the children of a node are tried in index order until one is accepted, and whatever they are, the following token and the
+ * accepted ones are distributed as if sampled from the target:
+ *  - without draft_logits child c of node v is accepted if u[c] * (1 - p_v of the tokens refused before it) < p_v(token of c), never
+ *    if its token has been refused before; if none is, the following token is drawn from p_v without the refused tokens;
+ *  - with draft_logits, q = softmax(draft row / temperature): accepted if u[c] * q_v(token) < p_v(token); if not, the following token
+ *    is drawn from max(p_v - q_v, 0).
+ * Drawn: the first token t at which the sum of what is left over tokens 0..t exceeds u[0] times the sum over all (if nothing is left, the
+ * likeliest). Weights are fp32, their sums fp64, in an order that depends on vocab alone. -inf (a filtered token) and NaN logits have no
+ * weight, +inf counts as the largest finite number; behind a row without a weight nothing is accepted and the token is -1.
+ * A parent or token outside its range makes its node (and those below) one that is not accepted. Allocates nothing; safe under capture. */
+int llmi_hip_verify_tree(const llmi_verify_tree_args* args);
+size_t llmi_hip_verify_tree_workspace_bytes(int32_t node_num, int32_t vocab);
+
+typedef struct llmi_kv_commit_tree_args {
+    void* key_cache;            /* device bf16, base of the whole cache (all layers), 16-byte aligned                     */
+    void* value_cache;
+    const int32_t* path;        /* device [node_num], from llmi_hip_verify_tree                                           */
+    const int32_t* result;      /* device: result[0] = accepted nodes                                                    */
+    const int32_t* pos_device;  /* optional, device int32: clamped to 0..pos                                              */
+    int32_t layer_num;
+    int32_t pos;                /* slot of node 0                                                                         */
+    int32_t node_num;
+    int32_t kv_dim;
+    int32_t head_dim;           /* must be 128 */
+    int32_t max_seq_len;
+    int32_t kv_layout;
+    void* stream;
+} llmi_kv_commit_tree_args;
+
+/* In every layer, for i = 1 .. result[0]-1: the K and V rows of slot pos + path[i] to slot pos + i. In place: an accepted
+ * path ascends, so no row is overwritten before it has been moved. Entries below i or beyond node_num move nothing, every other slot
+ * stays as it is. Does not change the position word: add result[0] to it behind this call. */
+int llmi_hip_kv_commit_tree(const llmi_kv_commit_tree_args* args);
 
 /* ---- pooled device allocator ------------------------------------------- */
 

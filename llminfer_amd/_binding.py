@@ -87,6 +87,36 @@ class QkNormRopeArgs(ctypes.Structure):
     ]
 
 
+class MhaTreeArgs(ctypes.Structure):
+    _fields_ = [("mha", MhaArgs), ("tree_mask", c_void_p), ("node_num", c_i32)]
+
+
+class QkNormRopeTreeArgs(ctypes.Structure):
+    _fields_ = [("row", QkNormRopeArgs), ("depth", c_void_p), ("pos_device", c_void_p), ("node_num", c_i32),
+                ("query_stride", ctypes.c_int64), ("query_src_stride", ctypes.c_int64), ("key_new_stride", ctypes.c_int64),
+                ("value_new_stride", ctypes.c_int64)]
+
+
+class VerifyTreeArgs(ctypes.Structure):
+    _fields_ = [
+        ("target_logits", c_void_p), ("draft_logits", c_void_p), ("tokens", c_void_p), ("parents", c_void_p), ("uniform", c_void_p),
+        ("path", c_void_p), ("result", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+        ("node_num", c_i32), ("vocab", c_i32), ("logits_type", c_i32), ("temperature", ctypes.c_float),
+        ("target_stride", ctypes.c_int64), ("draft_stride", ctypes.c_int64), ("stream", c_void_p),
+    ]
+
+
+class KvCommitTreeArgs(ctypes.Structure):
+    _fields_ = [
+        ("key_cache", c_void_p), ("value_cache", c_void_p), ("path", c_void_p), ("result", c_void_p), ("pos_device", c_void_p),
+        ("layer_num", c_i32), ("pos", c_i32), ("node_num", c_i32), ("kv_dim", c_i32), ("head_dim", c_i32), ("max_seq_len", c_i32),
+        ("kv_layout", c_i32), ("stream", c_void_p),
+    ]
+
+
+TREE_MAX_NODES = 64
+LOGITS_F32, LOGITS_BF16 = 0, 1
+
 DIAG_PLAIN, DIAG_SC0, DIAG_SC1, DIAG_SC0_SC1, DIAG_NT = range(5)  # llmi_hip_diag.h: cache policy of the hand-over probe
 
 
@@ -119,6 +149,13 @@ SYMBOLS = {
     "llmi_hip_qk_norm_rope_append": (ctypes.c_int, [ctypes.POINTER(QkNormRopeArgs)]),
     "llmi_hip_sincos_table": (ctypes.c_int, [c_void_p, c_void_p, c_i32, c_i32, c_void_p]),
     "llmi_hip_kv_restride": (ctypes.c_int, [c_void_p, c_void_p, c_i32, c_i32, c_i32, c_i32, c_i32, c_void_p]),
+    "llmi_hip_mha_decode_tree": (ctypes.c_int, [ctypes.POINTER(MhaTreeArgs)]),
+    "llmi_hip_mha_tree_plan": (ctypes.c_int, [ctypes.POINTER(MhaTreeArgs), ctypes.POINTER(MhaPlan)]),
+    "llmi_hip_mha_tree_workspace_bytes": (c_size_t, [c_i32, c_i32, c_i32]),
+    "llmi_hip_qk_norm_rope_append_tree": (ctypes.c_int, [ctypes.POINTER(QkNormRopeTreeArgs)]),
+    "llmi_hip_verify_tree": (ctypes.c_int, [ctypes.POINTER(VerifyTreeArgs)]),
+    "llmi_hip_verify_tree_workspace_bytes": (c_size_t, [c_i32, c_i32]),
+    "llmi_hip_kv_commit_tree": (ctypes.c_int, [ctypes.POINTER(KvCommitTreeArgs)]),
     "llmi_hip_gemv": (ctypes.c_int, [ctypes.POINTER(GemvArgs)]),
     "llmi_hip_qkv_gemv": (ctypes.c_int, [ctypes.POINTER(QkvGemvArgs)]),
     "llmi_pool_create": (c_void_p, [BACKING_ALLOC_FN, BACKING_FREE_FN, c_void_p]),

@@ -13,7 +13,7 @@ DIAG_LIB_PATH = os.path.join(HERE, "libllmi_diag.so")
 TORCH_OPS_PATH = os.path.join(HERE, "_torch_ops.so")
 
 HIP_SOURCES = ["mha_decode_group4.hip", "mha_decode_group8.hip", "mha_decode_group16.hip", "mha_decode_group2.hip", "mha_decode_group1.hip", "mha_stack.hip", "mha_heads.hip",
-               "mha_decode.hip", "qk_norm_rope.hip", "gemv.hip", "probes.hip", "c_api.cpp", "pool.cpp"]
+               "mha_decode.hip", "mha_tree.hip", "verify_tree.hip", "qk_norm_rope.hip", "gemv.hip", "probes.hip", "c_api.cpp", "tree_api.cpp", "pool.cpp"]
 DIAG_SOURCES = ["diag_probes.hip"]
 
 # -packed-fp32-ops: keep the compiler from forming packed fp32 VALU ops.

@@ -230,7 +230,7 @@ void dyn_split_rule(const llmi_mha_args& args, const llmi_mha_plan& plan, bool a
     *half = h < plan.num_splits ? h : plan.num_splits;
 }
 
-static int validate_mha(const llmi_mha_args* a) {
+int validate_mha(const llmi_mha_args* a) {
     if (!a) return LLMI_ERR_NULL_POINTER;
     if (!a->query || !a->key_cache || !a->value_cache || !a->output) return LLMI_ERR_NULL_POINTER;
     if (a->head_dim != 128) return LLMI_ERR_HEAD_DIM;                               // mha_kernel.cu:478-479

@@ -28,7 +28,8 @@ namespace {
     X(pos_device) X(workspace_side) X(key_new) X(value_new) X(norm_weight) X(sin_cache) X(cos_cache) X(eps) X(o_weight)          \
     X(residual) X(one_launch) X(layer_count) X(query_stride) X(key_new_stride) X(value_new_stride) X(norm_weight_stride)         \
     X(output_stride) X(query_src) X(input) X(weight) X(mode) X(key) X(value) X(src_pos_major) X(dst_head_major) X(layer_num)     \
-    X(num_pos)
+    X(num_pos) X(tree_mask) X(node_num) X(depth) X(target_logits) X(draft_logits) X(tokens) X(parents) X(uniform) X(path)         \
+    X(result) X(temperature)
 
 enum Key : int {
 #define X(name) k_##name,
@@ -124,16 +125,26 @@ struct Abi {
     int (*kv_restride)(const void*, void*, int32_t, int32_t, int32_t, int32_t, int32_t, void*);
     int (*gemv)(const llmi_gemv_args*);
     int (*qkv_gemv)(const llmi_qkv_gemv_args*);
+    int (*mha_decode_tree)(const llmi_mha_tree_args*);
+    int (*qk_norm_rope_append_tree)(const llmi_qk_norm_rope_tree_args*);
+    int (*verify_tree)(const llmi_verify_tree_args*);
+    int (*kv_commit_tree)(const llmi_kv_commit_tree_args*);
 } g_abi;
 PyObject *g_get_device, *g_get_stream;   // torch's current device, and its current stream as a number
 PyObject *g_check_dev, *g_check_status;  // ops._check_dev, _binding.check: they raise
-PyObject *g_bf16_types, *g_f32_types;    // what _check_dev is told to expect
+PyObject *g_bf16_types, *g_f32_types, *g_i32_types, *g_i64_types;  // what _check_dev is told to expect
 
 // ---- conversions ----
-enum class Kind { bf16, f32 };
+enum class Kind { bf16, f32, i32, i64 };
+
+PyObject* types_of(Kind kind) {
+    return kind == Kind::f32 ? g_f32_types : kind == Kind::i32 ? g_i32_types : kind == Kind::i64 ? g_i64_types : g_bf16_types;
+}
 
 inline bool type_fits(const at::Tensor& t, Kind kind) {
     const at::ScalarType s = t.scalar_type();
+    if (kind == Kind::i32) return s == at::kInt;
+    if (kind == Kind::i64) return s == at::kLong || s == at::ScalarType::UInt64;
     return kind == Kind::f32 ? s == at::kFloat : s == at::kBFloat16 || s == at::kShort || s == at::ScalarType::UInt16;
 }
 
@@ -147,7 +158,7 @@ void* address(PyObject* const* vals, Key key, Kind kind, bool* ok) {
         if (t.is_cuda() && type_fits(t, kind) && t.is_contiguous()) return t.data_ptr();
     }
     *ok = false;
-    PyObject* r = PyObject_CallFunctionObjArgs(g_check_dev, g_key[key], o, kind == Kind::f32 ? g_f32_types : g_bf16_types, nullptr);
+    PyObject* r = PyObject_CallFunctionObjArgs(g_check_dev, g_key[key], o, types_of(kind), nullptr);
     if (r) {
         Py_DECREF(r);
         PyErr_Format(PyExc_ValueError, "%s is not a tensor this call can take", kKeyText[key]);
@@ -271,7 +282,7 @@ void fill_append(PyObject* const* vals, llmi_mha_append_args* a, bool* ok) {
 #define LLMI_PARSE(sig)              \
     PyObject* vals[kKeys];           \
     if (!parse(sig, args, n_args, names, vals)) return nullptr; \
-    bool ok = true
+    [[maybe_unused]] bool ok = true
 
 constexpr Key kDecodePos[] = {k_query, k_key_cache, k_value_cache, k_output, k_workspace};
 const Signature kDecodeSig = {"mha_decode", kDecodePos, 5, kMhaKeywords,
@@ -441,10 +452,210 @@ LLMI_ENTRY(qkv_gemv) {
     Py_RETURN_NONE;
 }
 
-// bind(functions, get_device, get_stream, check_dev, check_status, bf16_types, f32_types); functions: C ABI name -> address
+// ---- drafted tokens ----
+// These calls know how long their rows are, and look: a tensor that is shorter than what the call would touch, or that lies on another
+// device than the one the launch goes to, is refused.
+struct Looked {
+    PyObject* const* vals;
+    bool ok = true;
+    int device = -1;  // the current one, once asked for
+
+    explicit Looked(PyObject* const* v) : vals(v) {}
+    bool absent(Key key) const { return !vals[key] || vals[key] == Py_None; }
+    const at::Tensor& tensor(Key key) const { return THPVariable_Unpack(vals[key]); }
+    bool here(Key key) {
+        if (device < 0 && ok) {
+            PyObject* d = PyObject_CallNoArgs(g_get_device);
+            if (d) device = (int)PyLong_AsLong(d);
+            Py_XDECREF(d);
+            if (PyErr_Occurred()) ok = false;
+        }
+        if (ok && tensor(key).device().index() != device) {
+            PyErr_Format(PyExc_ValueError, "%s is on device %d, the current device is %d", kKeyText[key], (int)tensor(key).device().index(), device);
+            ok = false;
+        }
+        return ok;
+    }
+    bool holds(Key key, int64_t least) {
+        if (ok && tensor(key).numel() < least) {
+            PyErr_Format(PyExc_ValueError, "%s has %lld elements, the call needs %lld", kKeyText[key], (long long)tensor(key).numel(), (long long)least);
+            ok = false;
+        }
+        return ok;
+    }
+    // A contiguous tensor of at least `least` elements.
+    template <typename P>
+    P* whole(Key key, Kind kind, int64_t least) {
+        void* p = address(vals, key, kind, &ok);
+        if (!ok || absent(key) || !here(key) || !holds(key, least)) return nullptr;
+        return static_cast<P*>(p);
+    }
+    // `rows` rows of `width` elements: a 2-D tensor whose rows may lie apart (a slice of a wider one).
+    void* rows(Key key, Kind kind, int64_t rows, int64_t width, int64_t* stride) {
+        *stride = 0;
+        if (!ok || absent(key)) return nullptr;
+        if (!THPVariable_Check(vals[key]) || !tensor(key).is_cuda() || !type_fits(tensor(key), kind) || tensor(key).dim() != 2)
+            return whole<void>(key, kind, rows * width);
+        const at::Tensor& t = tensor(key);
+        if (!here(key)) return nullptr;
+        if (t.size(0) < rows || t.size(1) != width || (width > 1 && t.stride(1) != 1) || (rows > 1 && t.stride(0) < width)) {
+            PyErr_Format(PyExc_ValueError, "%s must be [%lld][%lld] with contiguous rows", kKeyText[key], (long long)rows, (long long)width);
+            ok = false;
+            return nullptr;
+        }
+        *stride = rows > 1 ? t.stride(0) : 0;
+        return t.data_ptr();
+    }
+    float number(Key key, float unset) {
+        if (!ok || !vals[key]) return unset;
+        const double v = PyFloat_AsDouble(vals[key]);
+        if (PyErr_Occurred()) ok = false;
+        return (float)v;
+    }
+    int64_t positive(Key key) {
+        const int32_t v = int32(vals, key, 0, &ok);
+        return v > 0 ? v : 0;  // (what is out of range is the C ABI's to refuse)
+    }
+    const int32_t* position() {
+        if (ok && !absent(k_pos_device) && THPVariable_Check(vals[k_pos_device])) return whole<const int32_t>(k_pos_device, Kind::i32, 1);
+        return static_cast<const int32_t*>(tensor_or_address(vals, k_pos_device, &ok));
+    }
+};
+
+const Signature kTreeSig = {
+    "mha_decode_tree", kDecodePos, 5,
+    bits({k_tree_mask, k_node_num, k_stream, k_layer_id, k_pos, k_kv_dim, k_kv_mul, k_head_num, k_head_dim, k_max_seq_len, k_kv_layout,
+          k_num_splits, k_output_f32, k_pos_device}),
+    kMhaRequired | bits({k_query, k_key_cache, k_value_cache, k_output, k_workspace, k_node_num})};
+LLMI_ENTRY(mha_decode_tree) {
+    LLMI_PARSE(kTreeSig);
+    llmi_mha_tree_args t{};
+    fill_mha(vals, k_query, &t.mha, &ok);
+    if (!ok) return nullptr;
+    Looked look(vals);
+    t.node_num = int32(vals, k_node_num, 0, &look.ok);
+    const int64_t rows = look.positive(k_node_num) * look.positive(k_head_num) * look.positive(k_head_dim);
+    const int64_t cached = (look.positive(k_layer_id) + 1) * look.positive(k_max_seq_len) * look.positive(k_kv_dim);
+    look.whole<void>(k_query, Kind::bf16, rows);
+    look.whole<void>(k_key_cache, Kind::bf16, cached);
+    look.whole<void>(k_value_cache, Kind::bf16, cached);
+    look.whole<void>(k_output, Kind::bf16, rows);
+    look.whole<void>(k_output_f32, Kind::f32, rows);
+    look.whole<void>(k_workspace, Kind::f32, 0);
+    t.mha.pos_device = look.position();
+    t.tree_mask = look.whole<const uint64_t>(k_tree_mask, Kind::i64, look.positive(k_node_num));
+    if (!look.ok || !call("llmi_hip_mha_decode_tree", [&] { return g_abi.mha_decode_tree(&t); })) return nullptr;
+    return Py_NewRef(vals[k_output]);
+}
+
+const Signature kNormRopeTreeSig = {
+    "qk_norm_rope_append_tree", kNormRopePos, 8,
+    bits({k_node_num, k_depth, k_layer_id, k_pos, k_kv_dim, k_head_num, k_head_dim, k_max_seq_len, k_kv_layout, k_eps, k_query_src,
+          k_pos_device, k_stream}),
+    kNormRopeSig.required | bits({k_node_num})};
+LLMI_ENTRY(qk_norm_rope_append_tree) {
+    LLMI_PARSE(kNormRopeTreeSig);
+    Looked look(vals);
+    llmi_qk_norm_rope_tree_args t{};
+    llmi_qk_norm_rope_args& a = t.row;
+    t.node_num = int32(vals, k_node_num, 0, &look.ok);
+    a.layer_id = int32(vals, k_layer_id, 0, &look.ok);
+    a.pos = int32(vals, k_pos, 0, &look.ok);
+    a.kv_dim = int32(vals, k_kv_dim, 0, &look.ok);
+    a.head_num = int32(vals, k_head_num, 0, &look.ok);
+    a.head_dim = int32(vals, k_head_dim, 0, &look.ok);
+    a.max_seq_len = int32(vals, k_max_seq_len, 0, &look.ok);
+    a.kv_layout = int32(vals, k_kv_layout, LLMI_KV_LAYOUT_POS_MAJOR, &look.ok);
+    a.eps = look.number(k_eps, 1e-6f);
+    if (!look.ok) return nullptr;
+    const int64_t n = look.positive(k_node_num), dim = look.positive(k_head_num) * look.positive(k_head_dim), kv_dim = look.positive(k_kv_dim);
+    const int64_t cached = (look.positive(k_layer_id) + 1) * look.positive(k_max_seq_len) * kv_dim;
+    const int64_t table = look.positive(k_max_seq_len) * (look.positive(k_head_dim) / 2);
+    a.query = look.rows(k_query, Kind::bf16, n, dim, &t.query_stride);
+    a.query_src = look.rows(k_query_src, Kind::bf16, n, dim, &t.query_src_stride);
+    a.key_new = look.rows(k_key_new, Kind::bf16, n, kv_dim, &t.key_new_stride);
+    a.value_new = look.rows(k_value_new, Kind::bf16, n, kv_dim, &t.value_new_stride);
+    a.key_cache = look.whole<void>(k_key_cache, Kind::bf16, cached);
+    a.value_cache = look.whole<void>(k_value_cache, Kind::bf16, cached);
+    a.norm_weight = look.whole<const void>(k_norm_weight, Kind::bf16, 2 * look.positive(k_head_dim));
+    a.sin_cache = look.whole<const float>(k_sin_cache, Kind::f32, table);
+    a.cos_cache = look.whole<const float>(k_cos_cache, Kind::f32, table);
+    t.depth = look.whole<const int32_t>(k_depth, Kind::i32, n);
+    t.pos_device = look.position();
+    a.stream = stream_of(vals, &look.ok);
+    if (!look.ok || !call("llmi_hip_qk_norm_rope_append_tree", [&] { return g_abi.qk_norm_rope_append_tree(&t); })) return nullptr;
+    Py_RETURN_NONE;
+}
+
+constexpr Key kVerifyPos[] = {k_target_logits, k_tokens, k_uniform, k_path, k_result, k_workspace};
+const Signature kVerifySig = {"verify_tree", kVerifyPos, 6, bits({k_parents, k_draft_logits, k_temperature, k_stream}),
+                              bits({k_target_logits, k_tokens, k_uniform, k_path, k_result, k_workspace})};
+LLMI_ENTRY(verify_tree) {
+    LLMI_PARSE(kVerifySig);
+    Looked look(vals);
+    if (!THPVariable_Check(vals[k_target_logits]) || THPVariable_Unpack(vals[k_target_logits]).dim() != 2) {
+        PyErr_SetString(PyExc_ValueError, "target_logits must be a [nodes][vocab] tensor");
+        return nullptr;
+    }
+    const at::Tensor& target = look.tensor(k_target_logits);
+    const int64_t n = target.size(0), vocab = target.size(1);
+    if (n < 1 || n > LLMI_TREE_MAX_NODES || vocab < 1 || vocab > INT32_MAX) {
+        PyErr_Format(PyExc_ValueError, "target_logits must have 1 to %d rows of at least one token", LLMI_TREE_MAX_NODES);
+        return nullptr;
+    }
+    const Kind kind = target.scalar_type() == at::kFloat ? Kind::f32 : Kind::bf16;
+    llmi_verify_tree_args a{};
+    a.node_num = (int32_t)n;
+    a.vocab = (int32_t)vocab;
+    a.logits_type = kind == Kind::f32 ? LLMI_LOGITS_F32 : LLMI_LOGITS_BF16;
+    a.temperature = look.number(k_temperature, 1.0f);
+    a.target_logits = look.rows(k_target_logits, kind, n, vocab, &a.target_stride);
+    a.draft_logits = look.rows(k_draft_logits, kind, n, vocab, &a.draft_stride);
+    a.tokens = look.whole<const int32_t>(k_tokens, Kind::i32, n);
+    a.parents = look.whole<const int32_t>(k_parents, Kind::i32, n);
+    a.uniform = look.whole<const float>(k_uniform, Kind::f32, n);
+    a.path = look.whole<int32_t>(k_path, Kind::i32, n);
+    a.result = look.whole<int32_t>(k_result, Kind::i32, 2);
+    a.workspace = look.whole<void>(k_workspace, Kind::f32, 0);
+    if (a.workspace) a.workspace_bytes = look.tensor(k_workspace).nbytes();
+    a.stream = stream_of(vals, &look.ok);
+    if (!look.ok || !call("llmi_hip_verify_tree", [&] { return g_abi.verify_tree(&a); })) return nullptr;
+    return Py_NewRef(vals[k_result]);
+}
+
+constexpr Key kCommitPos[] = {k_key_cache, k_value_cache, k_path, k_result};
+const Signature kCommitSig = {
+    "kv_commit_tree", kCommitPos, 4,
+    bits({k_node_num, k_layer_num, k_pos, k_kv_dim, k_head_dim, k_max_seq_len, k_kv_layout, k_pos_device, k_stream}),
+    bits({k_key_cache, k_value_cache, k_path, k_result, k_node_num, k_layer_num, k_pos, k_kv_dim, k_head_dim, k_max_seq_len})};
+LLMI_ENTRY(kv_commit_tree) {
+    LLMI_PARSE(kCommitSig);
+    Looked look(vals);
+    llmi_kv_commit_tree_args a{};
+    a.node_num = int32(vals, k_node_num, 0, &look.ok);
+    a.layer_num = int32(vals, k_layer_num, 0, &look.ok);
+    a.pos = int32(vals, k_pos, 0, &look.ok);
+    a.kv_dim = int32(vals, k_kv_dim, 0, &look.ok);
+    a.head_dim = int32(vals, k_head_dim, 0, &look.ok);
+    a.max_seq_len = int32(vals, k_max_seq_len, 0, &look.ok);
+    a.kv_layout = int32(vals, k_kv_layout, LLMI_KV_LAYOUT_POS_MAJOR, &look.ok);
+    if (!look.ok) return nullptr;
+    const int64_t cached = look.positive(k_layer_num) * look.positive(k_max_seq_len) * look.positive(k_kv_dim);
+    a.key_cache = look.whole<void>(k_key_cache, Kind::bf16, cached);
+    a.value_cache = look.whole<void>(k_value_cache, Kind::bf16, cached);
+    a.path = look.whole<const int32_t>(k_path, Kind::i32, look.positive(k_node_num));
+    a.result = look.whole<const int32_t>(k_result, Kind::i32, 1);
+    a.pos_device = look.position();
+    a.stream = stream_of(vals, &look.ok);
+    if (!look.ok || !call("llmi_hip_kv_commit_tree", [&] { return g_abi.kv_commit_tree(&a); })) return nullptr;
+    Py_RETURN_NONE;
+}
+
+// bind(functions, get_device, get_stream, check_dev, check_status, bf16_types, f32_types, i32_types, i64_types); functions: C ABI name -> address
 PyObject* bind(PyObject*, PyObject* args) {
-    PyObject *functions, *objs[6];
-    if (!PyArg_ParseTuple(args, "O!OOOOOO", &PyDict_Type, &functions, &objs[0], &objs[1], &objs[2], &objs[3], &objs[4], &objs[5])) return nullptr;
+    PyObject *functions, *objs[8];
+    if (!PyArg_ParseTuple(args, "O!OOOOOOOO", &PyDict_Type, &functions, &objs[0], &objs[1], &objs[2], &objs[3], &objs[4], &objs[5], &objs[6], &objs[7]))
+        return nullptr;
     struct {
         const char* name;
         void* slot;
@@ -457,7 +668,11 @@ PyObject* bind(PyObject*, PyObject* args) {
                   {"llmi_hip_qk_norm_rope_append", &g_abi.qk_norm_rope_append},
                   {"llmi_hip_kv_restride", &g_abi.kv_restride},
                   {"llmi_hip_gemv", &g_abi.gemv},
-                  {"llmi_hip_qkv_gemv", &g_abi.qkv_gemv}};
+                  {"llmi_hip_qkv_gemv", &g_abi.qkv_gemv},
+                  {"llmi_hip_mha_decode_tree", &g_abi.mha_decode_tree},
+                  {"llmi_hip_qk_norm_rope_append_tree", &g_abi.qk_norm_rope_append_tree},
+                  {"llmi_hip_verify_tree", &g_abi.verify_tree},
+                  {"llmi_hip_kv_commit_tree", &g_abi.kv_commit_tree}};
     for (const auto& w : wanted) {
         PyObject* n = PyDict_GetItemString(functions, w.name);  // borrowed
         void* p = n ? PyLong_AsVoidPtr(n) : nullptr;
@@ -468,8 +683,8 @@ PyObject* bind(PyObject*, PyObject* args) {
         }
         *static_cast<void**>(w.slot) = p;
     }
-    PyObject** const keep[] = {&g_get_device, &g_get_stream, &g_check_dev, &g_check_status, &g_bf16_types, &g_f32_types};
-    for (int i = 0; i < 6; ++i) {
+    PyObject** const keep[] = {&g_get_device, &g_get_stream, &g_check_dev, &g_check_status, &g_bf16_types, &g_f32_types, &g_i32_types, &g_i64_types};
+    for (int i = 0; i < 8; ++i) {
         Py_INCREF(objs[i]);
         Py_XSETREF(*keep[i], objs[i]);
     }
@@ -519,6 +734,25 @@ PyMethodDef g_methods[] = {
     LLMI_METHOD(qkv_gemv, "($module, input, weight, query, key, value, *, stream=None)",
                 "The packed QKV projection: rows [0, dim) of weight @ input go to query, the next kv_dim to key,\n"
                 "the last kv_dim to value (llmi_hip_qkv_gemv)."),
+    LLMI_METHOD(mha_decode_tree,
+                "($module, query, key_cache, value_cache, output, workspace, *, node_num, tree_mask=None, stream=None, layer_id, pos, kv_dim, "
+                "kv_mul, head_num, head_dim, max_seq_len, kv_layout=0, num_splits=0, output_f32=None, pos_device=None)",
+                "Attention of the nodes of a tree of drafted tokens over `pos` cached positions and the nodes that each one's\n"
+                "64-bit word in `tree_mask` names (llmi_hip_mha_decode_tree); returns the output."),
+    LLMI_METHOD(qk_norm_rope_append_tree,
+                "($module, query, key_new, value_new, key_cache, value_cache, norm_weight, sin_cache, cos_cache, *, node_num, depth=None, "
+                "layer_id, pos, kv_dim, head_num, head_dim, max_seq_len, kv_layout=0, eps=1e-06, query_src=None, pos_device=None, stream=None)",
+                "qk_norm_rope_append for all nodes of a tree: node i to slot pos + i, rotated for position pos + depth[i]\n"
+                "(llmi_hip_qk_norm_rope_append_tree). The rows of query, query_src, key_new and value_new may be slices of wider ones."),
+    LLMI_METHOD(verify_tree,
+                "($module, target_logits, tokens, uniform, path, result, workspace, *, parents=None, draft_logits=None, temperature=1.0, "
+                "stream=None)",
+                "Drafted tokens against the target's logits [nodes][vocab], from given random numbers (llmi_hip_verify_tree): the accepted\n"
+                "nodes into `path`, their number and the token that follows into `result`, which is returned."),
+    LLMI_METHOD(kv_commit_tree,
+                "($module, key_cache, value_cache, path, result, *, node_num, layer_num, pos, kv_dim, head_dim, max_seq_len, kv_layout=0, "
+                "pos_device=None, stream=None)",
+                "The accepted nodes' K and V rows to consecutive slots from pos on, in all layers (llmi_hip_kv_commit_tree)."),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_torch_ops", "Native calls of llminfer_amd.ops.", -1, g_methods};

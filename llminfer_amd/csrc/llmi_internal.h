@@ -126,6 +126,13 @@ int launch_sincos_table(float* sin_cache, float* cos_cache, int32_t head_dim, in
                         hipStream_t stream);
 int launch_gemv(const void* input, const void* weight, void* const out[3], const int32_t seg_end[3], int32_t n,
                 int32_t k, int32_t mode, hipStream_t stream);
+// What every attention call asks of its arguments (c_api.cpp).
+int validate_mha(const llmi_mha_args* a);
+int launch_mha_tree(const llmi_mha_tree_args& args, const llmi_mha_plan& plan);
+int launch_qk_norm_rope_append_tree(const llmi_qk_norm_rope_tree_args& args);
+size_t verify_tree_workspace_bytes(int32_t node_num, int32_t vocab);
+int launch_verify_tree(const llmi_verify_tree_args& args);
+int launch_kv_commit_tree(const llmi_kv_commit_tree_args& args);
 int launch_kv_restride(const void* src, void* dst, int32_t layer_num, int32_t max_seq_len,
                        int32_t kv_dim, int32_t head_dim, int32_t num_pos, hipStream_t stream);
 

@@ -47,6 +47,22 @@ struct AppendArgs {
     float eps;
 };
 
+// One row on one wavefront: lane i owns the rotation pair (i, i + 64).
+__device__ __forceinline__ void norm_rope_row(const uint16_t* src, const uint16_t* w, const float* sin_row, const float* cos_row, float eps,
+                                              int i, uint16_t* dst) {
+    const float x0 = bf16_to_f32(src[i]);
+    const float x1 = bf16_to_f32(src[i + kHalf]);
+    float ss = x0 * x0 + x1 * x1;
+    ss = wave_sum(ss);
+    const float r = 1.0f / sqrtf(ss / (float)kHeadDim + eps);
+    const float av = x0 * bf16_to_f32(w[i]) * r;
+    const float bv = x1 * bf16_to_f32(w[i + kHalf]) * r;
+    const float sn = sin_row[i];
+    const float cs = cos_row[i];
+    dst[i] = f32_to_bf16(av * cs - bv * sn);
+    dst[i + kHalf] = f32_to_bf16(av * sn + bv * cs);
+}
+
 __global__ __launch_bounds__(kHalf) void qk_norm_rope_append_kernel(AppendArgs a) {
     const int b = blockIdx.x;
     const int i = threadIdx.x;
@@ -71,17 +87,68 @@ __global__ __launch_bounds__(kHalf) void qk_norm_rope_append_kernel(AppendArgs a
         dst = a.key_slot + kh * a.slot_head_stride;
         w = a.weight + kHeadDim;
     }
-    const float x0 = bf16_to_f32(src[i]);
-    const float x1 = bf16_to_f32(src[i + kHalf]);
-    float ss = x0 * x0 + x1 * x1;
-    ss = wave_sum(ss);
-    const float r = 1.0f / sqrtf(ss / (float)kHeadDim + a.eps);
-    const float av = x0 * bf16_to_f32(w[i]) * r;
-    const float bv = x1 * bf16_to_f32(w[i + kHalf]) * r;
-    const float sn = a.sin_row[i];
-    const float cs = a.cos_row[i];
-    dst[i] = f32_to_bf16(av * cs - bv * sn);
-    dst[i + kHalf] = f32_to_bf16(av * sn + bv * cs);
+    norm_rope_row(src, w, a.sin_row, a.cos_row, a.eps, i, dst);
+}
+
+// The same for the nodes of a tree: node i's rows to slot pos + i, rotated for position pos + depth[i].
+struct AppendTreeArgs {
+    uint16_t* query;
+    const uint16_t* query_src;
+    const uint16_t* key_new;
+    const uint16_t* value_new;
+    int64_t query_stride, query_src_stride, key_new_stride, value_new_stride;  // elements between nodes
+    uint16_t* key_layer;
+    uint16_t* value_layer;
+    const uint16_t* weight;
+    const float* sin_cache;
+    const float* cos_cache;
+    const int32_t* depth;    // optional
+    const int32_t* pos_dev;  // optional
+    int64_t row_stride, head_stride;  // elements between positions / KV heads of the caches
+    int32_t pos, max_seq_len, head_num, n_kv;
+    float eps;
+};
+
+__global__ __launch_bounds__(kHalf) void qk_norm_rope_append_tree_kernel(AppendTreeArgs a) {
+    const int b = blockIdx.x, node = blockIdx.y, i = threadIdx.x;
+    const int pos = a.pos_dev ? max(0, min(*a.pos_dev, a.pos)) : a.pos;
+    const int kh = b < a.head_num ? 0 : (b - a.head_num) % a.n_kv;
+    const int64_t slot = (int64_t)(pos + node) * a.row_stride + kh * a.head_stride;
+    if (b >= a.head_num + a.n_kv) {
+        const uint32_t* src = reinterpret_cast<const uint32_t*>(a.value_new + node * a.value_new_stride + kh * kHeadDim);
+        reinterpret_cast<uint32_t*>(a.value_layer + slot)[i] = src[i];
+        return;
+    }
+    const int64_t at = (int64_t)pos + (a.depth ? a.depth[node] : node);
+    const int64_t table = (at < 0 ? 0 : at < a.max_seq_len ? at : a.max_seq_len - 1) * kHalf;
+    const bool is_query = b < a.head_num;
+    norm_rope_row(is_query ? a.query_src + node * a.query_src_stride + b * kHeadDim : a.key_new + node * a.key_new_stride + kh * kHeadDim,
+                  a.weight + (is_query ? 0 : kHeadDim), a.sin_cache + table, a.cos_cache + table, a.eps, i,
+                  is_query ? a.query + node * a.query_stride + b * kHeadDim : a.key_layer + slot);
+}
+
+// Rows of accepted nodes, slot pos + path[i] to slot pos + i. A thread moves one 16-byte chunk of every row in path order: the path ascends, so
+// what it writes (place i) is behind everything it has still to read (path[j] >= j > i).
+struct CommitArgs {
+    uint4* cache[2];
+    const int32_t* path;
+    const int32_t* result;
+    const int32_t* pos_dev;  // optional
+    int64_t layer_chunks, row_chunks, head_chunks;
+    int32_t pos, nodes, n_kv;
+};
+
+__global__ __launch_bounds__(256) void kv_commit_tree_kernel(CommitArgs a) {
+    const int at = blockIdx.x * 256 + threadIdx.x;
+    const int kh = at >> 4;
+    if (kh >= a.n_kv) return;
+    const int pos = a.pos_dev ? max(0, min(*a.pos_dev, a.pos)) : a.pos;
+    const int count = min(a.result[0], a.nodes);
+    uint4* base = a.cache[blockIdx.z] + blockIdx.y * a.layer_chunks + pos * a.row_chunks + kh * a.head_chunks + (at & 15);
+    for (int i = 1; i < count; ++i) {
+        const int from = a.path[i];
+        if (from > i && from < a.nodes) base[i * a.row_chunks] = base[from * a.row_chunks];
+    }
 }
 
 __global__ void sincos_table_kernel(float* __restrict__ sin_cache, float* __restrict__ cos_cache, int32_t half,
@@ -153,6 +220,58 @@ int launch_qk_norm_rope_append(const llmi_qk_norm_rope_args& args) {
     a.eps = args.eps;
     const int blocks = args.head_num + n_kv + (args.value_new ? n_kv : 0);
     hipLaunchKernelGGL(qk_norm_rope_append_kernel, dim3(blocks), dim3(kHalf), 0,
+                       static_cast<hipStream_t>(args.stream), a);
+    return check_launch();
+}
+
+int launch_qk_norm_rope_append_tree(const llmi_qk_norm_rope_tree_args& args) {
+    const llmi_qk_norm_rope_args& r = args.row;
+    const bool by_head = r.kv_layout == LLMI_KV_LAYOUT_HEAD_MAJOR;
+    const int64_t layer = (int64_t)r.layer_id * r.max_seq_len * r.kv_dim, q_row = (int64_t)r.head_num * kHeadDim;
+    AppendTreeArgs a;
+    a.query = static_cast<uint16_t*>(r.query);
+    a.query_src = r.query_src ? static_cast<const uint16_t*>(r.query_src) : a.query;
+    a.key_new = static_cast<const uint16_t*>(r.key_new);
+    a.value_new = static_cast<const uint16_t*>(r.value_new);
+    a.query_stride = args.query_stride ? args.query_stride : q_row;
+    a.query_src_stride = !r.query_src ? a.query_stride : args.query_src_stride ? args.query_src_stride : q_row;
+    a.key_new_stride = args.key_new_stride ? args.key_new_stride : r.kv_dim;
+    a.value_new_stride = args.value_new_stride ? args.value_new_stride : r.kv_dim;
+    a.key_layer = static_cast<uint16_t*>(r.key_cache) + layer;
+    a.value_layer = static_cast<uint16_t*>(r.value_cache) + layer;
+    a.weight = static_cast<const uint16_t*>(r.norm_weight);
+    a.sin_cache = r.sin_cache;
+    a.cos_cache = r.cos_cache;
+    a.depth = args.depth;
+    a.pos_dev = args.pos_device;
+    a.row_stride = by_head ? kHeadDim : r.kv_dim;
+    a.head_stride = by_head ? (int64_t)r.max_seq_len * kHeadDim : kHeadDim;
+    a.pos = r.pos;
+    a.max_seq_len = r.max_seq_len;
+    a.head_num = r.head_num;
+    a.n_kv = r.kv_dim / kHeadDim;
+    a.eps = r.eps;
+    hipLaunchKernelGGL(qk_norm_rope_append_tree_kernel, dim3(a.head_num + 2 * a.n_kv, args.node_num), dim3(kHalf), 0,
+                       static_cast<hipStream_t>(r.stream), a);
+    return check_launch();
+}
+
+int launch_kv_commit_tree(const llmi_kv_commit_tree_args& args) {
+    if (args.node_num == 1) return LLMI_OK;  // (the root is in its place)
+    const bool by_head = args.kv_layout == LLMI_KV_LAYOUT_HEAD_MAJOR;
+    CommitArgs a;
+    a.cache[0] = static_cast<uint4*>(args.key_cache);
+    a.cache[1] = static_cast<uint4*>(args.value_cache);
+    a.path = args.path;
+    a.result = args.result;
+    a.pos_dev = args.pos_device;
+    a.n_kv = args.kv_dim / kHeadDim;
+    a.layer_chunks = (int64_t)args.max_seq_len * a.n_kv * 16;
+    a.row_chunks = by_head ? 16 : (int64_t)a.n_kv * 16;
+    a.head_chunks = by_head ? (int64_t)args.max_seq_len * 16 : 16;
+    a.pos = args.pos;
+    a.nodes = args.node_num;
+    hipLaunchKernelGGL(kv_commit_tree_kernel, dim3((a.n_kv * 16 + 255) / 256, args.layer_num, 2), dim3(256), 0,
                        static_cast<hipStream_t>(args.stream), a);
     return check_launch();
 }

@@ -36,6 +36,15 @@ def workspace_bytes(head_num, head_dim, max_seq_len):
     return int(B.lib().llmi_hip_mha_workspace_bytes(head_num, head_dim, max_seq_len))
 
 
+def tree_workspace_bytes(head_num, head_dim, node_num):
+    """Enough for mha_decode_tree at any length."""
+    return int(B.lib().llmi_hip_mha_tree_workspace_bytes(head_num, head_dim, node_num))
+
+
+def verify_workspace_bytes(node_num, vocab):
+    return int(B.lib().llmi_hip_verify_tree_workspace_bytes(node_num, vocab))
+
+
 def make_mha_args(query, key_cache, value_cache, output, workspace, *, layer_id, pos, kv_dim, kv_mul,
                   head_num, head_dim, max_seq_len, kv_layout=B.KV_LAYOUT_POS_MAJOR, force_path=B.PATH_AUTO,
                   num_splits=0, waves_per_group=0, output_f32=None, stream=None, pos_device=None, workspace_side=0):
@@ -105,10 +114,11 @@ def _native():
     lib = B.lib()
     names = ("llmi_hip_mha_decode", "llmi_hip_mha_decode_append", "llmi_hip_mha_decode_append_oproj", "llmi_hip_mha_oproj_launches",
              "llmi_hip_mha_decode_append_stack", "llmi_hip_mha_stack_launches", "llmi_hip_qk_norm_rope_append", "llmi_hip_kv_restride",
-             "llmi_hip_gemv", "llmi_hip_qkv_gemv")
+             "llmi_hip_gemv", "llmi_hip_qkv_gemv", "llmi_hip_mha_decode_tree", "llmi_hip_qk_norm_rope_append_tree", "llmi_hip_verify_tree",
+             "llmi_hip_kv_commit_tree")
     addresses = {n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names}
     abi = native.bind(addresses, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, _check_dev, B.check, _BF16_DTYPES,
-                      (torch.float32,))
+                      (torch.float32,), (torch.int32,), (torch.int64, torch.uint64))
     if abi != lib.llmi_hip_abi_version():
         raise RuntimeError("the torch front end was built against ABI %d, the library is %d" % (abi, lib.llmi_hip_abi_version()))
     return native
@@ -116,8 +126,9 @@ def _native():
 
 # The native calls by name. They take their places in this module when the first of them is asked for: importing it, and its argument
 # helpers, need nothing built.
-_CALLS = ("mha_decode", "mha_decode_append", "mha_decode_append_stack", "qk_norm_rope_append", "kv_restride", "gemv", "qkv_gemv")
-__all__ = ["workspace_bytes", "make_mha_args", "workspace_side", "mha_plan", "mha_decode_raw", "sincos_table", *_CALLS]
+_CALLS = ("mha_decode", "mha_decode_append", "mha_decode_append_stack", "qk_norm_rope_append", "kv_restride", "gemv", "qkv_gemv",
+          "mha_decode_tree", "qk_norm_rope_append_tree", "verify_tree", "kv_commit_tree")
+__all__ = ["workspace_bytes", "tree_workspace_bytes", "verify_workspace_bytes", "make_mha_args", "workspace_side", "mha_plan", "mha_decode_raw", "sincos_table", *_CALLS]
 
 
 def _bind_calls():
