@@ -128,6 +128,9 @@ int launch_gemv(const void* input, const void* weight, void* const out[3], const
                 int32_t k, int32_t mode, hipStream_t stream);
 // What every attention call asks of its arguments (c_api.cpp).
 int validate_mha(const llmi_mha_args* a);
+constexpr int kTreeKeys = 32;  // keys per tile of the tree attention
+// Bytes of workspace per split of a KV head's block of 32 query rows: 32 x 128 partial sums, 32 maxima and sums.
+constexpr size_t kTreeSplitBytes = 32 * (128 + 2) * sizeof(float);
 int launch_mha_tree(const llmi_mha_tree_args& args, const llmi_mha_plan& plan);
 int launch_qk_norm_rope_append_tree(const llmi_qk_norm_rope_tree_args& args);
 size_t verify_tree_workspace_bytes(int32_t node_num, int32_t vocab);

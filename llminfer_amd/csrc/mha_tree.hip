@@ -3,8 +3,19 @@
 //   out[i][h] = sum_j w_j V[j][h/g] / sum_j w_j,   w_j = exp(q[i][h].K[j][h/g] / sqrt(128) - max),
 // over the cached positions 0..pos-1 and the nodes t (slots pos + t) that node i's 64-bit word names.
 //
-// A workgroup takes one node and one query head: sixteen rows of sixteen lanes, each a running softmax of its own over every
-// sixteenth key, merged at the end.
+// A KV head's nodes * g query rows are taken 32 to a wavefront, K and V read once per workgroup in tiles of 32 keys. Both products
+// run on the matrix cores in the transposed form, S^T = K Q^T and O^T = V^T P^T (v_mfma_f32_32x32x16_bf16): a lane then holds
+// 16 keys of one query row, so that maximum and sum of a row are folds inside a lane and one swap of the wavefront's halves, and the
+// probabilities are in the registers where the second product wants them:
+//   S^T  lane L: query row L%32, keys 8*(r/4) + 4*(L/32) + r%4 in register r = 0..15
+//   P^T  lane L: query row L%32; its eight values of step s (16 keys) are registers 8s..8s+7 of S^T, which fixes the order of the keys in
+//        that product: place 8*(L/32) + j is key 16s + 8*(j/4) + 4*(L/32) + j%4
+//   V^T  lane L: column 32*b + L%32 (b = 0..3), keys in that order: two transposing LDS reads (ds_read_b64_tr_b16), four keys each
+//   O^T  lane L: query row L%32, columns 32*b + 8*(r/4) + 4*(L/32) + r%4
+// Tiles lie in LDS as rows of 256 bytes, filled by LDS-DMA loads whose lanes fetch from where the swizzle wants it: K's 16-byte chunks are
+// exchanged by the row's low four bits, V's 64-byte quarters rotated by the row's low two, which spreads either read over the banks.
+//
+// Keys are split over workgroups; a second launch joins the splits.
 
 #include <hip/hip_runtime.h>
 #include <float.h>
@@ -16,6 +27,13 @@
 namespace llmi {
 namespace {
 
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kKeys = kTreeKeys;       // keys per tile
+constexpr int kTileBytes = 2 * kKeys * kHeadDim * 2;
+constexpr int kWaves = 4;
+constexpr int kSlots = 16;             // a lane's 64 accumulators of O^T as float4: slot 4*b + r/4
+
 struct TreeArgs {
     const uint16_t* q;          // [nodes][n_q][128]
     const uint16_t* k;          // layer base
@@ -24,73 +42,365 @@ struct TreeArgs {
     float* out_f32;             // optional
     const uint64_t* mask;       // optional
     const int32_t* pos_dev;     // optional
+    f32x4* part;                // [block][split][slot][lane]: a block is 32 query rows of a KV head
+    float2* part_ml;            // [block][split][32]: maximum (exp2 domain), sum
     int64_t row_stride;         // elements between positions of one KV head
     int64_t head_stride;        // elements between KV heads
-    int32_t pos, nodes, group, n_q;
+    int32_t pos, nodes, group, n_q, rows, blocks, splits;  // rows = nodes * group, blocks = per KV head
     float scale_log2e;          // log2(e) / sqrt(128)
 };
 
-constexpr int kStreams = 16;
+__device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
-__global__ __launch_bounds__(256) void mha_tree_kernel(TreeArgs a) {
-    __shared__ float part_o[kStreams][kHeadDim];
-    __shared__ float part_m[kStreams], part_l[kStreams];
-    const int hq = blockIdx.x, node = blockIdx.y;
-    const int kvh = hq / a.group;
-    const int stream = threadIdx.x >> 4, c = threadIdx.x & 15;
-    const int pos = a.pos_dev ? max(0, min(*a.pos_dev, a.pos)) : a.pos;
-    const uint64_t sees = a.mask ? a.mask[node] : ~0ull >> (63 - node);
-    const u32x4 q = reinterpret_cast<const u32x4*>(a.q + ((int64_t)node * a.n_q + hq) * kHeadDim)[c];
-    const uint16_t* kp = a.k + kvh * a.head_stride;
-    const uint16_t* vp = a.v + kvh * a.head_stride;
-    float m = -FLT_MAX, l = 0.0f, o[8] = {};  // (a finite maximum: scores of -inf get weight 0, not NaN)
-    for (int j = stream; j < pos + a.nodes; j += kStreams) {
-        if (j >= pos && !(sees >> (j - pos) & 1)) continue;
-        const u32x4 kv = reinterpret_cast<const u32x4*>(kp + j * a.row_stride)[c];
-        const u32x4 vv = reinterpret_cast<const u32x4*>(vp + j * a.row_stride)[c];
-        float s = dot8_bf16(kv, q, 0.0f);
-        s += dpp_partner<0xB1>(s);
-        s += dpp_partner<0x4E>(s);
-        s += dpp_partner<0x141>(s);
-        s += dpp_partner<0x140>(s);
-        s *= a.scale_log2e;
-        const float m_new = fmaxf(m, s);
-        const float alpha = fast_exp2(m - m_new), p = fast_exp2(s - m_new);
-        m = m_new;
-        l = l * alpha + p;
+__device__ __forceinline__ float halves_max(float x) {
+    const unsigned u = __builtin_bit_cast(unsigned, x);
+    const auto h = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const unsigned h0 = h[0], h1 = h[1];
+    return fmaxf(__builtin_bit_cast(float, h0), __builtin_bit_cast(float, h1));
+}
+
+// (scalar: everything that is the same for a workgroup's wavefronts derives from it)
+__device__ __forceinline__ int position(const TreeArgs& a) {
+    return __builtin_amdgcn_readfirstlane(a.pos_dev ? max(0, min(*a.pos_dev, a.pos)) : a.pos);
+}
+
+// A load's base in scalar registers, for long enough (see scalar_bases).
+__device__ __forceinline__ void scalar_base(const char*& p) { asm volatile("s_nop 4" : "+s"(p)); }
+
+// The bf16 values of a dword that are not finite.
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+    const uint32_t lo = (w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u, hi = (w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u;
+    return lo | hi;
+}
+// 1.0 where an element of `w`, one of `which`, counts as an infinity of the sign (NaN: of both).
+__device__ __forceinline__ uint32_t infinities(uint32_t w, uint32_t which, bool negative) {
+    const uint32_t flip = negative ? 0u : 0x80008000u;
+    const uint32_t lo = (w & 0x7fu) || ((w ^ flip) & 0x8000u) ? 0x3f80u : 0u;
+    const uint32_t hi = (w & 0x7f0000u) || ((w ^ flip) & 0x80000000u) ? 0x3f800000u : 0u;
+    return (lo | hi) & which;
+}
+
+// A finished row's four columns.
+__device__ __forceinline__ void write_out(const TreeArgs& a, int kvh, int row, int col, f32x4 o, float sum) {
+    if (row >= a.rows) return;
+    const float r = sum == 0.0f ? 0.0f : 1.0f / sum;  // (no key: zeros)
+    const int node = row / a.group;
+    const int64_t at = ((int64_t)node * a.n_q + kvh * a.group + (row - node * a.group)) * kHeadDim + col;
+    f32x4 y;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const uint32_t w = vv[e];
-            o[2 * e] = o[2 * e] * alpha + p * bf16_lo(w);
-            o[2 * e + 1] = o[2 * e + 1] * alpha + p * bf16_hi(w);
+    for (int e = 0; e < 4; ++e) y[e] = sum == 0.0f ? 0.0f : o[e] * r;
+    *reinterpret_cast<u32x2*>(a.out + at) = u32x2{pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3])};
+    if (a.out_f32) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a.out_f32[at + e] = y[e];
+    }
+}
+
+// WM wavefronts side by side on 32 query rows each, 4 / WM of them on a tile each of the same rows. EXACT: a probability enters the second
+// product as the sum of two bf16 numbers (relative error 2^-17), otherwise as one (2^-8).
+template <int WM, bool EXACT, int STAGES>
+__global__ __launch_bounds__(kWaves * 64, 2) void mha_tree_kernel(TreeArgs a) {
+    constexpr int WK = kWaves / WM;
+    constexpr int kStageBytes = WK * kTileBytes;
+    constexpr int kLoads = 16 / WM;  // 1 KiB blocks of a tile per wavefront: eight of K, eight of V
+    __shared__ __attribute__((aligned(1024))) char smem[STAGES * kStageBytes];
+    __shared__ float merge_m[kWaves][32], merge_l[kWaves][32];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave % WM, wk = wave / WM;
+    const int half = lane >> 5, n32 = lane & 31;
+    const int kvh = blockIdx.x, split = blockIdx.y;
+    const int block = blockIdx.z * WM + wm;  // of 32 query rows
+    const int row = block * 32 + n32;
+    const bool has_rows = block * 32 < a.rows;
+
+    const int pos = position(a);
+    const int keys = pos + a.nodes;
+    const int tiles = (keys + kKeys - 1) / kKeys;
+    const int run = __builtin_amdgcn_readfirstlane(tiles / a.splits), longer = tiles - run * a.splits;
+    const int t0 = split * run + min(split, longer), t1 = t0 + run + (split < longer ? 1 : 0);
+    const int iters = (t1 - t0 + WK - 1) / WK;
+
+    // The query rows (those behind the last one repeat it) and the nodes they see.
+    u32x4 q[8];
+    const int row_in = min(row, a.rows - 1);
+    const int node = row_in / a.group;
+    {
+        const u32x4* src = reinterpret_cast<const u32x4*>(a.q + ((int64_t)node * a.n_q + kvh * a.group + (row_in - node * a.group)) * kHeadDim);
+#pragma unroll
+        for (int s = 0; s < 8; ++s) q[s] = src[2 * s + half];
+    }
+    uint64_t sees = a.mask ? a.mask[node] : ~0ull >> (63 - node);
+    sees &= ~0ull >> (64 - a.nodes);
+
+    const uint32_t rs = (uint32_t)a.row_stride * 2u;
+    const char* kb = reinterpret_cast<const char*>(a.k + (int64_t)kvh * a.head_stride);
+    const char* vb = reinterpret_cast<const char*>(a.v + (int64_t)kvh * a.head_stride);
+    const int rho = lane >> 4, c16 = lane & 15;
+    const uint32_t v_col = (uint32_t)((((c16 >> 2) - rho) & 3) * 64 + (c16 & 3) * 16);
+    const uint32_t smem0 = (uint32_t)(uintptr_t)smem;
+
+    uint32_t k_off[4];  // (a block is four rows, and the low four bits of a row follow from the block's low two)
+#pragma unroll
+    for (int b = 0; b < 4; ++b) k_off[b] = (uint32_t)rho * rs + (uint32_t)((c16 ^ (4 * b + rho)) * 16);
+    const uint32_t v_off = (uint32_t)rho * rs + v_col;
+
+    auto issue = [&](int it, int stage) __attribute__((always_inline)) {
+        const int t = t0 + it * WK + wk;
+        if (t >= t1) return;
+        const char* kt = kb + (int64_t)t * kKeys * rs;
+        const char* vt = vb + (int64_t)t * kKeys * rs;
+        const int last = keys - 1 - t * kKeys;  // rows past the keys repeat the last one: seen by nobody
+        const uint32_t to = smem0 + (uint32_t)(stage * kStageBytes + wk * kTileBytes);
+        const bool whole = last >= kKeys - 1;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int b = wm * kLoads + i;  // (a wavefront of four has blocks of K or of V alone)
+            const bool is_k = WM == 4 ? wm < 2 : WM == 2 ? wm < 1 : i < 8;
+            const int b8 = b & 7;
+            const uint32_t lane_off = is_k ? k_off[i & 3] : v_off;
+            const char* base = is_k ? kt : vt;
+            const uint32_t ragged = (uint32_t)min(4 * b8 + rho, last) * rs + (lane_off - (uint32_t)rho * rs);
+            if (whole) base += (int64_t)(4 * b8) * rs;
+            scalar_base(base);
+            dma16(base, whole ? lane_off : ragged, to + (uint32_t)(b * 1024));
         }
-    }
+    };
+
+    const uint32_t k_x = (uint32_t)(half ^ (n32 & 15));  // chunk 2s + half of row n32 lies at chunk (2s) ^ k_x
+    const uint32_t k_row = (uint32_t)n32 * 256u;
+    const int i16 = lane & 15;
+    const uint32_t v_row = (uint32_t)((4 * half + (i16 >> 2)) * 256 + ((lane >> 4) & 1) * 32 + (i16 & 3) * 8);
+    float m_run = -FLT_MAX, l_run = 0.0f;  // (a finite maximum: scores of -inf get weight 0, not NaN)
+    f32x16 o[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) part_o[stream][8 * c + e] = o[e];
-    if (c == 0) {
-        part_m[stream] = m;
-        part_l[stream] = l;
+    for (int b = 0; b < 4; ++b) o[b] = f32x16{};
+
+    auto compute = [&](int t, int stage, auto with_nodes) __attribute__((always_inline)) {
+        constexpr bool masked = decltype(with_nodes)::value;
+        const char* kt = smem + stage * kStageBytes + wk * kTileBytes;
+        const char* vt = kt + kTileBytes / 2;
+        f32x16 c{};
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            const u32x4 kf = *reinterpret_cast<const u32x4*>(kt + k_row + (((uint32_t)(2 * s) ^ k_x) << 4));
+            c = mfma(__builtin_bit_cast(bf16x8, kf), __builtin_bit_cast(bf16x8, q[s]), c);
+        }
+        // Tiles with nodes in them: what a row does not see has no weight.
+        uint32_t vis = ~0u;  // bit o: the tile's key 4 * half + o
+        if constexpr (masked) {
+            const int at = t * kKeys + 4 * half - pos;
+            vis = at <= -32 ? ~0u : at >= 64 ? 0u : at >= 0 ? (uint32_t)(sees >> at) : (uint32_t)(sees << -at) | ((1u << -at) - 1u);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) c[r] = vis >> (8 * (r >> 2) + (r & 3)) & 1u ? c[r] : -INFINITY;
+        }
+        float top = c[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) top = fmaxf(top, c[r]);
+        top = halves_max(top) * a.scale_log2e;
+        // The accumulators are rescaled only where a row's maximum has grown by more than 2^8: up to that its weights are
+        // just larger than 1.
+        if (__any(top > m_run + 8.0f)) {
+            const float m_new = fmaxf(m_run, top);
+            const float alpha = fast_exp2(m_run - m_new);
+            m_run = m_new;
+            l_run *= alpha;
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[b][r] *= alpha;
+        }
+        float p[16];
+        float sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            p[r] = fast_exp2(__builtin_fmaf(c[r], a.scale_log2e, -m_run));
+            sum += p[r];
+        }
+        l_run += sum;
+        u32x4 ph[2], pl[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float x = p[8 * s + 2 * j], y = p[8 * s + 2 * j + 1];
+                const uint32_t w = pack_bf16(x, y);
+                ph[s][j] = w;
+                if constexpr (EXACT) pl[s][j] = pack_bf16(x - bf16_lo(w), y - bf16_hi(w));
+            }
+        auto v_frag = [&](int b, int s) __attribute__((always_inline)) {
+            const char* at = vt + v_row + (uint32_t)(((b + (i16 >> 2)) & 3) * 64) + s * 16 * 256;
+            typedef __attribute__((address_space(3))) i16x4* lds4;
+            const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)(uint32_t)(uintptr_t)at);
+            const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)(uint32_t)(uintptr_t)(at + 8 * 256));
+            const u32x2 xu = __builtin_bit_cast(u32x2, x), yu = __builtin_bit_cast(u32x2, y);
+            return u32x4{xu[0], xu[1], yu[0], yu[1]};
+        };
+        auto add = [&](int b, int s, u32x4 vf) __attribute__((always_inline)) {
+            o[b] = mfma(__builtin_bit_cast(bf16x8, vf), __builtin_bit_cast(bf16x8, ph[s]), o[b]);
+            if constexpr (EXACT) o[b] = mfma(__builtin_bit_cast(bf16x8, vf), __builtin_bit_cast(bf16x8, pl[s]), o[b]);
+        };
+        if constexpr (!masked) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) add(b, s, v_frag(b, s));
+        } else {
+            // A weight of 0 times an infinity or NaN would be NaN: values that are not finite enter as 0, and which rows see an
+            // infinity of either sign is counted by a product with 1 for each key seen (NaN counts as both).
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const u32x4 vf = v_frag(b, s);
+                    u32x4 bad;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) bad[j] = not_finite(vf[j]);
+                    if (__builtin_expect(__any((bad[0] | bad[1] | bad[2] | bad[3]) != 0u), 0)) {
+                        u32x4 seen, above, below, fine;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int r = 8 * s + 2 * j;
+                            seen[j] = (vis >> (8 * (r >> 2) + (r & 3)) & 1u ? 0x3f80u : 0u) | (vis >> (8 * (r >> 2) + (r & 3) + 1) & 1u ? 0x3f800000u : 0u);
+                            above[j] = infinities(vf[j], bad[j], false);
+                            below[j] = infinities(vf[j], bad[j], true);
+                            fine[j] = vf[j] & ~bad[j];
+                        }
+                        add(b, s, fine);
+                        const f32x16 up = mfma(__builtin_bit_cast(bf16x8, above), __builtin_bit_cast(bf16x8, seen), f32x16{});
+                        const f32x16 down = mfma(__builtin_bit_cast(bf16x8, below), __builtin_bit_cast(bf16x8, seen), f32x16{});
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            o[b][r] = up[r] > 0.0f ? o[b][r] + INFINITY : o[b][r];
+                            o[b][r] = down[r] > 0.0f ? o[b][r] - INFINITY : o[b][r];
+                        }
+                    } else {
+                        add(b, s, vf);
+                    }
+                }
+        }
+    };
+
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) issue(s, s);
+    // One stage: the oldest has landed (newer ones stay in flight), for every wavefront, and all have read the one that is refilled.
+    auto step = [&](int it, int stage, int refill, auto with_nodes) __attribute__((always_inline)) {
+        if (it + STAGES - 1 < iters) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * kLoads) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (it + STAGES - 1 < iters) issue(it + STAGES - 1, refill);
+        const int t = t0 + it * WK + wk;
+        if (has_rows && t < t1) compute(t, stage, with_nodes);
+    };
+    // Stages of cached positions alone, then those with nodes among their tiles.
+    const int cached = min(max((pos / kKeys - t0) / WK, 0), iters);
+    int it = 0, stage = 0;
+    for (; it + STAGES <= cached; it += STAGES)
+        static_for<0, STAGES>([&](auto s) __attribute__((always_inline)) { step(it + s.value, s.value, (s.value + STAGES - 1) % STAGES, std::false_type{}); });
+    static_for<0, STAGES - 1>([&](auto s) __attribute__((always_inline)) {
+        if (it < cached) {
+            step(it, s.value, (s.value + STAGES - 1) % STAGES, std::false_type{});
+            ++it;
+            stage = s.value + 1;
+        }
+    });
+#pragma unroll 1
+    for (; it < iters; ++it) {
+        step(it, stage, stage == 0 ? STAGES - 1 : stage - 1, std::true_type{});
+        stage = stage == STAGES - 1 ? 0 : stage + 1;
     }
-    __syncthreads();
-    const int d = threadIdx.x;
-    if (d >= kHeadDim) return;
-    float top = part_m[0];
-    for (int i = 1; i < kStreams; ++i) top = fmaxf(top, part_m[i]);
-    float sum = 0.0f, num = 0.0f;
-    for (int i = 0; i < kStreams; ++i) {
-        const float w = fast_exp2(part_m[i] - top);
-        sum += w * part_l[i];
-        num += w * part_o[i][d];
+
+    // Join the wavefronts of the same rows, each a part of the columns; then out, or to the workspace.
+    l_run = halves_sum(l_run);
+    f32x4 mine[kSlots / WK];
+    if constexpr (WK > 1) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        static_assert(kWaves * kSlots * 64 * 16 <= sizeof(smem), "the accumulators of all wavefronts fit the ring");
+        f32x4* parts = reinterpret_cast<f32x4*>(smem);
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4)
+                parts[(wave * kSlots + 4 * b + r4) * 64 + lane] = f32x4{o[b][4 * r4], o[b][4 * r4 + 1], o[b][4 * r4 + 2], o[b][4 * r4 + 3]};
+        if (half == 0) {
+            merge_m[wave][n32] = m_run;
+            merge_l[wave][n32] = l_run;
+        }
+        __syncthreads();
+        float m = -FLT_MAX, w[WK], sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < WK; ++i) m = fmaxf(m, merge_m[i * WM + wm][n32]);
+#pragma unroll
+        for (int i = 0; i < WK; ++i) {
+            w[i] = fast_exp2(merge_m[i * WM + wm][n32] - m);
+            sum += w[i] * merge_l[i * WM + wm][n32];
+        }
+#pragma unroll
+        for (int x = 0; x < kSlots / WK; ++x) {
+            mine[x] = f32x4{};
+#pragma unroll
+            for (int i = 0; i < WK; ++i) {
+                const f32x4 y = parts[((i * WM + wm) * kSlots + wk * (kSlots / WK) + x) * 64 + lane];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mine[x][e] += w[i] * y[e];
+            }
+        }
+        m_run = m;
+        l_run = sum;
+    } else {
+#pragma unroll
+        for (int x = 0; x < kSlots; ++x) mine[x] = f32x4{o[x >> 2][4 * (x & 3)], o[x >> 2][4 * (x & 3) + 1], o[x >> 2][4 * (x & 3) + 2], o[x >> 2][4 * (x & 3) + 3]};
     }
-    const float r = sum == 0.0f ? 0.0f : num / sum;  // (no key: zeros)
-    const int64_t at = ((int64_t)node * a.n_q + hq) * kHeadDim + d;
-    a.out[at] = f32_to_bf16(r);
-    if (a.out_f32) a.out_f32[at] = r;
+    if (!has_rows) return;
+    if (a.splits == 1) {
+#pragma unroll
+        for (int x = 0; x < kSlots / WK; ++x) {
+            const int slot = wk * (kSlots / WK) + x;
+            write_out(a, kvh, row, 32 * (slot >> 2) + 8 * (slot & 3) + 4 * half, mine[x], l_run);
+        }
+        return;
+    }
+    const int64_t at = (int64_t)(kvh * a.blocks + block) * a.splits + split;
+    if (t1 > t0) {
+#pragma unroll
+        for (int x = 0; x < kSlots / WK; ++x) a.part[(at * kSlots + wk * (kSlots / WK) + x) * 64 + lane] = mine[x];
+    }
+    // (a split without keys leaves no part: a maximum of -inf says so)
+    if (wk == 0 && half == 0) a.part_ml[at * 32 + n32] = t1 > t0 ? make_float2(m_run, l_run) : make_float2(-INFINITY, 0.0f);
+}
+
+// The splits of a block joined: a wavefront per slot.
+__global__ __launch_bounds__(256) void mha_tree_join_kernel(TreeArgs a) {
+    const int lane = threadIdx.x & 63;
+    const int slot = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int half = lane >> 5, n32 = lane & 31;
+    const int kvh = blockIdx.y / a.blocks, block = blockIdx.y - kvh * a.blocks;
+    const int64_t first = (int64_t)blockIdx.y * a.splits;
+    const float2* ml = a.part_ml + first * 32 + n32;
+    const f32x4* part = a.part + (first * kSlots + slot) * 64 + lane;
+    float m = -FLT_MAX;
+#pragma unroll 8
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[s * 32].x);
+    float sum = 0.0f;
+    f32x4 o{};
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s) {
+        const float2 x = ml[s * 32];
+        const f32x4 y = part[(int64_t)s * kSlots * 64];
+        const float w = fast_exp2(x.x - m);
+        sum += w * x.y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = w == 0.0f ? o[e] : o[e] + w * y[e];
+    }
+    write_out(a, kvh, block * 32 + n32, 32 * (slot >> 2) + 8 * (slot & 3) + 4 * half, o, sum);
 }
 
 }  // namespace
 
-int launch_mha_tree(const llmi_mha_tree_args& args, const llmi_mha_plan&) {
+int launch_mha_tree(const llmi_mha_tree_args& args, const llmi_mha_plan& plan) {
     const llmi_mha_args& m = args.mha;
     TreeArgs a;
     const int64_t layer = (int64_t)m.layer_id * m.max_seq_len * m.kv_dim;
@@ -108,8 +418,20 @@ int launch_mha_tree(const llmi_mha_tree_args& args, const llmi_mha_plan&) {
     a.nodes = args.node_num;
     a.group = m.kv_mul;
     a.n_q = m.head_num;
+    a.rows = args.node_num * m.kv_mul;
+    const int n_kv = m.kv_dim / kHeadDim, wm = plan.group_pad / 32;
+    a.blocks = (a.rows + 31) / 32;
+    a.splits = plan.num_splits;
+    a.part = static_cast<f32x4*>(m.workspace);
+    a.part_ml = reinterpret_cast<float2*>(a.part + (size_t)n_kv * a.blocks * a.splits * kSlots * 64);
     a.scale_log2e = 1.4426950408889634f / sqrtf((float)kHeadDim);
-    hipLaunchKernelGGL(mha_tree_kernel, dim3(m.head_num, args.node_num), dim3(256), 0, static_cast<hipStream_t>(m.stream), a);
+    const hipStream_t stream = static_cast<hipStream_t>(m.stream);
+    const dim3 grid(n_kv, a.splits, (a.blocks + wm - 1) / wm);
+    if (wm == 1) hipLaunchKernelGGL((mha_tree_kernel<1, true, 2>), grid, dim3(kWaves * 64), 0, stream, a);
+    else if (wm == 2) hipLaunchKernelGGL((mha_tree_kernel<2, true, 2>), grid, dim3(kWaves * 64), 0, stream, a);
+    else if (grid.z == 1) hipLaunchKernelGGL((mha_tree_kernel<4, true, 3>), grid, dim3(kWaves * 64), 0, stream, a);
+    else hipLaunchKernelGGL((mha_tree_kernel<4, false, 3>), grid, dim3(kWaves * 64), 0, stream, a);
+    if (a.splits > 1) hipLaunchKernelGGL(mha_tree_join_kernel, dim3(kSlots / 4, n_kv * a.blocks), dim3(256), 0, stream, a);
     return check_launch();
 }
 

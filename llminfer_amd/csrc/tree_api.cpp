@@ -25,14 +25,39 @@ int validate_tree(const llmi_mha_tree_args* a) {
     return LLMI_OK;
 }
 
+// Wavefronts of a workgroup that take query rows side by side, 32 each (the others of its four take other keys of the same rows).
+int tree_row_waves(int blocks) { return blocks <= 1 ? 1 : blocks <= 2 ? 2 : 4; }
+// Workgroups the splits aim for.
+int tree_groups(int wm) { return wm == 1 ? 256 : 512; }
+// Contexts of up to so many tiles run as one split: a second launch joins the others.
+constexpr int kTreeSingleTiles = 8;
+
 int make_tree_plan(const llmi_mha_tree_args* a, llmi_mha_plan* p) {
     if (int rc = validate_tree(a)) return rc;
+    const int n_kv = a->mha.kv_dim / a->mha.head_dim;
+    const int blocks = (a->node_num * a->mha.kv_mul + 31) / 32;
+    const int wm = tree_row_waves(blocks), rows_of_groups = (blocks + wm - 1) / wm;
+    const int tiles = (a->mha.pos + a->node_num + kTreeKeys - 1) / kTreeKeys;
+    const size_t per_split = (size_t)n_kv * blocks * kTreeSplitBytes;
+    const size_t room = a->mha.workspace ? a->mha.workspace_bytes / per_split : 0;
+    int splits = a->mha.num_splits;
+    if (splits == 0) {
+        splits = tiles <= kTreeSingleTiles ? 1 : std::max(1, tree_groups(wm) / (n_kv * rows_of_groups));
+        splits = std::min(splits, kMaxSplits);
+        if (splits > 1) splits = std::max(1, std::min(splits, tiles / (4 / wm)));
+        if ((size_t)splits > room) splits = (int)room;
+    } else {
+        splits = std::min(splits, tiles);
+        if (splits > 1 && (size_t)splits > room) return LLMI_ERR_WORKSPACE;
+    }
+    if (splits < 2) splits = 1;
     *p = llmi_mha_plan{};
-    p->path = LLMI_PATH_SINGLE_PASS;
-    p->num_splits = 1;
-    p->rows_per_split = a->mha.pos + a->node_num;
+    p->path = splits > 1 ? LLMI_PATH_SPLIT : LLMI_PATH_SINGLE_PASS;
+    p->num_splits = splits;
+    p->rows_per_split = (tiles + splits - 1) / splits * kTreeKeys;
     p->waves_per_group = 4;
-    p->group_pad = 1;
+    p->group_pad = 32 * wm;
+    p->workspace_needed = splits > 1 ? per_split * splits : 0;
     return LLMI_OK;
 }
 
@@ -56,7 +81,16 @@ int llmi_hip_mha_decode_tree(const llmi_mha_tree_args* args) {
 
 size_t llmi_hip_mha_tree_workspace_bytes(int32_t head_num, int32_t head_dim, int32_t node_num) {
     if (head_num <= 0 || head_dim <= 0 || node_num <= 0) return 0;
-    return 16;
+    if (node_num > LLMI_TREE_MAX_NODES) return 0;
+    // (how many KV heads share the query heads is not said: whatever needs most)
+    size_t most = 16;
+    for (int group = 1; group <= kMaxGroup; ++group) {
+        if (head_num % group != 0) continue;
+        const int n_kv = head_num / group, blocks = (node_num * group + 31) / 32, wm = tree_row_waves(blocks);
+        const int splits = std::min(tree_groups(wm) / (n_kv * ((blocks + wm - 1) / wm)), kMaxSplits);
+        if (splits > 1) most = std::max(most, (size_t)splits * n_kv * blocks * kTreeSplitBytes);
+    }
+    return most;
 }
 
 int llmi_hip_qk_norm_rope_append_tree(const llmi_qk_norm_rope_tree_args* a) {
