@@ -67,19 +67,6 @@ __device__ __forceinline__ int position(const TreeArgs& a) {
 // A load's base in scalar registers, for long enough (see scalar_bases).
 __device__ __forceinline__ void scalar_base(const char*& p) { asm volatile("s_nop 4" : "+s"(p)); }
 
-// The bf16 values of a dword that are not finite.
-__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
-    const uint32_t lo = (w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u, hi = (w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u;
-    return lo | hi;
-}
-// 1.0 where an element of `w`, one of `which`, counts as an infinity of the sign (NaN: of both).
-__device__ __forceinline__ uint32_t infinities(uint32_t w, uint32_t which, bool negative) {
-    const uint32_t flip = negative ? 0u : 0x80008000u;
-    const uint32_t lo = (w & 0x7fu) || ((w ^ flip) & 0x8000u) ? 0x3f80u : 0u;
-    const uint32_t hi = (w & 0x7f0000u) || ((w ^ flip) & 0x80000000u) ? 0x3f800000u : 0u;
-    return (lo | hi) & which;
-}
-
 // A finished row's four columns.
 __device__ __forceinline__ void write_out(const TreeArgs& a, int kvh, int row, int col, f32x4 o, float sum) {
     if (row >= a.rows) return;
@@ -176,6 +163,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void mha_tree_kernel(TreeArgs a) {
 #pragma unroll
     for (int b = 0; b < 4; ++b) o[b] = f32x16{};
 
+    uint32_t broken = 0u;  // bits 15 and 31: a value that is not finite among the nodes' tiles
     auto compute = [&](int t, int stage, auto with_nodes) __attribute__((always_inline)) {
         constexpr bool masked = decltype(with_nodes)::value;
         const char* kt = smem + stage * kStageBytes + wk * kTileBytes;
@@ -236,49 +224,25 @@ __global__ __launch_bounds__(kWaves * 64, 2) void mha_tree_kernel(TreeArgs a) {
             const u32x2 xu = __builtin_bit_cast(u32x2, x), yu = __builtin_bit_cast(u32x2, y);
             return u32x4{xu[0], xu[1], yu[0], yu[1]};
         };
-        auto add = [&](int b, int s, u32x4 vf) __attribute__((always_inline)) {
-            o[b] = mfma(__builtin_bit_cast(bf16x8, vf), __builtin_bit_cast(bf16x8, ph[s]), o[b]);
-            if constexpr (EXACT) o[b] = mfma(__builtin_bit_cast(bf16x8, vf), __builtin_bit_cast(bf16x8, pl[s]), o[b]);
-        };
-        if constexpr (!masked) {
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
+        for (int b = 0; b < 4; ++b)
 #pragma unroll
-                for (int s = 0; s < 2; ++s) add(b, s, v_frag(b, s));
-        } else {
-            // A weight of 0 times an infinity or NaN would be NaN: values that are not finite enter as 0, and which rows see an
-            // infinity of either sign is counted by a product with 1 for each key seen (NaN counts as both).
+            for (int s = 0; s < 2; ++s) {
+                u32x4 vf = v_frag(b, s);
+                if constexpr (masked) {
+                    // A weight of 0 times an infinity or NaN would be NaN: those enter as 0 here and are added at the end, for the rows that
+                    // see them. (An exponent of all ones carries into the sign's place.)
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    const u32x4 vf = v_frag(b, s);
-                    u32x4 bad;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) bad[j] = not_finite(vf[j]);
-                    if (__builtin_expect(__any((bad[0] | bad[1] | bad[2] | bad[3]) != 0u), 0)) {
-                        u32x4 seen, above, below, fine;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int r = 8 * s + 2 * j;
-                            seen[j] = (vis >> (8 * (r >> 2) + (r & 3)) & 1u ? 0x3f80u : 0u) | (vis >> (8 * (r >> 2) + (r & 3) + 1) & 1u ? 0x3f800000u : 0u);
-                            above[j] = infinities(vf[j], bad[j], false);
-                            below[j] = infinities(vf[j], bad[j], true);
-                            fine[j] = vf[j] & ~bad[j];
-                        }
-                        add(b, s, fine);
-                        const f32x16 up = mfma(__builtin_bit_cast(bf16x8, above), __builtin_bit_cast(bf16x8, seen), f32x16{});
-                        const f32x16 down = mfma(__builtin_bit_cast(bf16x8, below), __builtin_bit_cast(bf16x8, seen), f32x16{});
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            o[b][r] = up[r] > 0.0f ? o[b][r] + INFINITY : o[b][r];
-                            o[b][r] = down[r] > 0.0f ? o[b][r] - INFINITY : o[b][r];
-                        }
-                    } else {
-                        add(b, s, vf);
+                    for (int j = 0; j < 4; ++j) {
+                        typedef short i16x2 __attribute__((ext_vector_type(2)));
+                        const uint32_t carry = (vf[j] & 0x7f807f80u) + 0x00800080u;
+                        broken |= carry;
+                        vf[j] &= ~__builtin_bit_cast(uint32_t, __builtin_bit_cast(i16x2, carry) >> 15);
                     }
                 }
-        }
+                o[b] = mfma(__builtin_bit_cast(bf16x8, vf), __builtin_bit_cast(bf16x8, ph[s]), o[b]);
+                if constexpr (EXACT) o[b] = mfma(__builtin_bit_cast(bf16x8, vf), __builtin_bit_cast(bf16x8, pl[s]), o[b]);
+            }
     };
 
 #pragma unroll
@@ -309,6 +273,29 @@ __global__ __launch_bounds__(kWaves * 64, 2) void mha_tree_kernel(TreeArgs a) {
     for (; it < iters; ++it) {
         step(it, stage, stage == 0 ? STAGES - 1 : stage - 1, std::true_type{});
         stage = stage == STAGES - 1 ? 0 : stage + 1;
+    }
+
+    // Infinities and NaN among the values of nodes, for the rows that see them.
+    if (__builtin_expect(__any((broken & 0x80008000u) != 0u), 0)) {
+#pragma unroll 1
+        for (int n = 0; n < a.nodes; ++n) {
+            const int t = (pos + n) / kKeys;
+            if (t < t0 || t >= t1 || (t - t0) % WK != wk) continue;
+            const char* at = vb + (int64_t)(pos + n) * rs + 8 * half;
+            const bool seen = sees >> n & 1;
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int r4 = 0; r4 < 4; ++r4) {
+                    const u32x2 w = *reinterpret_cast<const u32x2*>(at + 64 * b + 16 * r4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t we = w[e >> 1];
+                        const float x = (e & 1) ? bf16_hi(we) : bf16_lo(we);
+                        if (seen && !(fabsf(x) < INFINITY)) o[b][4 * r4 + e] += x;
+                    }
+                }
+        }
     }
 
     // Join the wavefronts of the same rows, each a part of the columns; then out, or to the workspace.
@@ -372,30 +359,65 @@ __global__ __launch_bounds__(kWaves * 64, 2) void mha_tree_kernel(TreeArgs a) {
     if (wk == 0 && half == 0) a.part_ml[at * 32 + n32] = t1 > t0 ? make_float2(m_run, l_run) : make_float2(-INFINITY, 0.0f);
 }
 
-// The splits of a block joined: a wavefront per slot.
-__global__ __launch_bounds__(256) void mha_tree_join_kernel(TreeArgs a) {
-    const int lane = threadIdx.x & 63;
-    const int slot = blockIdx.x * 4 + (threadIdx.x >> 6);
+// The splits of a block joined: a workgroup per slot, its wavefronts on every fourth split, eight of them asked for at once.
+__global__ __launch_bounds__(kWaves * 64) void mha_tree_join_kernel(TreeArgs a) {
+    constexpr int kAhead = 8;
+    __shared__ f32x4 wave_o[kWaves][64];
+    __shared__ float wave_m[kWaves][64], wave_l[kWaves][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int kvh = blockIdx.x, slot = blockIdx.y, block = blockIdx.z;
     const int half = lane >> 5, n32 = lane & 31;
-    const int kvh = blockIdx.y / a.blocks, block = blockIdx.y - kvh * a.blocks;
-    const int64_t first = (int64_t)blockIdx.y * a.splits;
+    const int64_t first = (int64_t)(kvh * a.blocks + block) * a.splits;
     const float2* ml = a.part_ml + first * 32 + n32;
     const f32x4* part = a.part + (first * kSlots + slot) * 64 + lane;
-    float m = -FLT_MAX;
-#pragma unroll 8
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[s * 32].x);
-    float sum = 0.0f;
+    float m = -FLT_MAX, sum = 0.0f;
     f32x4 o{};
-#pragma unroll 4
-    for (int s = 0; s < a.splits; ++s) {
-        const float2 x = ml[s * 32];
-        const f32x4 y = part[(int64_t)s * kSlots * 64];
-        const float w = fast_exp2(x.x - m);
-        sum += w * x.y;
+    for (int s0 = wave; s0 < a.splits; s0 += kWaves * kAhead) {
+        float2 x[kAhead];
+        f32x4 y[kAhead];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = w == 0.0f ? o[e] : o[e] + w * y[e];
+        for (int i = 0; i < kAhead; ++i) {
+            const int s = min(s0 + kWaves * i, a.splits - 1);
+            x[i] = ml[s * 32];
+            y[i] = part[(int64_t)s * kSlots * 64];
+            if (s0 + kWaves * i >= a.splits) x[i] = make_float2(-INFINITY, 0.0f);
+        }
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) top = fmaxf(top, x[i].x);
+        const float before = fast_exp2(m - top);
+        m = top;
+        sum *= before;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] *= before;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const float w = fast_exp2(x[i].x - m);
+            sum += w * x[i].y;
+            // (a split without keys has left no part)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = w == 0.0f ? o[e] : o[e] + w * y[i][e];
+        }
     }
-    write_out(a, kvh, block * 32 + n32, 32 * (slot >> 2) + 8 * (slot & 3) + 4 * half, o, sum);
+    wave_o[wave][lane] = o;
+    wave_m[wave][lane] = m;
+    wave_l[wave][lane] = sum;
+    __syncthreads();
+    if (wave != 0) return;
+    float top = m;
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) top = fmaxf(top, wave_m[i][lane]);
+    f32x4 all{};
+    float total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        const float w = fast_exp2(wave_m[i][lane] - top);
+        const f32x4 y = wave_o[i][lane];
+        total += w * wave_l[i][lane];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) all[e] += w * y[e];
+    }
+    write_out(a, kvh, block * 32 + n32, 32 * (slot >> 2) + 8 * (slot & 3) + 4 * half, all, total);
 }
 
 }  // namespace
@@ -431,7 +453,7 @@ int launch_mha_tree(const llmi_mha_tree_args& args, const llmi_mha_plan& plan) {
     else if (wm == 2) hipLaunchKernelGGL((mha_tree_kernel<2, true, 2>), grid, dim3(kWaves * 64), 0, stream, a);
     else if (grid.z == 1) hipLaunchKernelGGL((mha_tree_kernel<4, true, 3>), grid, dim3(kWaves * 64), 0, stream, a);
     else hipLaunchKernelGGL((mha_tree_kernel<4, false, 3>), grid, dim3(kWaves * 64), 0, stream, a);
-    if (a.splits > 1) hipLaunchKernelGGL(mha_tree_join_kernel, dim3(kSlots / 4, n_kv * a.blocks), dim3(256), 0, stream, a);
+    if (a.splits > 1) hipLaunchKernelGGL(mha_tree_join_kernel, dim3(n_kv, kSlots, a.blocks), dim3(kWaves * 64), 0, stream, a);
     return check_launch();
 }
 
