@@ -164,19 +164,32 @@ __global__ __launch_bounds__(kWaves * 64, 2) void mha_tree_kernel(TreeArgs a) {
     for (int b = 0; b < 4; ++b) o[b] = f32x16{};
 
     uint32_t broken = 0u;  // bits 15 and 31: a value that is not finite among the nodes' tiles
-    auto compute = [&](int t, int stage, auto with_nodes) __attribute__((always_inline)) {
-        constexpr bool masked = decltype(with_nodes)::value;
+    auto compute = [&](int t, int stage) __attribute__((always_inline)) {
+        const bool masked = (t + 1) * kKeys > pos;
         const char* kt = smem + stage * kStageBytes + wk * kTileBytes;
         const char* vt = kt + kTileBytes / 2;
+        // (all of K's fragments are asked for before the first product waits for one; V's travel while the weights are formed)
+        u32x4 kf[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s) kf[s] = *reinterpret_cast<const u32x4*>(kt + k_row + (((uint32_t)(2 * s) ^ k_x) << 4));
+        asm volatile("" : "+v"(kf[0]), "+v"(kf[1]), "+v"(kf[2]), "+v"(kf[3]), "+v"(kf[4]), "+v"(kf[5]), "+v"(kf[6]), "+v"(kf[7]));
+        u32x2 vh[4][2][2];
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    typedef __attribute__((address_space(3))) i16x4* lds4;
+                    const char* at = vt + v_row + (uint32_t)(((b + (i16 >> 2)) & 3) * 64) + (s * 16 + x * 8) * 256;
+                    vh[b][s][x] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)(uint32_t)(uintptr_t)at));
+                }
         f32x16 c{};
 #pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            const u32x4 kf = *reinterpret_cast<const u32x4*>(kt + k_row + (((uint32_t)(2 * s) ^ k_x) << 4));
-            c = mfma(__builtin_bit_cast(bf16x8, kf), __builtin_bit_cast(bf16x8, q[s]), c);
-        }
+        for (int s = 0; s < 8; ++s) c = mfma(__builtin_bit_cast(bf16x8, kf[s]), __builtin_bit_cast(bf16x8, q[s]), c);
         // Tiles with nodes in them: what a row does not see has no weight.
         uint32_t vis = ~0u;  // bit o: the tile's key 4 * half + o
-        if constexpr (masked) {
+        if (masked) {
             const int at = t * kKeys + 4 * half - pos;
             vis = at <= -32 ? ~0u : at >= 64 ? 0u : at >= 0 ? (uint32_t)(sees >> at) : (uint32_t)(sees << -at) | ((1u << -at) - 1u);
 #pragma unroll
@@ -216,30 +229,27 @@ __global__ __launch_bounds__(kWaves * 64, 2) void mha_tree_kernel(TreeArgs a) {
                 ph[s][j] = w;
                 if constexpr (EXACT) pl[s][j] = pack_bf16(x - bf16_lo(w), y - bf16_hi(w));
             }
-        auto v_frag = [&](int b, int s) __attribute__((always_inline)) {
-            const char* at = vt + v_row + (uint32_t)(((b + (i16 >> 2)) & 3) * 64) + s * 16 * 256;
-            typedef __attribute__((address_space(3))) i16x4* lds4;
-            const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)(uint32_t)(uintptr_t)at);
-            const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)(uint32_t)(uintptr_t)(at + 8 * 256));
-            const u32x2 xu = __builtin_bit_cast(u32x2, x), yu = __builtin_bit_cast(u32x2, y);
-            return u32x4{xu[0], xu[1], yu[0], yu[1]};
-        };
+        if (masked) {
+            // A weight of 0 times an infinity or NaN would be NaN: those enter as 0 here and are added at the end, for the rows that
+            // see them. (An exponent of all ones carries into the sign's place.)
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        typedef short i16x2 __attribute__((ext_vector_type(2)));
+                        uint32_t w = vh[b][s][j >> 1][j & 1];
+                        const uint32_t carry = (w & 0x7f807f80u) + 0x00800080u;
+                        broken |= carry;
+                        vh[b][s][j >> 1][j & 1] = w & ~__builtin_bit_cast(uint32_t, __builtin_bit_cast(i16x2, carry) >> 15);
+                    }
+        }
 #pragma unroll
         for (int b = 0; b < 4; ++b)
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                u32x4 vf = v_frag(b, s);
-                if constexpr (masked) {
-                    // A weight of 0 times an infinity or NaN would be NaN: those enter as 0 here and are added at the end, for the rows that
-                    // see them. (An exponent of all ones carries into the sign's place.)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        typedef short i16x2 __attribute__((ext_vector_type(2)));
-                        const uint32_t carry = (vf[j] & 0x7f807f80u) + 0x00800080u;
-                        broken |= carry;
-                        vf[j] &= ~__builtin_bit_cast(uint32_t, __builtin_bit_cast(i16x2, carry) >> 15);
-                    }
-                }
+                const u32x4 vf = {vh[b][s][0][0], vh[b][s][0][1], vh[b][s][1][0], vh[b][s][1][1]};
                 o[b] = mfma(__builtin_bit_cast(bf16x8, vf), __builtin_bit_cast(bf16x8, ph[s]), o[b]);
                 if constexpr (EXACT) o[b] = mfma(__builtin_bit_cast(bf16x8, vf), __builtin_bit_cast(bf16x8, pl[s]), o[b]);
             }
@@ -247,31 +257,18 @@ __global__ __launch_bounds__(kWaves * 64, 2) void mha_tree_kernel(TreeArgs a) {
 
 #pragma unroll
     for (int s = 0; s < STAGES - 1; ++s) issue(s, s);
-    // One stage: the oldest has landed (newer ones stay in flight), for every wavefront, and all have read the one that is refilled.
-    auto step = [&](int it, int stage, int refill, auto with_nodes) __attribute__((always_inline)) {
+    // One stage after the other: the oldest has landed (newer ones stay in flight), for every wavefront, and all have read the one
+    // that is refilled.
+    int stage = 0;
+#pragma unroll 1
+    for (int it = 0; it < iters; ++it) {
         if (it + STAGES - 1 < iters) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * kLoads) : "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (it + STAGES - 1 < iters) issue(it + STAGES - 1, refill);
+        if (it + STAGES - 1 < iters) issue(it + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
         const int t = t0 + it * WK + wk;
-        if (has_rows && t < t1) compute(t, stage, with_nodes);
-    };
-    // Stages of cached positions alone, then those with nodes among their tiles.
-    const int cached = min(max((pos / kKeys - t0) / WK, 0), iters);
-    int it = 0, stage = 0;
-    for (; it + STAGES <= cached; it += STAGES)
-        static_for<0, STAGES>([&](auto s) __attribute__((always_inline)) { step(it + s.value, s.value, (s.value + STAGES - 1) % STAGES, std::false_type{}); });
-    static_for<0, STAGES - 1>([&](auto s) __attribute__((always_inline)) {
-        if (it < cached) {
-            step(it, s.value, (s.value + STAGES - 1) % STAGES, std::false_type{});
-            ++it;
-            stage = s.value + 1;
-        }
-    });
-#pragma unroll 1
-    for (; it < iters; ++it) {
-        step(it, stage, stage == 0 ? STAGES - 1 : stage - 1, std::true_type{});
+        if (has_rows && t < t1) compute(t, stage);
         stage = stage == STAGES - 1 ? 0 : stage + 1;
     }
 
