@@ -3,12 +3,14 @@
 // for what is accepted and drawn.
 //
 // Two launches. The first reads every row once, a workgroup per slice of 4096 tokens: maximum, its lowest index, sum of the weights
-// relative to the slice's maximum. The second joins the slices, decides the nodes on one wavefront (a node per lane, sets of nodes as
-// 64-bit words) and reads the last accepted node's row again for the token to draw.
+// relative to the slice's maximum. The second, sampling, has a workgroup per slice too: each joins the slices of all rows (a few lanes a row),
+// decides the nodes for itself on one wavefront (a node per lane, sets of nodes as 64-bit words), and sums what is left of
+// the last accepted node's row over its slice; the one that comes last finds the slice and the token. Greedy it is one workgroup, and the
+// row's maximum is the token.
 //
 // Weights are fp32: the exponent is formed as a pair (product and its rounding error, so that (x - m) / T is not rounded to 24
-// bits before the exponential), the exponential is the hardware's. Their sums are fp64: whichever of two neighbouring tokens a sum
-// falls on then depends on the weights' own rounding alone.
+// bits before the exponential), the exponential is the hardware's. A thread adds its sixteen weights of a slice in fp32, everything above that in
+// fp64: whichever of two neighbouring tokens a sum falls on then depends on the weights' own rounding alone.
 
 #include <hip/hip_runtime.h>
 #include <float.h>
@@ -20,8 +22,8 @@ namespace llmi {
 namespace {
 
 constexpr int kSlice = 4096;
-constexpr int kStatThreads = 256;
-constexpr int kWalkThreads = 1024;
+constexpr int kThreads = 256;
+constexpr int kEach = kSlice / kThreads;  // tokens of a slice per thread
 constexpr int kNodes = LLMI_TREE_MAX_NODES;
 
 struct Part {
@@ -41,6 +43,7 @@ struct VerifyArgs {
     int32_t* result;
     Part* parts;        // [rows][slices]: the target's rows, then the draft's
     double* left;       // [slices]: what is left of the last node's weights
+    uint32_t* arrived;  // workgroups of the second launch that have left their sum
     int32_t nodes, vocab, slices;
     float c_hi, c_lo;   // log2(e) / temperature, as a sum of two floats; 0: greedy
 };
@@ -49,6 +52,34 @@ struct VerifyArgs {
 __device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : fminf(x, FLT_MAX); }
 __device__ __forceinline__ float logit(const float* row, int64_t t) { return clean(row[t]); }
 __device__ __forceinline__ float logit(const uint16_t* row, int64_t t) { return clean(__builtin_bit_cast(float, (uint32_t)row[t] << 16)); }
+
+// A thread's tokens of a slice: chunks of 16 bytes (four or eight tokens), the workgroup's chunks side by side. Token e of thread i is
+// token place<T>(i, e) of the slice. Rows may start anywhere: the loads need no alignment.
+template <typename T>
+constexpr int kChunk = 16 / (int)sizeof(T);
+template <typename T>
+__device__ __forceinline__ int place(int thread, int e) {
+    return ((e / kChunk<T>)*kThreads + thread) * kChunk<T> + e % kChunk<T>;
+}
+template <typename T>
+__device__ __forceinline__ void load_slice(const T* row, int slice, int vocab, float (&v)[kEach]) {
+    struct __attribute__((packed, aligned(sizeof(T)))) Chunk {
+        T x[kChunk<T>];
+    };
+    const int64_t first = (int64_t)slice * kSlice;
+#pragma unroll
+    for (int c = 0; c < kEach / kChunk<T>; ++c) {
+        const int64_t t = first + place<T>((int)threadIdx.x, c * kChunk<T>);
+        if (t + kChunk<T> <= vocab) {
+            const Chunk x = *reinterpret_cast<const Chunk*>(row + t);
+#pragma unroll
+            for (int e = 0; e < kChunk<T>; ++e) v[c * kChunk<T> + e] = logit(x.x, e);
+        } else {
+#pragma unroll
+            for (int e = 0; e < kChunk<T>; ++e) v[c * kChunk<T> + e] = t + e < vocab ? logit(row, t + e) : -INFINITY;
+        }
+    }
+}
 
 // exp((x - m) / T). Below 2^-126 there is nothing left of a weight.
 __device__ __forceinline__ float weight(float x, float m, float c_hi, float c_lo) {
@@ -68,223 +99,319 @@ __device__ __forceinline__ Top better(Top a, Top b) {
     const bool b_wins = b.max > a.max || (b.max == a.max && (uint32_t)b.arg < (uint32_t)a.arg);  // (-1 is the highest)
     return b_wins ? b : a;
 }
-__device__ __forceinline__ Top wave_top(Top x) {
-    for (int s = 32; s; s >>= 1) x = better(x, Top{__shfl_xor(x.max, s), __shfl_xor(x.arg, s)});
+__device__ __forceinline__ Top lanes_top(Top x, int lanes) {
+    for (int s = lanes >> 1; s; s >>= 1) x = better(x, Top{__shfl_xor(x.max, s), __shfl_xor(x.arg, s)});
     return x;
 }
-__device__ __forceinline__ double wave_sum64(double x) {
-    for (int s = 32; s; s >>= 1) x += __shfl_xor(x, s);
+__device__ __forceinline__ double lanes_sum(double x, int lanes) {
+    for (int s = lanes >> 1; s; s >>= 1) x += __shfl_xor(x, s);
     return x;
+}
+template <typename V>
+__device__ __forceinline__ V lane_value(V x, int lane) {
+    if constexpr (sizeof(V) == 8) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, x);
+        const uint64_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = (uint32_t)__builtin_amdgcn_readlane((int)(u >> 32), lane);
+        return __builtin_bit_cast(V, hi << 32 | lo);
+    } else {
+        return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane));
+    }
 }
 
-template <typename T>
-__global__ __launch_bounds__(kStatThreads) void verify_stats_kernel(VerifyArgs a) {
-    __shared__ Top tops[kStatThreads / 64];
-    __shared__ double sums[kStatThreads / 64];
+template <typename T, bool GREEDY>
+__global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
+    __shared__ Top tops[kThreads / 64];
+    __shared__ double sums[kThreads / 64];
     const int slice = blockIdx.x, row = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const bool of_draft = row >= a.nodes;
     const T* x = static_cast<const T*>(of_draft ? a.draft : a.target) + (of_draft ? (row - a.nodes) * a.draft_stride : row * a.target_stride);
-    constexpr int kEach = kSlice / kStatThreads;
     float v[kEach];
-    Top top{-INFINITY, -1};
-    const int64_t first = (int64_t)slice * kSlice + threadIdx.x;
+    load_slice(x, slice, a.vocab, v);
+    if (slice == 0 && row == 0 && threadIdx.x == 0) *a.arrived = 0u;
+    float max = v[0];
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-        const int64_t t = first + e * kStatThreads;
-        v[e] = t < a.vocab ? logit(x, t) : -INFINITY;
-        if (v[e] > top.max) top = Top{v[e], (int32_t)t};
-    }
-    top = wave_top(top);
+    for (int e = 1; e < kEach; ++e) max = fmaxf(max, v[e]);
+    int arg = -1;
+#pragma unroll
+    for (int e = kEach - 1; e >= 0; --e) arg = v[e] == max ? e : arg;  // (places ascend with e)
+    Top top{max, max > -INFINITY ? slice * kSlice + place<T>((int)threadIdx.x, arg) : -1};
+    top = lanes_top(top, 64);
     if (lane == 0) tops[wave] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kStatThreads / 64; ++w) top = better(top, tops[w]);
+    for (int w = 0; w < kThreads / 64; ++w) top = better(top, tops[w]);
     double sum = 0.0;
+    if constexpr (!GREEDY) {
+        float s = 0.0f;
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) sum += weight(v[e], top.max, a.c_hi, a.c_lo);
-    sum = wave_sum64(sum);
-    if (lane == 0) sums[wave] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kStatThreads / 64; ++w) sum += sums[w];
-        a.parts[(int64_t)row * a.slices + slice] = Part{sum, top.max, top.arg};
+        for (int e = 0; e < kEach; ++e) s += weight(v[e], top.max, a.c_hi, a.c_lo);
+        sum = lanes_sum(s, 64);
+        if (lane == 0) sums[wave] = sum;
+        __syncthreads();
+        sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
     }
+    if (threadIdx.x == 0) a.parts[(int64_t)row * a.slices + slice] = Part{sum, top.max, top.arg};
 }
 
-// What is left of token t's weight at the last accepted node.
-struct Left {
-    float m_p, m_q;
-    double s_p, s_q;
-    bool subtract;           // max(p - q, 0)
-    int refused_n;
-    const int32_t* refused;  // tokens without weight
+// What the nodes' decision leaves for the token behind the path.
+struct Walk {
+    Top tops[2 * kNodes];
+    double sums[2 * kNodes];
+    int32_t refused[kNodes];
+    int32_t last, refused_n, count;
 };
-template <typename T>
-__device__ __forceinline__ double left_of(const VerifyArgs& a, const Left& f, const T* target, const T* draft, int64_t t) {
-    double w = weight(logit(target, t), f.m_p, a.c_hi, a.c_lo);
-    if (f.subtract) {
-        const double q = f.s_q > 0.0 ? weight(logit(draft, t), f.m_q, a.c_hi, a.c_lo) / f.s_q : 0.0;
-        w = fmax(w / f.s_p - q, 0.0);
-    }
-    for (int i = 0; i < f.refused_n; ++i)
-        if (f.refused[i] == (int32_t)t) w = 0.0;
-    return w;
-}
 
-// Sum over the lanes in front of this one.
-__device__ __forceinline__ double wave_before(double x, int lane) {
-    double s = x;
-    for (int d = 1; d < 64; d <<= 1) {
-        const double y = __shfl_up(s, d);
-        if (lane >= d) s += y;
-    }
-    const double b = __shfl_up(s, 1);
-    return lane ? b : 0.0;
-}
-
-template <typename T>
-__global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyArgs a) {
-    constexpr int kWaves = kWalkThreads / 64;
-    __shared__ Top tops[2 * kNodes];
-    __shared__ double sums[2 * kNodes];
-    __shared__ int32_t refused[kNodes];
-    __shared__ int32_t last_s, refused_s, slice_s;
-    __shared__ double target_s, before_s;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// All rows' slices joined, `lanes` lanes a row; then the nodes. `writes`: this workgroup writes the path.
+template <typename T, bool GREEDY>
+__device__ __forceinline__ void walk(const VerifyArgs& a, Walk& w, bool writes) {
     const int rows = a.draft ? 2 * a.nodes - 1 : a.nodes;
-    const bool greedy = a.c_hi == 0.0f;
-    for (int r = wave; r < rows; r += kWaves) {
-        const Part* parts = a.parts + (int64_t)r * a.slices;
+    int lanes = 64;
+    while (lanes * rows > kThreads) lanes >>= 1;
+    {
+        const int r = (int)threadIdx.x / lanes, l = (int)threadIdx.x % lanes;
+        const bool mine = r < rows;
+        const Part* parts = a.parts + (int64_t)(mine ? r : 0) * a.slices;
         Top top{-INFINITY, -1};
-        for (int s = lane; s < a.slices; s += 64) top = better(top, Top{parts[s].max, parts[s].arg});
-        top = wave_top(top);
+#pragma unroll 8
+        for (int s = l; s < a.slices; s += lanes) top = better(top, Top{parts[s].max, parts[s].arg});
+        top = lanes_top(top, lanes);
         double sum = 0.0;
-        for (int s = lane; s < a.slices; s += 64) sum += parts[s].sum * weight(parts[s].max, top.max, a.c_hi, a.c_lo);
-        sum = wave_sum64(sum);
-        if (lane == 0) {
-            tops[r] = top;
-            sums[r] = sum;
+        if constexpr (!GREEDY) {
+#pragma unroll 8
+            for (int s = l; s < a.slices; s += lanes) sum += parts[s].sum * weight(parts[s].max, top.max, a.c_hi, a.c_lo);
+            sum = lanes_sum(sum, lanes);
+        }
+        if (mine && l == 0) {
+            w.tops[r] = top;
+            w.sums[r] = sum;
         }
     }
     __syncthreads();
-    const T* target = static_cast<const T*>(a.target);
-    const T* draft = static_cast<const T*>(a.draft);
-    if (wave == 0) {
-        const int i = lane;
+    if (threadIdx.x < 64) {
+        const T* target = static_cast<const T*>(a.target);
+        const T* draft = static_cast<const T*>(a.draft);
+        const int i = threadIdx.x;
         const int parent = i == 0 || i >= a.nodes ? -1 : a.parents ? a.parents[i] : i - 1;
         const int token = i > 0 && i < a.nodes ? a.tokens[i] : -1;
         const bool valid = parent >= 0 && parent < i && token >= 0 && token < a.vocab;
         const int at = valid ? parent : 0;
+        const uint64_t valid_set = __ballot(valid);
         bool accept = false, again = false;
-        if (greedy) {
-            accept = valid && tops[at].arg == token;
+        if constexpr (GREEDY) {
+            accept = valid && w.tops[at].arg == token;
         } else {
             const double u = valid ? (double)a.uniform[i] : 0.0;
-            const double mass = valid ? (double)weight(logit(target + at * a.target_stride, token), tops[at].max, a.c_hi, a.c_lo) : 0.0;
+            const double mass = valid ? (double)weight(logit(target + at * a.target_stride, token), w.tops[at].max, a.c_hi, a.c_lo) : 0.0;
             if (a.draft) {
-                const double q = valid ? (double)weight(logit(draft + at * a.draft_stride, token), tops[a.nodes + at].max, a.c_hi, a.c_lo) : 0.0;
-                accept = mass > 0.0 && u * q * sums[at] < mass * (valid ? sums[a.nodes + at] : 0.0);
+                const double q = valid ? (double)weight(logit(draft + at * a.draft_stride, token), w.tops[a.nodes + at].max, a.c_hi, a.c_lo) : 0.0;
+                accept = mass > 0.0 && u * q * w.sums[at] < mass * (valid ? w.sums[a.nodes + at] : 0.0);
             } else {
                 // earlier siblings, one after the other: whether one has this token, then what they have taken away
-                // (every lane asks for lane j's values before any test: a lane that has left a test answers nobody)
-                for (int j = 1; j < a.nodes; ++j) {
-                    const int valid_j = __shfl((int)valid, j), parent_j = __shfl(parent, j), token_j = __shfl(token, j);
-                    again |= valid && valid_j && j < i && parent_j == parent && token_j == token;
+                if (a.parents) {
+                    for (uint64_t left = valid_set; left; left &= left - 1) {
+                        const int j = __ffsll((unsigned long long)left) - 1;
+                        again |= valid && j < i && lane_value(parent, j) == parent && lane_value(token, j) == token;
+                    }
                 }
                 double before = 0.0;
-                for (int j = 1; j < a.nodes; ++j) {
-                    const int first_j = __shfl((int)(valid && !again), j), parent_j = __shfl(parent, j);
-                    const double mass_j = __shfl(mass, j);
-                    if (valid && first_j && j < i && parent_j == parent) before += mass_j;
+                if (a.parents) {
+                    for (uint64_t left = __ballot(valid && !again); left; left &= left - 1) {
+                        const int j = __ffsll((unsigned long long)left) - 1;
+                        if (valid && j < i && lane_value(parent, j) == parent) before += lane_value(mass, j);
+                    }
                 }
-                accept = !again && mass > 0.0 && u * (sums[at] - before) < mass;
+                accept = valid && !again && mass > 0.0 && u * (w.sums[at] - before) < mass;
             }
         }
         // the first accepted child of each node, then those whose parents are on the path
-        uint64_t on = 1;
-        for (int j = 1; j < a.nodes; ++j) {
-            const int valid_j = __shfl((int)valid, j), parent_j = __shfl(parent, j), accept_j = __shfl((int)accept, j);
-            const int above = valid_j ? parent_j : -1;
-            const uint64_t earlier = __ballot(lane < j && lane > 0 && parent == above && accept);
-            if (above >= 0 && (on >> above & 1) && !earlier && accept_j) on |= 1ull << j;
+        bool first = accept;
+        const uint64_t accepted = __ballot(accept);
+        for (uint64_t left = accepted; left; left &= left - 1) {
+            const int j = __ffsll((unsigned long long)left) - 1;
+            first = first && !(j < i && lane_value(parent, j) == parent);
+        }
+        uint64_t on = 1, before = 0;
+        while (on != before) {  // (a step for each node of the path)
+            before = on;
+            on |= __ballot(first && (on >> at & 1));
         }
         const int count = __popcll(on), last = 63 - __clzll(on);
-        if (lane < a.nodes) {
-            if (on >> lane & 1) a.path[__popcll(on & ((1ull << lane) - 1))] = lane;
-            if (lane >= count) a.path[lane] = -1;
-        }
         const bool gone = valid && parent == last && !again;
         const uint64_t gone_set = a.draft ? 0ull : __ballot(gone);
-        if (!a.draft && gone) refused[__popcll(gone_set & ((1ull << lane) - 1))] = token;
-        if (lane == 0) {
-            last_s = last;
-            refused_s = __popcll(gone_set);
-            a.result[0] = count;
+        if (!a.draft && gone) w.refused[__popcll(gone_set & ((1ull << i) - 1))] = token;
+        if (i == 0) {
+            w.last = last;
+            w.count = count;
+            w.refused_n = __popcll(gone_set);
+        }
+        if (writes) {
+            if (on >> i & 1) a.path[__popcll(on & ((1ull << i) - 1))] = i;
+            if (i >= count && i < a.nodes) a.path[i] = -1;
+            if (i == 0) a.result[0] = count;
         }
     }
     __syncthreads();
-    const int last = last_s;
-    if (greedy || tops[last].arg < 0) {
-        if (threadIdx.x == 0) a.result[1] = tops[last].arg;
+}
+
+// What is left of a thread's weights at the last accepted node.
+template <typename T>
+__device__ __forceinline__ void left_of(const VerifyArgs& a, const Walk& w, int slice, float (&v)[kEach], double (&left)[kEach]) {
+    const int last = w.last;
+    const float m = w.tops[last].max;
+    load_slice(static_cast<const T*>(a.target) + last * a.target_stride, slice, a.vocab, v);
+    if (a.draft && last < a.nodes - 1) {
+        float q[kEach];
+        load_slice(static_cast<const T*>(a.draft) + last * a.draft_stride, slice, a.vocab, q);
+        const float m_q = w.tops[a.nodes + last].max;
+        const double p_1 = 1.0 / w.sums[last], q_1 = w.sums[a.nodes + last] > 0.0 ? 1.0 / w.sums[a.nodes + last] : 0.0;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e)
+            left[e] = fmax(weight(v[e], m, a.c_hi, a.c_lo) * p_1 - weight(q[e], m_q, a.c_hi, a.c_lo) * q_1, 0.0);
+    } else {
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) left[e] = weight(v[e], m, a.c_hi, a.c_lo);
+        for (int i = 0; i < w.refused_n; ++i) {
+            const int32_t t = w.refused[i] - slice * kSlice;
+            if (t < 0 || t >= kSlice) continue;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e)
+                if (place<T>((int)threadIdx.x, e) == t) left[e] = 0.0;
+        }
+    }
+}
+
+// Inclusive sum over the lanes up to this one.
+__device__ __forceinline__ double lanes_upto(double x, int lane) {
+    for (int d = 1; d < 64; d <<= 1) {
+        const double y = __shfl_up(x, d);
+        if (lane >= d) x += y;
+    }
+    return x;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void verify_greedy_kernel(VerifyArgs a) {
+    __shared__ Walk w;
+    walk<T, true>(a, w, true);
+    if (threadIdx.x == 0) a.result[1] = w.tops[w.last].arg;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs a) {
+    constexpr int kWaves = kThreads / 64, kChunks = kEach / kChunk<T>;
+    __shared__ Walk w;
+    __shared__ double sums[kChunks * kWaves], goal_s, before_s;
+    __shared__ int32_t last_one, slice_s, token_s, positive_s;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, slice = blockIdx.x;
+    walk<T, false>(a, w, slice == 0);
+    if (w.tops[w.last].arg < 0) {  // (no token has a weight)
+        if (slice == 0 && threadIdx.x == 0) a.result[1] = -1;
         return;
     }
-    const bool subtract = a.draft && last < a.nodes - 1;
-    const Left f{tops[last].max, subtract ? tops[a.nodes + last].max : 0.0f, sums[last], subtract ? sums[a.nodes + last] : 0.0, subtract, refused_s, refused};
-    target += last * a.target_stride;
-    if (subtract) draft += last * a.draft_stride;
-    // what is left in each slice: sixteen wavefronts, four tokens of 4096 per thread, side by side
-    for (int s = wave; s < a.slices; s += kWaves) {
-        double sum = 0.0;
-        for (int e = 0; e < kSlice / 64; ++e) {
-            const int64_t t = (int64_t)s * kSlice + e * 64 + lane;
-            if (t < a.vocab) sum += left_of(a, f, target, draft, t);
-        }
-        sum = wave_sum64(sum);
-        if (lane == 0) a.left[s] = sum;
-    }
+    float v[kEach];
+    double left[kEach];
+    left_of<T>(a, w, slice, v, left);
+    double sum = 0.0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) sum += left[e];
+    sum = lanes_sum(sum, 64);
+    if (lane == 0) sums[wave] = sum;
     __syncthreads();
     if (threadIdx.x == 0) {
+        sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+        __hip_atomic_store(&a.left[slice], sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last_one = __hip_atomic_fetch_add(a.arrived, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)a.slices - 1u;
+    }
+    __syncthreads();
+    if (!last_one) return;
+    // the slice: the first one where the sum passes the goal, or the last one with a weight
+    if (wave == 0) {
         double total = 0.0;
-        for (int s = 0; s < a.slices; ++s) total += a.left[s];
+        for (int s0 = 0; s0 < a.slices; s0 += 64) {
+            const double x = s0 + lane < a.slices ? __hip_atomic_load(&a.left[s0 + lane], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+            total = lane_value(total + lanes_upto(x, lane), 63);
+        }
         const double goal = (double)a.uniform[0] * total;
         double before = 0.0, found_before = 0.0;
         int found = -1;
-        for (int s = 0; s < a.slices; ++s) {
-            const double w = a.left[s];
-            if (w > 0.0) {
-                found = s;
-                found_before = before;
-                if (before + w > goal) break;
+        for (int s0 = 0; s0 < a.slices; s0 += 64) {
+            const double x = s0 + lane < a.slices ? __hip_atomic_load(&a.left[s0 + lane], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+            const double upto = before + lanes_upto(x, lane);
+            const uint64_t positive = __ballot(x > 0.0), passed = __ballot(x > 0.0 && upto > goal);
+            const int l = passed ? __ffsll((unsigned long long)passed) - 1 : 63 - __clzll(positive);
+            if (positive) {
+                found = s0 + l;
+                found_before = l ? lane_value(upto, l ? l - 1 : 0) : before;
             }
-            before += w;
+            if (passed) break;
+            before = lane_value(upto, 63);
         }
-        slice_s = found;
-        target_s = goal;
-        before_s = found_before;
+        if (lane == 0) {
+            slice_s = found;
+            goal_s = goal;
+            before_s = found_before;
+            token_s = INT32_MAX;
+            positive_s = -1;
+        }
     }
     __syncthreads();
-    if (slice_s < 0) {  // nothing is left
-        if (threadIdx.x == 0) a.result[1] = tops[last].arg;
+    const int found = slice_s;
+    if (found < 0) {  // nothing is left
+        if (threadIdx.x == 0) a.result[1] = w.tops[w.last].arg;
         return;
     }
-    // the token: the first one of the slice where the sum passes the goal, or the slice's last one with a weight
-    if (wave == 0) {
-        const double goal = target_s;
-        double before = before_s;
-        int token = -1;
-        for (int e = 0; e < kSlice / 64; ++e) {
-            const int64_t t = (int64_t)slice_s * kSlice + e * 64 + lane;
-            const double w = t < a.vocab ? left_of(a, f, target, draft, t) : 0.0;
-            const double upto = before + wave_before(w, lane) + w;
-            const uint64_t positive = __ballot(w > 0.0), passed = __ballot(w > 0.0 && upto > goal);
-            if (passed) {
-                token = slice_s * kSlice + e * 64 + __ffsll((unsigned long long)passed) - 1;
-                break;
+    // the token, in the same way: sums in front of each chunk of each thread, in the order of the tokens
+    left_of<T>(a, w, found, v, left);
+    double upto[kChunks], own[kChunks];
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+        own[c] = 0.0;
+#pragma unroll
+        for (int e = 0; e < kChunk<T>; ++e) own[c] += left[c * kChunk<T> + e];
+        upto[c] = lanes_upto(own[c], lane);
+        if (lane == 63) sums[c * kWaves + wave] = upto[c];
+    }
+    __syncthreads();
+    double before = before_s;
+    int token = INT32_MAX, positive = -1;  // (a thread's places ascend)
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+        for (int x = 0; x < kWaves; ++x) {
+            if (x == wave) {
+                double at = before + (upto[c] - own[c]);
+#pragma unroll
+                for (int e = 0; e < kChunk<T>; ++e) {
+                    const double y = left[c * kChunk<T> + e];
+                    const int t = place<T>((int)threadIdx.x, c * kChunk<T> + e);
+                    at += y;
+                    positive = y > 0.0 ? t : positive;
+                    if (y > 0.0 && at > goal_s) token = min(token, t);
+                }
             }
-            if (positive) token = slice_s * kSlice + e * 64 + 63 - __clzll(positive);
-            before = __shfl(upto, 63);
+            before += sums[c * kWaves + x];
         }
-        if (lane == 0) a.result[1] = token;
+    for (int s = 32; s; s >>= 1) {
+        token = min(token, __shfl_xor(token, s));
+        positive = max(positive, __shfl_xor(positive, s));
+    }
+    if (lane == 0) {
+        atomicMin(&token_s, token);
+        atomicMax(&positive_s, positive);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) a.result[1] = found * kSlice + (token_s != INT32_MAX ? token_s : positive_s);
+}
+
+template <typename T>
+void launch(const VerifyArgs& a, int rows, hipStream_t stream) {
+    const dim3 grid(a.slices, rows), block(kThreads);
+    if (a.c_hi == 0.0f) {
+        hipLaunchKernelGGL((verify_stats_kernel<T, true>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((verify_greedy_kernel<T>), dim3(1), block, 0, stream, a);
+    } else {
+        hipLaunchKernelGGL((verify_stats_kernel<T, false>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((verify_draw_kernel<T>), dim3(a.slices), block, 0, stream, a);
     }
 }
 
@@ -292,7 +419,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyArgs a)
 
 size_t verify_tree_workspace_bytes(int32_t node_num, int32_t vocab) {
     const size_t slices = ((size_t)vocab + kSlice - 1) / kSlice;
-    return slices * (2 * (size_t)node_num * sizeof(Part) + sizeof(double));
+    return slices * (2 * (size_t)node_num * sizeof(Part) + sizeof(double)) + 16;
 }
 
 int launch_verify_tree(const llmi_verify_tree_args& args) {
@@ -311,18 +438,14 @@ int launch_verify_tree(const llmi_verify_tree_args& args) {
     a.slices = (int32_t)(((int64_t)args.vocab + kSlice - 1) / kSlice);
     a.parts = static_cast<Part*>(args.workspace);
     a.left = reinterpret_cast<double*>(a.parts + (size_t)2 * a.nodes * a.slices);
+    a.arrived = reinterpret_cast<uint32_t*>(a.left + a.slices);
     const double c = args.temperature > 0.0f ? 1.4426950408889634 / (double)args.temperature : 0.0;
     a.c_hi = (float)c;
     a.c_lo = (float)(c - (double)a.c_hi);
-    const dim3 grid(a.slices, a.draft ? 2 * a.nodes - 1 : a.nodes);
+    const int rows = a.draft ? 2 * a.nodes - 1 : a.nodes;
     const hipStream_t stream = static_cast<hipStream_t>(args.stream);
-    if (args.logits_type == LLMI_LOGITS_F32) {
-        hipLaunchKernelGGL((verify_stats_kernel<float>), grid, dim3(kStatThreads), 0, stream, a);
-        hipLaunchKernelGGL((verify_walk_kernel<float>), dim3(1), dim3(kWalkThreads), 0, stream, a);
-    } else {
-        hipLaunchKernelGGL((verify_stats_kernel<uint16_t>), grid, dim3(kStatThreads), 0, stream, a);
-        hipLaunchKernelGGL((verify_walk_kernel<uint16_t>), dim3(1), dim3(kWalkThreads), 0, stream, a);
-    }
+    if (args.logits_type == LLMI_LOGITS_F32) launch<float>(a, rows, stream);
+    else launch<uint16_t>(a, rows, stream);
     return check_launch();
 }
 
