@@ -48,8 +48,8 @@ struct VerifyArgs {
     float c_hi, c_lo;   // log2(e) / temperature, as a sum of two floats; 0: greedy
 };
 
-// A logit as the definition takes it: NaN without weight, +inf the largest finite number.
-__device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : fminf(x, FLT_MAX); }
+// A logit as the definition takes it: NaN without weight (a maximum is the operand that is a number), +inf the largest finite number.
+__device__ __forceinline__ float clean(float x) { return fminf(fmaxf(x, -INFINITY), FLT_MAX); }
 __device__ __forceinline__ float logit(const float* row, int64_t t) { return clean(row[t]); }
 __device__ __forceinline__ float logit(const uint16_t* row, int64_t t) { return clean(__builtin_bit_cast(float, (uint32_t)row[t] << 16)); }
 
@@ -81,12 +81,11 @@ __device__ __forceinline__ void load_slice(const T* row, int slice, int vocab, f
     }
 }
 
-// exp((x - m) / T). Below 2^-126 there is nothing left of a weight.
+// exp((x - m) / T). (-inf, and NaN where there is no maximum, are far below: weight 0.)
 __device__ __forceinline__ float weight(float x, float m, float c_hi, float c_lo) {
-    const float d = x - m;
+    const float d = fmaxf(x - m, -1e30f);
     const float t = d * c_hi;
-    if (!(t >= -126.0f)) return 0.0f;  // (-inf and, with no maximum, NaN among them)
-    const float lo = __builtin_fmaf(d, c_hi, -t) + d * c_lo;
+    const float lo = __builtin_fmaf(d, c_lo, __builtin_fmaf(d, c_hi, -t));
     const float e = __builtin_amdgcn_exp2f(t);
     return __builtin_fmaf(e, lo * 0.69314718f, e);
 }
@@ -99,13 +98,46 @@ __device__ __forceinline__ Top better(Top a, Top b) {
     const bool b_wins = b.max > a.max || (b.max == a.max && (uint32_t)b.arg < (uint32_t)a.arg);  // (-1 is the highest)
     return b_wins ? b : a;
 }
-__device__ __forceinline__ Top lanes_top(Top x, int lanes) {
-    for (int s = lanes >> 1; s; s >>= 1) x = better(x, Top{__shfl_xor(x.max, s), __shfl_xor(x.arg, s)});
+
+// x of a lane's partner in step S of a fold: neighbours, pairs, fours, eights of a row of 16 lanes, rows, halves of the wavefront. After step S
+// all of 2^(S + 1) lanes that lie together have the fold.
+template <int S>
+__device__ __forceinline__ int partner(int x) {
+    constexpr int ctrl[4] = {0xB1, 0x4E, 0x141, 0x140};
+    if constexpr (S < 4) {
+        return __builtin_amdgcn_update_dpp(0, x, ctrl[S], 0xf, 0xf, false);
+    } else {
+        const bool upper = threadIdx.x & (S == 4 ? 16 : 32);
+        const auto h = S == 4 ? __builtin_amdgcn_permlane16_swap((unsigned)x, (unsigned)x, false, false)
+                              : __builtin_amdgcn_permlane32_swap((unsigned)x, (unsigned)x, false, false);
+        const unsigned h0 = h[0], h1 = h[1];  // (the lower halves' values, the upper halves')
+        return (int)(upper ? h0 : h1);
+    }
+}
+template <int S>
+__device__ __forceinline__ float partner(float x) { return __builtin_bit_cast(float, partner<S>(__builtin_bit_cast(int, x))); }
+template <int S>
+__device__ __forceinline__ double partner(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint64_t lo = (uint32_t)partner<S>((int)(uint32_t)u), hi = (uint32_t)partner<S>((int)(u >> 32));
+    return __builtin_bit_cast(double, hi << 32 | lo);
+}
+template <int S>
+__device__ __forceinline__ Top partner(Top x) { return Top{partner<S>(x.max), partner<S>(x.arg)}; }
+
+// Folds over groups of `lanes` lanes (a power of two, the same for all), the result in every lane.
+template <int S = 0, typename V, typename F>
+__device__ __forceinline__ V lanes_fold(V x, int lanes, F&& f) {
+    if constexpr (S < 6) {
+        if (lanes > 1 << S) return lanes_fold<S + 1>(f(x, partner<S>(x)), lanes, f);
+    }
     return x;
 }
+__device__ __forceinline__ Top lanes_top(Top x, int lanes) {
+    return lanes_fold(x, lanes, [](Top a, Top b) { return better(a, b); });
+}
 __device__ __forceinline__ double lanes_sum(double x, int lanes) {
-    for (int s = lanes >> 1; s; s >>= 1) x += __shfl_xor(x, s);
-    return x;
+    return lanes_fold(x, lanes, [](double a, double b) { return a + b; });
 }
 template <typename V>
 __device__ __forceinline__ V lane_value(V x, int lane) {
@@ -120,37 +152,45 @@ __device__ __forceinline__ V lane_value(V x, int lane) {
 
 template <typename T, bool GREEDY>
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
-    __shared__ Top tops[kThreads / 64];
+    __shared__ float tops[kThreads / 64];
     __shared__ double sums[kThreads / 64];
+    __shared__ uint32_t arg_s;
     const int slice = blockIdx.x, row = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const bool of_draft = row >= a.nodes;
     const T* x = static_cast<const T*>(of_draft ? a.draft : a.target) + (of_draft ? (row - a.nodes) * a.draft_stride : row * a.target_stride);
     float v[kEach];
     load_slice(x, slice, a.vocab, v);
-    if (slice == 0 && row == 0 && threadIdx.x == 0) *a.arrived = 0u;
-    float max = v[0];
+    if (threadIdx.x == 0) {
+        arg_s = ~0u;
+        if (slice == 0 && row == 0) *a.arrived = 0u;
+    }
+    float mine = v[0];
 #pragma unroll
-    for (int e = 1; e < kEach; ++e) max = fmaxf(max, v[e]);
-    int arg = -1;
-#pragma unroll
-    for (int e = kEach - 1; e >= 0; --e) arg = v[e] == max ? e : arg;  // (places ascend with e)
-    Top top{max, max > -INFINITY ? slice * kSlice + place<T>((int)threadIdx.x, arg) : -1};
-    top = lanes_top(top, 64);
-    if (lane == 0) tops[wave] = top;
+    for (int e = 1; e < kEach; ++e) mine = fmaxf(mine, v[e]);
+    float max = lanes_fold(mine, 64, [](float p, float q) { return fmaxf(p, q); });
+    if (lane == 0) tops[wave] = max;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kThreads / 64; ++w) top = better(top, tops[w]);
+    for (int w = 0; w < kThreads / 64; ++w) max = fmaxf(max, tops[w]);
+    if (mine == max && max > -INFINITY) {  // (the few threads that have it)
+        int arg = 0;
+#pragma unroll
+        for (int e = kEach - 1; e >= 0; --e) arg = v[e] == max ? place<T>((int)threadIdx.x, e) : arg;  // (places ascend with e)
+        atomicMin(&arg_s, (uint32_t)(slice * kSlice + arg));
+    }
     double sum = 0.0;
     if constexpr (!GREEDY) {
         float s = 0.0f;
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) s += weight(v[e], top.max, a.c_hi, a.c_lo);
+        for (int e = 0; e < kEach; ++e) s += weight(v[e], max, a.c_hi, a.c_lo);
         sum = lanes_sum(s, 64);
         if (lane == 0) sums[wave] = sum;
-        __syncthreads();
-        sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
     }
-    if (threadIdx.x == 0) a.parts[(int64_t)row * a.slices + slice] = Part{sum, top.max, top.arg};
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        if constexpr (!GREEDY) sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+        a.parts[(int64_t)row * a.slices + slice] = Part{sum, max, (int32_t)arg_s};
+    }
 }
 
 // What the nodes' decision leaves for the token behind the path.
@@ -158,6 +198,7 @@ struct Walk {
     Top tops[2 * kNodes];
     double sums[2 * kNodes];
     int32_t refused[kNodes];
+    uint32_t alike[kThreads / 64][kNodes];  // sixteen nodes each: same parent (low half), same token
     int32_t last, refused_n, count;
 };
 
@@ -167,69 +208,105 @@ __device__ __forceinline__ void walk(const VerifyArgs& a, Walk& w, bool writes) 
     const int rows = a.draft ? 2 * a.nodes - 1 : a.nodes;
     int lanes = 64;
     while (lanes * rows > kThreads) lanes >>= 1;
+    // What the nodes need is asked for ahead of the slices.
+    const T* target = static_cast<const T*>(a.target);
+    const T* draft = static_cast<const T*>(a.draft);
+    const int i = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int parent = -1, token = -1;
+    float u = 0.0f, x_p = -INFINITY, x_q = -INFINITY;
+    if (i > 0 && i < a.nodes) {
+        parent = a.parents ? a.parents[i] : i - 1;
+        token = a.tokens[i];
+    }
+    const bool valid = parent >= 0 && parent < i && token >= 0 && token < a.vocab;
+    const int at = valid ? parent : 0;
+    if constexpr (!GREEDY) {
+        if (valid && wave == 0) {
+            u = a.uniform[i];
+            x_p = logit(target + at * a.target_stride, token);
+            if (a.draft) x_q = logit(draft + at * a.draft_stride, token);
+        }
+    }
+    // Which nodes have this one's parent and which its token, sixteen nodes to a wavefront. (A loop over siblings on one wavefront, their
+    // values handed on one by one, took 10 us at 64 nodes.)
+    if (a.parents) {
+        const int key = valid ? parent : -1;
+        uint32_t alike = 0u;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            alike |= lane_value(key, 16 * wave + k) == key ? 1u << k : 0u;
+            if constexpr (!GREEDY) alike |= lane_value(token, 16 * wave + k) == token ? 0x10000u << k : 0u;
+        }
+        w.alike[wave][i] = alike;
+    }
     {
         const int r = (int)threadIdx.x / lanes, l = (int)threadIdx.x % lanes;
         const bool mine = r < rows;
         const Part* parts = a.parts + (int64_t)(mine ? r : 0) * a.slices;
+        // (sixteen slices at a time asked for together, the running maximum and sum of a softmax)
         Top top{-INFINITY, -1};
-#pragma unroll 8
-        for (int s = l; s < a.slices; s += lanes) top = better(top, Top{parts[s].max, parts[s].arg});
-        top = lanes_top(top, lanes);
         double sum = 0.0;
-        if constexpr (!GREEDY) {
-#pragma unroll 8
-            for (int s = l; s < a.slices; s += lanes) sum += parts[s].sum * weight(parts[s].max, top.max, a.c_hi, a.c_lo);
-            sum = lanes_sum(sum, lanes);
+        for (int s0 = l; s0 < a.slices; s0 += 16 * lanes) {
+            Part p[16];
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+                const int s = s0 + x * lanes;
+                p[x] = parts[min(s, a.slices - 1)];
+                if (s >= a.slices) p[x] = Part{0.0, -INFINITY, -1};
+            }
+            const float before = top.max;
+#pragma unroll
+            for (int x = 0; x < 16; ++x) top = better(top, Top{p[x].max, p[x].arg});
+            if constexpr (!GREEDY) {
+                sum *= weight(before, top.max, a.c_hi, a.c_lo);
+#pragma unroll
+                for (int x = 0; x < 16; ++x) sum += p[x].sum * weight(p[x].max, top.max, a.c_hi, a.c_lo);
+            }
         }
+        const float own = top.max;
+        top = lanes_top(top, lanes);
+        if constexpr (!GREEDY) sum = lanes_sum(sum * weight(own, top.max, a.c_hi, a.c_lo), lanes);
         if (mine && l == 0) {
             w.tops[r] = top;
             w.sums[r] = sum;
         }
     }
     __syncthreads();
-    if (threadIdx.x < 64) {
-        const T* target = static_cast<const T*>(a.target);
-        const T* draft = static_cast<const T*>(a.draft);
-        const int i = threadIdx.x;
-        const int parent = i == 0 || i >= a.nodes ? -1 : a.parents ? a.parents[i] : i - 1;
-        const int token = i > 0 && i < a.nodes ? a.tokens[i] : -1;
-        const bool valid = parent >= 0 && parent < i && token >= 0 && token < a.vocab;
-        const int at = valid ? parent : 0;
+    if (wave == 0) {
         const uint64_t valid_set = __ballot(valid);
+        uint64_t siblings = 0, equals = 0;
+        if (a.parents) {
+#pragma unroll
+            for (int x = 0; x < kThreads / 64; ++x) {
+                siblings |= (uint64_t)(w.alike[x][i] & 0xffffu) << 16 * x;
+                equals |= (uint64_t)(w.alike[x][i] >> 16) << 16 * x;
+            }
+            siblings &= valid ? valid_set & ((1ull << i) - 1) : 0ull;  // earlier ones
+        }
         bool accept = false, again = false;
         if constexpr (GREEDY) {
             accept = valid && w.tops[at].arg == token;
         } else {
-            const double u = valid ? (double)a.uniform[i] : 0.0;
-            const double mass = valid ? (double)weight(logit(target + at * a.target_stride, token), w.tops[at].max, a.c_hi, a.c_lo) : 0.0;
+            const double mass = valid ? (double)weight(x_p, w.tops[at].max, a.c_hi, a.c_lo) : 0.0;
             if (a.draft) {
-                const double q = valid ? (double)weight(logit(draft + at * a.draft_stride, token), w.tops[a.nodes + at].max, a.c_hi, a.c_lo) : 0.0;
-                accept = mass > 0.0 && u * q * w.sums[at] < mass * (valid ? w.sums[a.nodes + at] : 0.0);
+                const double q = valid ? (double)weight(x_q, w.tops[a.nodes + at].max, a.c_hi, a.c_lo) : 0.0;
+                accept = mass > 0.0 && (double)u * q * w.sums[at] < mass * (valid ? w.sums[a.nodes + at] : 0.0);
             } else {
-                // earlier siblings, one after the other: whether one has this token, then what they have taken away
-                if (a.parents) {
-                    for (uint64_t left = valid_set; left; left &= left - 1) {
-                        const int j = __ffsll((unsigned long long)left) - 1;
-                        again |= valid && j < i && lane_value(parent, j) == parent && lane_value(token, j) == token;
-                    }
-                }
+                // a token that has been refused is not tried again, and its mass is taken away once
+                again = valid && (siblings & equals);
+                uint64_t taken = valid ? siblings & __ballot(valid && !again) : 0ull;
                 double before = 0.0;
-                if (a.parents) {
-                    for (uint64_t left = __ballot(valid && !again); left; left &= left - 1) {
-                        const int j = __ffsll((unsigned long long)left) - 1;
-                        if (valid && j < i && lane_value(parent, j) == parent) before += lane_value(mass, j);
-                    }
+                while (__any(taken != 0)) {  // (in index order; every lane takes part in the hand-over)
+                    const int j = taken ? __ffsll((unsigned long long)taken) - 1 : 0;
+                    const double mass_j = __shfl(mass, j);
+                    before += taken ? mass_j : 0.0;
+                    taken &= taken - 1;
                 }
-                accept = valid && !again && mass > 0.0 && u * (w.sums[at] - before) < mass;
+                accept = valid && !again && mass > 0.0 && (double)u * (w.sums[at] - before) < mass;
             }
         }
         // the first accepted child of each node, then those whose parents are on the path
-        bool first = accept;
-        const uint64_t accepted = __ballot(accept);
-        for (uint64_t left = accepted; left; left &= left - 1) {
-            const int j = __ffsll((unsigned long long)left) - 1;
-            first = first && !(j < i && lane_value(parent, j) == parent);
-        }
+        const bool first = accept && !(siblings & __ballot(accept));
         uint64_t on = 1, before = 0;
         while (on != before) {  // (a step for each node of the path)
             before = on;
@@ -280,12 +357,21 @@ __device__ __forceinline__ void left_of(const VerifyArgs& a, const Walk& w, int 
     }
 }
 
-// Inclusive sum over the lanes up to this one.
-__device__ __forceinline__ double lanes_upto(double x, int lane) {
-    for (int d = 1; d < 64; d <<= 1) {
-        const double y = __shfl_up(x, d);
-        if (lane >= d) x += y;
-    }
+// Inclusive sum over the lanes up to this one: shifts inside the rows of 16 lanes, then the rows' last values handed on.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double moved(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint64_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, false);
+    const uint64_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(double, hi << 32 | lo);  // (lanes without a source: 0)
+}
+__device__ __forceinline__ double lanes_upto(double x) {
+    x += moved<0x111, 0xf>(x);
+    x += moved<0x112, 0xf>(x);
+    x += moved<0x114, 0xf>(x);
+    x += moved<0x118, 0xf>(x);
+    x += moved<0x142, 0xa>(x);  // lane 15 of rows 0 and 2 to rows 1 and 3
+    x += moved<0x143, 0xc>(x);  // lane 31 to rows 2 and 3
     return x;
 }
 
@@ -326,17 +412,16 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs a) {
     if (!last_one) return;
     // the slice: the first one where the sum passes the goal, or the last one with a weight
     if (wave == 0) {
-        double total = 0.0;
-        for (int s0 = 0; s0 < a.slices; s0 += 64) {
-            const double x = s0 + lane < a.slices ? __hip_atomic_load(&a.left[s0 + lane], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
-            total = lane_value(total + lanes_upto(x, lane), 63);
-        }
+        auto left_in = [&](int s) { return s < a.slices ? __hip_atomic_load(&a.left[s], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0; };
+        const double x0 = left_in(lane);
+        double total = lane_value(lanes_upto(x0), 63);
+        for (int s0 = 64; s0 < a.slices; s0 += 64) total = lane_value(total + lanes_upto(left_in(s0 + lane)), 63);
         const double goal = (double)a.uniform[0] * total;
         double before = 0.0, found_before = 0.0;
         int found = -1;
         for (int s0 = 0; s0 < a.slices; s0 += 64) {
-            const double x = s0 + lane < a.slices ? __hip_atomic_load(&a.left[s0 + lane], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
-            const double upto = before + lanes_upto(x, lane);
+            const double x = s0 ? left_in(s0 + lane) : x0;
+            const double upto = before + lanes_upto(x);
             const uint64_t positive = __ballot(x > 0.0), passed = __ballot(x > 0.0 && upto > goal);
             const int l = passed ? __ffsll((unsigned long long)passed) - 1 : 63 - __clzll(positive);
             if (positive) {
@@ -368,33 +453,31 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs a) {
         own[c] = 0.0;
 #pragma unroll
         for (int e = 0; e < kChunk<T>; ++e) own[c] += left[c * kChunk<T> + e];
-        upto[c] = lanes_upto(own[c], lane);
+        upto[c] = lanes_upto(own[c]);
         if (lane == 63) sums[c * kWaves + wave] = upto[c];
     }
     __syncthreads();
-    double before = before_s;
-    int token = INT32_MAX, positive = -1;  // (a thread's places ascend)
+    double at[kChunks], running = before_s;
 #pragma unroll
     for (int c = 0; c < kChunks; ++c)
 #pragma unroll
         for (int x = 0; x < kWaves; ++x) {
-            if (x == wave) {
-                double at = before + (upto[c] - own[c]);
-#pragma unroll
-                for (int e = 0; e < kChunk<T>; ++e) {
-                    const double y = left[c * kChunk<T> + e];
-                    const int t = place<T>((int)threadIdx.x, c * kChunk<T> + e);
-                    at += y;
-                    positive = y > 0.0 ? t : positive;
-                    if (y > 0.0 && at > goal_s) token = min(token, t);
-                }
-            }
-            before += sums[c * kWaves + x];
+            at[c] = x == wave ? running + (upto[c] - own[c]) : at[c];
+            running += sums[c * kWaves + x];
         }
-    for (int s = 32; s; s >>= 1) {
-        token = min(token, __shfl_xor(token, s));
-        positive = max(positive, __shfl_xor(positive, s));
-    }
+    int token = INT32_MAX, positive = -1;  // (a thread's places ascend)
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+        for (int e = 0; e < kChunk<T>; ++e) {
+            const double y = left[c * kChunk<T> + e];
+            const int t = place<T>((int)threadIdx.x, c * kChunk<T> + e);
+            at[c] += y;
+            positive = y > 0.0 ? t : positive;
+            token = y > 0.0 && at[c] > goal_s ? min(token, t) : token;
+        }
+    token = lanes_fold(token, 64, [](int p, int q) { return min(p, q); });
+    positive = lanes_fold(positive, 64, [](int p, int q) { return max(p, q); });
     if (lane == 0) {
         atomicMin(&token_s, token);
         atomicMax(&positive_s, positive);
