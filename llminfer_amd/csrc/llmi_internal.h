@@ -129,8 +129,18 @@ int launch_gemv(const void* input, const void* weight, void* const out[3], const
 // What every attention call asks of its arguments (c_api.cpp).
 int validate_mha(const llmi_mha_args* a);
 constexpr int kTreeKeys = 32;  // keys per tile of the tree attention
-// Bytes of workspace per split of a KV head's block of 32 query rows: 32 x 128 partial sums, 32 maxima and sums.
-constexpr size_t kTreeSplitBytes = 32 * (128 + 2) * sizeof(float);
+// How it takes the query rows (node x head) of a KV head: blocks of 16 or 32 rows, one to a wavefront, row_waves wavefronts of a
+// workgroup's four on different blocks (the others on other keys of the same).
+struct TreeForm {
+    int rows, blocks, row_waves;
+};
+inline TreeForm tree_form(int query_rows) {
+    if (query_rows <= 16) return {16, 1, 1};
+    const int blocks = (query_rows + 31) / 32;
+    return {32, blocks, blocks <= 1 ? 1 : blocks <= 2 ? 2 : 4};
+}
+// Bytes of workspace per block and split: partial sums, maxima and sums.
+inline size_t tree_split_bytes(const TreeForm& f) { return (size_t)f.rows * (128 + 2) * sizeof(float); }
 int launch_mha_tree(const llmi_mha_tree_args& args, const llmi_mha_plan& plan);
 int launch_qk_norm_rope_append_tree(const llmi_qk_norm_rope_tree_args& args);
 size_t verify_tree_workspace_bytes(int32_t node_num, int32_t vocab);

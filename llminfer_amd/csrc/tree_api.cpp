@@ -25,24 +25,22 @@ int validate_tree(const llmi_mha_tree_args* a) {
     return LLMI_OK;
 }
 
-// Wavefronts of a workgroup that take query rows side by side, 32 each (the others of its four take other keys of the same rows).
-int tree_row_waves(int blocks) { return blocks <= 1 ? 1 : blocks <= 2 ? 2 : 4; }
 // Workgroups the splits aim for.
-int tree_groups(int wm) { return wm == 1 ? 256 : 512; }
+int tree_groups(const TreeForm& f) { return f.row_waves == 1 ? 256 : 512; }
 // Contexts of up to so many tiles run as one split: a second launch joins the others.
 constexpr int kTreeSingleTiles = 8;
 
 int make_tree_plan(const llmi_mha_tree_args* a, llmi_mha_plan* p) {
     if (int rc = validate_tree(a)) return rc;
     const int n_kv = a->mha.kv_dim / a->mha.head_dim;
-    const int blocks = (a->node_num * a->mha.kv_mul + 31) / 32;
-    const int wm = tree_row_waves(blocks), rows_of_groups = (blocks + wm - 1) / wm;
+    const TreeForm form = tree_form(a->node_num * a->mha.kv_mul);
+    const int wm = form.row_waves, row_groups = (form.blocks + wm - 1) / wm;
     const int tiles = (a->mha.pos + a->node_num + kTreeKeys - 1) / kTreeKeys;
-    const size_t per_split = (size_t)n_kv * blocks * kTreeSplitBytes;
+    const size_t per_split = (size_t)n_kv * form.blocks * tree_split_bytes(form);
     const size_t room = a->mha.workspace ? a->mha.workspace_bytes / per_split : 0;
     int splits = a->mha.num_splits;
     if (splits == 0) {
-        splits = tiles <= kTreeSingleTiles ? 1 : std::max(1, tree_groups(wm) / (n_kv * rows_of_groups));
+        splits = tiles <= kTreeSingleTiles ? 1 : std::max(1, tree_groups(form) / (n_kv * row_groups));
         splits = std::min(splits, kMaxSplits);
         if (splits > 1) splits = std::max(1, std::min(splits, tiles / (4 / wm)));
         if ((size_t)splits > room) splits = (int)room;
@@ -56,7 +54,7 @@ int make_tree_plan(const llmi_mha_tree_args* a, llmi_mha_plan* p) {
     p->num_splits = splits;
     p->rows_per_split = (tiles + splits - 1) / splits * kTreeKeys;
     p->waves_per_group = 4;
-    p->group_pad = 32 * wm;
+    p->group_pad = form.rows * wm;
     p->workspace_needed = splits > 1 ? per_split * splits : 0;
     return LLMI_OK;
 }
@@ -86,9 +84,10 @@ size_t llmi_hip_mha_tree_workspace_bytes(int32_t head_num, int32_t head_dim, int
     size_t most = 16;
     for (int group = 1; group <= kMaxGroup; ++group) {
         if (head_num % group != 0) continue;
-        const int n_kv = head_num / group, blocks = (node_num * group + 31) / 32, wm = tree_row_waves(blocks);
-        const int splits = std::min(tree_groups(wm) / (n_kv * ((blocks + wm - 1) / wm)), kMaxSplits);
-        if (splits > 1) most = std::max(most, (size_t)splits * n_kv * blocks * kTreeSplitBytes);
+        const TreeForm form = tree_form(node_num * group);
+        const int n_kv = head_num / group, row_groups = (form.blocks + form.row_waves - 1) / form.row_waves;
+        const int splits = std::min(tree_groups(form) / (n_kv * row_groups), kMaxSplits);
+        if (splits > 1) most = std::max(most, (size_t)splits * n_kv * form.blocks * tree_split_bytes(form));
     }
     return most;
 }
