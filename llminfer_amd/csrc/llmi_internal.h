@@ -128,20 +128,16 @@ int launch_gemv(const void* input, const void* weight, void* const out[3], const
                 int32_t k, int32_t mode, hipStream_t stream);
 // What every attention call asks of its arguments (c_api.cpp).
 int validate_mha(const llmi_mha_args* a);
-constexpr int kTreeKeys = 32;  // keys per tile of the tree attention
-// How it takes the query rows (node x head) of a KV head: blocks of 16 or 32 rows, one to a wavefront, row_waves wavefronts of a
-// workgroup's four on different blocks (the others on other keys of the same).
+// How the tree attention takes a call (rules and measurements: tree_api.cpp): tiles of kTreeKeys keys, query rows (node x head) of a KV
+// head in blocks of 16 or 32, one to a wavefront, row_waves of a workgroup's four wavefronts on different blocks (the others on other keys of
+// the same), the keys dealt to `splits` workgroups.
+constexpr int kTreeKeys = 32;
 struct TreeForm {
-    int rows, blocks, row_waves;
+    int rows, blocks, row_waves, splits;
 };
-inline TreeForm tree_form(int query_rows) {
-    if (query_rows <= 16) return {16, 1, 1};
-    const int blocks = (query_rows + 31) / 32;
-    return {32, blocks, blocks <= 1 ? 1 : blocks <= 2 ? 2 : 4};
-}
-// Bytes of workspace per block and split: partial sums, maxima and sums.
+// Bytes of workspace per KV head, block and split: partial sums, maxima and sums.
 inline size_t tree_split_bytes(const TreeForm& f) { return (size_t)f.rows * (128 + 2) * sizeof(float); }
-int launch_mha_tree(const llmi_mha_tree_args& args, const llmi_mha_plan& plan);
+int launch_mha_tree(const llmi_mha_tree_args& args, const TreeForm& form);
 int launch_qk_norm_rope_append_tree(const llmi_qk_norm_rope_tree_args& args);
 size_t verify_tree_workspace_bytes(int32_t node_num, int32_t vocab);
 int launch_verify_tree(const llmi_verify_tree_args& args);

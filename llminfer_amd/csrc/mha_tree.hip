@@ -456,7 +456,7 @@ void launch(const TreeArgs& a, int n_kv, hipStream_t stream) {
 
 }  // namespace
 
-int launch_mha_tree(const llmi_mha_tree_args& args, const llmi_mha_plan& plan) {
+int launch_mha_tree(const llmi_mha_tree_args& args, const TreeForm& form) {
     const llmi_mha_args& m = args.mha;
     TreeArgs a;
     const int64_t layer = (int64_t)m.layer_id * m.max_seq_len * m.kv_dim;
@@ -476,9 +476,8 @@ int launch_mha_tree(const llmi_mha_tree_args& args, const llmi_mha_plan& plan) {
     a.n_q = m.head_num;
     a.rows = args.node_num * m.kv_mul;
     const int n_kv = m.kv_dim / kHeadDim;
-    const TreeForm form = tree_form(a.rows);
     a.blocks = form.blocks;
-    a.splits = plan.num_splits;
+    a.splits = form.splits;
     a.part = static_cast<f32x4*>(m.workspace);
     a.part_ml = reinterpret_cast<float2*>(a.part + (size_t)n_kv * a.blocks * a.splits * (form.rows / 2) * 64);
     a.scale_log2e = 1.4426950408889634f / sqrtf((float)kHeadDim);

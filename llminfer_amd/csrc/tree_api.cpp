@@ -25,38 +25,42 @@ int validate_tree(const llmi_mha_tree_args* a) {
     return LLMI_OK;
 }
 
-// Workgroups the splits aim for.
-int tree_groups(const TreeForm& f) { return f.row_waves == 1 ? 256 : 512; }
 // Contexts of up to so many tiles run as one split: a second launch joins the others.
-constexpr int kTreeSingleTiles = 8;
+constexpr int kSingleTiles = 8;
+constexpr int kSmallGroups = 1024;
 
-int make_tree_plan(const llmi_mha_tree_args* a, llmi_mha_plan* p) {
+// The rows' blocks. Sixteen rows where a KV head has no more, and up to a length that leaves each of the chip's 1024 SIMDs four tiles for
+// sixteen rows or fewer: short calls wait for a tile's arithmetic, which is half as long. us, 32 : 16 rows, 8 KV heads: 8 nodes of 32 heads 8.9 : 7.4 at 250
+// positions, 10.0 : 8.8 at 2000, 11.1 : 10.2 at 4099, 13.6 : 13.9 at 8192; 16 nodes 10.0 : 9.2 at 2000, 12.7 : 15.8 at 6000; 61 nodes 12.2 : 10.4
+// at 500, 12.5 : 13.5 at 1000.
+TreeForm tree_blocks(int rows, int n_kv, int64_t tiles) {
+    const int small = (rows + 15) / 16;
+    if (small == 1 || (int64_t)n_kv * small * ((tiles + 3) / 4) <= kSmallGroups) return {16, small, 1, 1};
+    const int blocks = (rows + 31) / 32;
+    return {32, blocks, blocks <= 1 ? 1 : blocks <= 2 ? 2 : 4, 1};
+}
+
+// Splits that a KV head's tiles are dealt to where nothing else limits them: a workgroup for each of 256 compute units, two from 64 tiles a
+// workgroup on (one : two, us: 26 nodes of 32 heads, 8 KV heads 16.1 : 19.8 at 6007 positions, 25.8 : 30.2 at 16000, 61 nodes 20.6 : 24.0 at 6000,
+// 62.7 : 60.2 at 32768, 64 nodes of 64 heads 451 : 358 at 131000: the parts of twice the splits have to be written and read).
+int tree_splits(const TreeForm& f, int n_kv, int64_t tiles) {
+    if (tiles <= kSingleTiles) return 1;
+    const int row_groups = (f.blocks + f.row_waves - 1) / f.row_waves;
+    const int groups = f.row_waves == 4 && tiles * n_kv * row_groups >= 256 * 64 ? 512 : 256;
+    const int64_t splits = std::min<int64_t>(std::min(groups / (n_kv * row_groups), kMaxSplits), tiles * f.row_waves / 4);
+    return splits < 2 ? 1 : (int)splits;
+}
+
+int make_form(const llmi_mha_tree_args* a, TreeForm* f) {
     if (int rc = validate_tree(a)) return rc;
-    const int n_kv = a->mha.kv_dim / a->mha.head_dim;
-    const TreeForm form = tree_form(a->node_num * a->mha.kv_mul);
-    const int wm = form.row_waves, row_groups = (form.blocks + wm - 1) / wm;
-    const int tiles = (a->mha.pos + a->node_num + kTreeKeys - 1) / kTreeKeys;
-    const size_t per_split = (size_t)n_kv * form.blocks * tree_split_bytes(form);
-    const size_t room = a->mha.workspace ? a->mha.workspace_bytes / per_split : 0;
-    int splits = a->mha.num_splits;
-    if (splits == 0) {
-        splits = tiles <= kTreeSingleTiles ? 1 : std::max(1, tree_groups(form) / (n_kv * row_groups));
-        splits = std::min(splits, kMaxSplits);
-        if (splits > 1) splits = std::max(1, std::min(splits, tiles / (4 / wm)));
-        if ((size_t)splits > room) splits = (int)room;
-    } else {
-        splits = std::min(splits, tiles);
-        if (splits > 1 && (size_t)splits > room) return LLMI_ERR_WORKSPACE;
-    }
-    if (splits < 2) splits = 1;
-    *p = llmi_mha_plan{};
-    p->path = splits > 1 ? LLMI_PATH_SPLIT : LLMI_PATH_SINGLE_PASS;
-    p->num_splits = splits;
-    p->rows_per_split = (tiles + splits - 1) / splits * kTreeKeys;
-    p->waves_per_group = 4;
-    p->group_pad = form.rows * wm;
-    p->workspace_needed = splits > 1 ? per_split * splits : 0;
-    return LLMI_OK;
+    const llmi_mha_args& m = a->mha;
+    const int n_kv = m.kv_dim / m.head_dim;
+    const int tiles = (m.pos + a->node_num + kTreeKeys - 1) / kTreeKeys;
+    *f = tree_blocks(a->node_num * m.kv_mul, n_kv, tiles);
+    const size_t room = m.workspace ? m.workspace_bytes / ((size_t)n_kv * f->blocks * tree_split_bytes(*f)) : 0;
+    f->splits = m.num_splits ? std::min(m.num_splits, tiles) : (int)std::min<size_t>(tree_splits(*f, n_kv, tiles), room);
+    if (f->splits < 2) f->splits = 1;
+    return f->splits > 1 && (size_t)f->splits > room ? LLMI_ERR_WORKSPACE : LLMI_OK;
 }
 
 }  // namespace
@@ -68,28 +72,37 @@ extern "C" {
 
 int llmi_hip_mha_tree_plan(const llmi_mha_tree_args* args, llmi_mha_plan* plan) {
     if (!plan) return LLMI_ERR_NULL_POINTER;
-    return make_tree_plan(args, plan);
+    TreeForm f;
+    if (int rc = make_form(args, &f)) return rc;
+    const int tiles = (args->mha.pos + args->node_num + kTreeKeys - 1) / kTreeKeys;
+    *plan = llmi_mha_plan{};
+    plan->path = f.splits > 1 ? LLMI_PATH_SPLIT : LLMI_PATH_SINGLE_PASS;
+    plan->num_splits = f.splits;
+    plan->rows_per_split = (tiles + f.splits - 1) / f.splits * kTreeKeys;
+    plan->waves_per_group = 4;
+    plan->group_pad = f.rows * f.row_waves;
+    plan->workspace_needed = f.splits > 1 ? (size_t)(args->mha.kv_dim / 128) * f.blocks * f.splits * tree_split_bytes(f) : 0;
+    return LLMI_OK;
 }
 
 int llmi_hip_mha_decode_tree(const llmi_mha_tree_args* args) {
-    llmi_mha_plan plan;
-    if (int rc = make_tree_plan(args, &plan)) return rc;
-    return launch_mha_tree(*args, plan);
+    TreeForm f;
+    if (int rc = make_form(args, &f)) return rc;
+    return launch_mha_tree(*args, f);
 }
 
 size_t llmi_hip_mha_tree_workspace_bytes(int32_t head_num, int32_t head_dim, int32_t node_num) {
-    if (head_num <= 0 || head_dim <= 0 || node_num <= 0) return 0;
-    if (node_num > LLMI_TREE_MAX_NODES) return 0;
-    // (how many KV heads share the query heads is not said: whatever needs most)
+    if (head_num <= 0 || head_dim <= 0 || node_num <= 0 || node_num > LLMI_TREE_MAX_NODES) return 0;
+    // (how many KV heads share the query heads is not said, nor the length: whatever needs most. Sixteen rows by length are bounded
+    // by the workgroups the rule allows them)
     size_t most = 16;
     for (int group = 1; group <= kMaxGroup; ++group) {
         if (head_num % group != 0) continue;
-        const TreeForm form = tree_form(node_num * group);
-        const int n_kv = head_num / group, row_groups = (form.blocks + form.row_waves - 1) / form.row_waves;
-        const int splits = std::min(tree_groups(form) / (n_kv * row_groups), kMaxSplits);
-        if (splits > 1) most = std::max(most, (size_t)splits * n_kv * form.blocks * tree_split_bytes(form));
+        const int n_kv = head_num / group;
+        const TreeForm f = tree_blocks(node_num * group, n_kv, INT32_MAX);
+        most = std::max(most, (size_t)tree_splits(f, n_kv, INT32_MAX) * n_kv * f.blocks * tree_split_bytes(f));
     }
-    return most;
+    return std::max(most, kSmallGroups * tree_split_bytes({16, 1, 1, 1}));
 }
 
 int llmi_hip_qk_norm_rope_append_tree(const llmi_qk_norm_rope_tree_args* a) {
