@@ -105,7 +105,6 @@ __global__ __launch_bounds__(kWaves * 64, ROWS == 32 && WM == 1 ? 1 : 2) void mh
     constexpr int kScores = ROWS / 2;    // a lane's keys of a tile
     constexpr int kSteps = 128 * ROWS / 512;  // fragments of a query row per lane
     constexpr int kS = kSlots<ROWS>;
-    static_assert(STAGES == 2 || WK == 1, "the wait for the oldest of several stages counts on a tile in each");
     __shared__ __attribute__((aligned(1024))) char smem[STAGES * kStageBytes];
     __shared__ float merge_m[kWaves][ROWS], merge_l[kWaves][ROWS];
     const int lane = threadIdx.x & 63;
@@ -189,21 +188,30 @@ __global__ __launch_bounds__(kWaves * 64, ROWS == 32 && WM == 1 ? 1 : 2) void mh
     for (int b = 0; b < kAccs; ++b) o[b] = Acc{};
 
     uint32_t broken = 0u;  // bits 15 and 31: a value that is not finite among the nodes' tiles
-    auto compute = [&](int t, int stage) __attribute__((always_inline)) {
-        constexpr int kFrags = 8;  // of K, 16 or 32 rows alike
-        const bool masked = (t + 1) * kKeys > pos;
+    constexpr int kV = kAccs * (ROWS == 32 ? 2 : 1);  // V fragments: step s of columns b
+    struct KFrags {
+        u32x4 f[8];
+    };
+    struct VFrags {
+        u32x2 f[kV][2];
+    };
+    struct Scores {
+        float c[kScores];
+    };
+    // (all of K's fragments are asked for before the first product waits for one)
+    auto read_k = [&](int stage) __attribute__((always_inline)) {
         const char* kt = smem + stage * kStageBytes + wk * kTileBytes;
-        const char* vt = kt + kTileBytes / 2;
-        // (all of K's fragments are asked for before the first product waits for one; V's travel while the weights are formed)
-        u32x4 kf[kFrags];
+        KFrags k;
 #pragma unroll
-        for (int x = 0; x < kFrags; ++x) {
+        for (int x = 0; x < 8; ++x) {
             const int s = x % kSteps, u = x / kSteps;  // (16 rows: the tile's upper sixteen keys behind the lower)
-            kf[x] = *reinterpret_cast<const u32x4*>(kt + k_row + u * 4096 + (((uint32_t)((64 / ROWS) * s) ^ k_x) << 4));
+            k.f[x] = *reinterpret_cast<const u32x4*>(kt + k_row + u * 4096 + (((uint32_t)((64 / ROWS) * s) ^ k_x) << 4));
         }
-        asm volatile("" : "+v"(kf[0]), "+v"(kf[1]), "+v"(kf[2]), "+v"(kf[3]), "+v"(kf[4]), "+v"(kf[5]), "+v"(kf[6]), "+v"(kf[7]));
-        constexpr int kV = kAccs * (ROWS == 32 ? 2 : 1);  // V fragments: step s of columns b
-        u32x2 vh[kV][2];
+        return k;
+    };
+    auto read_v = [&](int stage) __attribute__((always_inline)) {
+        const char* vt = smem + stage * kStageBytes + wk * kTileBytes + kTileBytes / 2;
+        VFrags v;
 #pragma unroll
         for (int f = 0; f < kV; ++f)
 #pragma unroll
@@ -211,25 +219,45 @@ __global__ __launch_bounds__(kWaves * 64, ROWS == 32 && WM == 1 ? 1 : 2) void mh
                 typedef __attribute__((address_space(3))) i16x4* lds4;
                 const int b = ROWS == 32 ? f >> 1 : f, key = ROWS == 32 ? 16 * (f & 1) + 8 * x : 16 * x;
                 const char* at = vt + v_row + (uint32_t)(((b * (ROWS / 16) + v_piece) & 7) * 32) + key * 256;
-                vh[f][x] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)(uint32_t)(uintptr_t)at));
+                v.f[f][x] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)(uint32_t)(uintptr_t)at));
             }
-        float c[kScores];
+        return v;
+    };
+    auto scores = [&](const KFrags& k) __attribute__((always_inline)) {
+        Scores y;
 #pragma unroll
         for (int u = 0; u < 8 / kSteps; ++u) {
             Acc x{};
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) x = mfma(__builtin_bit_cast(bf16x8, kf[u * kSteps + s]), __builtin_bit_cast(bf16x8, q[s]), x);
+            for (int s = 0; s < kSteps; ++s) x = mfma(__builtin_bit_cast(bf16x8, k.f[u * kSteps + s]), __builtin_bit_cast(bf16x8, q[s]), x);
 #pragma unroll
-            for (int r = 0; r < kAccSize; ++r) c[u * kAccSize + r] = x[r];
+            for (int r = 0; r < kAccSize; ++r) y.c[u * kAccSize + r] = x[r];
         }
+        return y;
+    };
+    // A tile's scores and values into the running softmax. NEXT: `k` are the next tile's keys, whose scores are formed between the
+    // exponentials of this one's and returned.
+    auto fold = [&](int t, Scores y, VFrags v, const KFrags& k, auto next) __attribute__((always_inline)) {
+        constexpr bool NEXT = decltype(next)::value;
+        auto& c = y.c;
         // Tiles with nodes in them: what a row does not see has no weight. Bit of `vis`: the key less 4 * kg.
-        uint32_t vis = ~0u;
-        auto bit_of = [](int r) { return ROWS == 32 ? 8 * (r >> 2) + (r & 3) : 16 * (r >> 2) + (r & 3); };
-        if (masked) {
+        if ((t + 1) * kKeys > pos) {
             const int at = t * kKeys + 4 * kg - pos;
-            vis = at <= -32 ? ~0u : at >= 64 ? 0u : at >= 0 ? (uint32_t)(sees >> at) : (uint32_t)(sees << -at) | ((1u << -at) - 1u);
+            const uint32_t vis = at <= -32 ? ~0u : at >= 64 ? 0u : at >= 0 ? (uint32_t)(sees >> at) : (uint32_t)(sees << -at) | ((1u << -at) - 1u);
 #pragma unroll
-            for (int r = 0; r < kScores; ++r) c[r] = vis >> bit_of(r) & 1u ? c[r] : -INFINITY;
+            for (int r = 0; r < kScores; ++r) c[r] = vis >> ((ROWS == 32 ? 8 : 16) * (r >> 2) + (r & 3)) & 1u ? c[r] : -INFINITY;
+            // A weight of 0 times an infinity or NaN would be NaN: those enter as 0 here and are added at the end, for the rows that
+            // see them. (An exponent of all ones carries into the sign's place.)
+#pragma unroll
+            for (int f = 0; f < kV; ++f)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    typedef short i16x2 __attribute__((ext_vector_type(2)));
+                    const uint32_t w = v.f[f][j >> 1][j & 1];
+                    const uint32_t carry = (w & 0x7f807f80u) + 0x00800080u;
+                    broken |= carry;
+                    v.f[f][j >> 1][j & 1] = w & ~__builtin_bit_cast(uint32_t, __builtin_bit_cast(i16x2, carry) >> 15);
+                }
         }
         float top = c[0];
 #pragma unroll
@@ -247,62 +275,85 @@ __global__ __launch_bounds__(kWaves * 64, ROWS == 32 && WM == 1 ? 1 : 2) void mh
 #pragma unroll
                 for (int r = 0; r < kAccSize; ++r) o[b][r] *= alpha;
         }
-        float p[kScores];
+        Scores y_next;
+        Acc x_next{};
         float sum = 0.0f;
-#pragma unroll
-        for (int r = 0; r < kScores; ++r) {
-            p[r] = fast_exp2(__builtin_fmaf(c[r], a.scale_log2e, -m_run));
-            sum += p[r];
-        }
-        l_run += sum;
         u32x4 ph[kScores / 8], pl[kScores / 8];
 #pragma unroll
-        for (int s = 0; s < kScores / 8; ++s)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float x = p[8 * s + 2 * j], y = p[8 * s + 2 * j + 1];
-                const uint32_t w = pack_bf16(x, y);
-                ph[s][j] = w;
-                if constexpr (EXACT) pl[s][j] = pack_bf16(x - bf16_lo(w), y - bf16_hi(w));
+        for (int s = 0; s < kScores / 2; ++s) {
+            if constexpr (NEXT) {
+                // (a product, then the vector instructions of two scores, which do not wait for it: in this order)
+                static_assert(!NEXT || ROWS == 32, "");
+                x_next = mfma(__builtin_bit_cast(bf16x8, k.f[s]), __builtin_bit_cast(bf16x8, q[s]), x_next);
             }
-        if (masked) {
-            // A weight of 0 times an infinity or NaN would be NaN: those enter as 0 here and are added at the end, for the rows that
-            // see them. (An exponent of all ones carries into the sign's place.)
+            const float p0 = fast_exp2(__builtin_fmaf(c[2 * s], a.scale_log2e, -m_run));
+            const float p1 = fast_exp2(__builtin_fmaf(c[2 * s + 1], a.scale_log2e, -m_run));
+            sum += p0 + p1;
+            const uint32_t w = pack_bf16(p0, p1);
+            ph[s >> 2][s & 3] = w;
+            if constexpr (EXACT) pl[s >> 2][s & 3] = pack_bf16(p0 - bf16_lo(w), p1 - bf16_hi(w));
+            if constexpr (NEXT) __builtin_amdgcn_sched_barrier(0);
+        }
+        l_run += sum;
+        if constexpr (NEXT) {
 #pragma unroll
-            for (int f = 0; f < kV; ++f)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    typedef short i16x2 __attribute__((ext_vector_type(2)));
-                    const uint32_t w = vh[f][j >> 1][j & 1];
-                    const uint32_t carry = (w & 0x7f807f80u) + 0x00800080u;
-                    broken |= carry;
-                    vh[f][j >> 1][j & 1] = w & ~__builtin_bit_cast(uint32_t, __builtin_bit_cast(i16x2, carry) >> 15);
-                }
+            for (int r = 0; r < kAccSize; ++r) y_next.c[r] = x_next[r];
         }
 #pragma unroll
         for (int f = 0; f < kV; ++f) {
             const int b = ROWS == 32 ? f >> 1 : f, s = ROWS == 32 ? f & 1 : 0;
-            const u32x4 vf = {vh[f][0][0], vh[f][0][1], vh[f][1][0], vh[f][1][1]};
+            const u32x4 vf = {v.f[f][0][0], v.f[f][0][1], v.f[f][1][0], v.f[f][1][1]};
             o[b] = mfma(__builtin_bit_cast(bf16x8, vf), __builtin_bit_cast(bf16x8, ph[s]), o[b]);
             if constexpr (EXACT) o[b] = mfma(__builtin_bit_cast(bf16x8, vf), __builtin_bit_cast(bf16x8, pl[s]), o[b]);
         }
+        return y_next;
+    };
+    const int my_tiles = t1 - t0 > wk ? (t1 - t0 - wk + WK - 1) / WK : 0;
+    // This wavefront's tile `it` has landed, up to `newer` ones behind it stay in flight; then every wavefront's, and all have read what is
+    // refilled next.
+    auto wait_for = [&](int it, int newer) __attribute__((always_inline)) {
+        newer = min(newer, my_tiles - 1 - it);
+        if (newer >= 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * kLoads) : "memory");
+        else if (newer == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kLoads) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
     };
 
 #pragma unroll
     for (int s = 0; s < STAGES - 1; ++s) issue(s, s);
-    // One stage after the other: the oldest has landed (newer ones stay in flight), for every wavefront, and all have read the one
-    // that is refilled.
-    int stage = 0;
+    if constexpr (STAGES == 4) {
+        // A tile's scores are formed an iteration ahead: matrix cores and vector ALU of one wavefront work side by side. In use are the next
+        // tile's keys and this one's values; one tile is in flight, one is asked for in the place of the tile before.
+        Scores y;
+        if (iters > 0) {
+            wait_for(0, 2);
+            y = scores(read_k(0));
+        }
 #pragma unroll 1
-    for (int it = 0; it < iters; ++it) {
-        if (it + STAGES - 1 < iters) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * kLoads) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (it + STAGES - 1 < iters) issue(it + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
-        const int t = t0 + it * WK + wk;
-        if (has_rows && t < t1) compute(t, stage);
-        stage = stage == STAGES - 1 ? 0 : stage + 1;
+        for (int it = 0; it < iters; ++it) {
+            if (it + 1 < iters) wait_for(it + 1, 1);
+            if (it + 3 < iters) issue(it + 3, (it + 3) & 3);
+            if (has_rows && it < my_tiles) {
+                const VFrags v = read_v(it & 3);
+                const KFrags k = read_k((it + 1) & 3);  // (behind the last tile: whatever lies there, not used)
+                y = fold(t0 + it * WK + wk, y, v, k, std::true_type{});
+            }
+        }
+    } else {
+        int stage = 0;
+#pragma unroll 1
+        for (int it = 0; it < iters; ++it) {
+            wait_for(it, 0);
+            if (it + 1 < iters) issue(it + 1, stage ^ 1);
+            if (has_rows && it < my_tiles) {
+                KFrags k = read_k(stage);
+                asm volatile("" : "+v"(k.f[0]), "+v"(k.f[1]), "+v"(k.f[2]), "+v"(k.f[3]), "+v"(k.f[4]), "+v"(k.f[5]), "+v"(k.f[6]), "+v"(k.f[7]));
+                const VFrags v = read_v(stage);
+                fold(t0 + it * WK + wk, scores(k), v, k, std::false_type{});
+            }
+            stage ^= 1;
+        }
     }
 
     // Infinities and NaN among the values of nodes, for the rows that see them.
@@ -484,9 +535,9 @@ int launch_mha_tree(const llmi_mha_tree_args& args, const TreeForm& form) {
     const hipStream_t stream = static_cast<hipStream_t>(m.stream);
     if (form.rows == 16) launch<16, 1, true, 2>(a, n_kv, stream);
     else if (form.row_waves == 1) launch<32, 1, true, 2>(a, n_kv, stream);
-    else if (form.row_waves == 2) launch<32, 2, true, 2>(a, n_kv, stream);
-    else if (form.blocks <= 4) launch<32, 4, true, 3>(a, n_kv, stream);
-    else launch<32, 4, false, 3>(a, n_kv, stream);
+    else if (form.row_waves == 2) launch<32, 2, true, 4>(a, n_kv, stream);
+    else if (form.blocks <= 4) launch<32, 4, true, 4>(a, n_kv, stream);
+    else launch<32, 4, false, 4>(a, n_kv, stream);
     return check_launch();
 }
 
