@@ -107,6 +107,7 @@ __global__ __launch_bounds__(kWaves * 64, ROWS == 32 && WM == 1 ? 1 : 2) void mh
     constexpr int kS = kSlots<ROWS>;
     __shared__ __attribute__((aligned(1024))) char smem[STAGES * kStageBytes];
     __shared__ float merge_m[kWaves][ROWS], merge_l[kWaves][ROWS];
+    __shared__ uint64_t sees_s[WM][ROWS];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave % WM, wk = wave / WM;
@@ -144,11 +145,19 @@ __global__ __launch_bounds__(kWaves * 64, ROWS == 32 && WM == 1 ? 1 : 2) void mh
     // Where a lane of a load fetches from: row rho of a block of four, the chunk that the swizzle wants at place i16 (a row's low bits
     // follow from the block's).
     const int rho = lane >> 4;
-    uint32_t k_off[4], v_off[2];
+    auto k_off = [&](int b) { return (uint32_t)rho * rs + (uint32_t)((i16 ^ (4 * (b & 3) + rho)) * 16); };
+    auto v_off = [&](int b) { return (uint32_t)rho * rs + (uint32_t)((((i16 >> 1) - (4 * (b & 1) + rho)) & 7) * 32 + (i16 & 1) * 16); };
+    // (several wavefronts share a tile's blocks: one has blocks of K or of V alone)
+    uint32_t lane_off[WM == 1 ? 8 : 4];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) k_off[b] = (uint32_t)rho * rs + (uint32_t)((i16 ^ (4 * b + rho)) * 16);
-#pragma unroll
-    for (int b = 0; b < 2; ++b) v_off[b] = (uint32_t)rho * rs + (uint32_t)((((i16 >> 1) - (4 * b + rho)) & 7) * 32 + (i16 & 1) * 16);
+    for (int b = 0; b < 4; ++b) {
+        if constexpr (WM == 1) {
+            lane_off[b] = k_off(b);
+            lane_off[4 + b] = v_off(b);
+        } else {
+            lane_off[b] = wm < WM / 2 ? k_off(b) : v_off(b);
+        }
+    }
 
     auto issue = [&](int it, int stage) __attribute__((always_inline)) {
         const int t = t0 + it * WK + wk;
@@ -160,10 +169,9 @@ __global__ __launch_bounds__(kWaves * 64, ROWS == 32 && WM == 1 ? 1 : 2) void mh
         auto load = [&](auto whole) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                const int b = wm * kLoads + i;  // (a wavefront of four has blocks of K or of V alone)
-                const bool is_k = WM == 4 ? wm < 2 : WM == 2 ? wm < 1 : i < 8;
-                const int b8 = b & 7;
-                uint32_t off = is_k ? k_off[i & 3] : v_off[i & 1];
+                const int b = wm * kLoads + i, b8 = b & 7;
+                const bool is_k = WM == 1 ? i < 8 : wm < WM / 2;
+                uint32_t off = lane_off[(i & 3) + (WM == 1 && i >= 8 ? 4 : 0)];
                 const char* base = is_k ? kt : vt;
                 if constexpr (decltype(whole)::value) base += (int64_t)(4 * b8) * rs;
                 else off += (uint32_t)(min(4 * b8 + rho, last) - rho) * rs;  // rows past the keys repeat the last one: seen by nobody
@@ -189,75 +197,70 @@ __global__ __launch_bounds__(kWaves * 64, ROWS == 32 && WM == 1 ? 1 : 2) void mh
 
     uint32_t broken = 0u;  // bits 15 and 31: a value that is not finite among the nodes' tiles
     constexpr int kV = kAccs * (ROWS == 32 ? 2 : 1);  // V fragments: step s of columns b
-    struct KFrags {
-        u32x4 f[8];
-    };
-    struct VFrags {
-        u32x2 f[kV][2];
+    typedef __attribute__((address_space(3))) char LdsChar;
+    typedef __attribute__((address_space(3))) i16x4 LdsVec;
+    const LdsChar* ring = (const LdsChar*)smem + wk * kTileBytes;
+    struct VFrag {
+        u32x2 half[2];
     };
     struct Scores {
         float c[kScores];
     };
-    // (all of K's fragments are asked for before the first product waits for one)
-    auto read_k = [&](int stage) __attribute__((always_inline)) {
-        const char* kt = smem + stage * kStageBytes + wk * kTileBytes;
-        KFrags k;
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-            const int s = x % kSteps, u = x / kSteps;  // (16 rows: the tile's upper sixteen keys behind the lower)
-            k.f[x] = *reinterpret_cast<const u32x4*>(kt + k_row + u * 4096 + (((uint32_t)((64 / ROWS) * s) ^ k_x) << 4));
-        }
-        return k;
+    auto k_frag = [&](int stage, int x) __attribute__((always_inline)) {
+        const int s = x % kSteps, u = x / kSteps;  // (16 rows: the tile's upper sixteen keys behind the lower)
+        const LdsChar* at = ring + k_row + (((uint32_t)((64 / ROWS) * s) ^ k_x) << 4);
+        return *(const __attribute__((address_space(3))) u32x4*)(at + (stage * kStageBytes + u * 4096));
     };
-    auto read_v = [&](int stage) __attribute__((always_inline)) {
-        const char* vt = smem + stage * kStageBytes + wk * kTileBytes + kTileBytes / 2;
-        VFrags v;
+    auto v_frag = [&](int stage, int f) __attribute__((always_inline)) {
+        const int b = ROWS == 32 ? f >> 1 : f;
+        const LdsChar* at = ring + v_row + (uint32_t)(((b * (ROWS / 16) + v_piece) & 7) * 32);  // (the rest: a constant of the instruction)
+        VFrag v;
 #pragma unroll
-        for (int f = 0; f < kV; ++f)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                typedef __attribute__((address_space(3))) i16x4* lds4;
-                const int b = ROWS == 32 ? f >> 1 : f, key = ROWS == 32 ? 16 * (f & 1) + 8 * x : 16 * x;
-                const char* at = vt + v_row + (uint32_t)(((b * (ROWS / 16) + v_piece) & 7) * 32) + key * 256;
-                v.f[f][x] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)(uint32_t)(uintptr_t)at));
-            }
+        for (int x = 0; x < 2; ++x) {
+            const int key = ROWS == 32 ? 16 * (f & 1) + 8 * x : 16 * x;
+            v.half[x] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsVec*)(at + (stage * kStageBytes + kTileBytes / 2 + key * 256))));
+        }
         return v;
     };
-    auto scores = [&](const KFrags& k) __attribute__((always_inline)) {
+    auto scores = [&](int stage) __attribute__((always_inline)) {
+        // (all of K's fragments are asked for before the first product waits for one)
+        u32x4 k[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) k[x] = k_frag(stage, x);
+        asm volatile("" : "+v"(k[0]), "+v"(k[1]), "+v"(k[2]), "+v"(k[3]), "+v"(k[4]), "+v"(k[5]), "+v"(k[6]), "+v"(k[7]));
         Scores y;
 #pragma unroll
         for (int u = 0; u < 8 / kSteps; ++u) {
             Acc x{};
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) x = mfma(__builtin_bit_cast(bf16x8, k.f[u * kSteps + s]), __builtin_bit_cast(bf16x8, q[s]), x);
+            for (int s = 0; s < kSteps; ++s) x = mfma(__builtin_bit_cast(bf16x8, k[u * kSteps + s]), __builtin_bit_cast(bf16x8, q[s]), x);
 #pragma unroll
             for (int r = 0; r < kAccSize; ++r) y.c[u * kAccSize + r] = x[r];
         }
         return y;
     };
-    // A tile's scores and values into the running softmax. NEXT: `k` are the next tile's keys, whose scores are formed between the
-    // exponentials of this one's and returned.
-    auto fold = [&](int t, Scores y, VFrags v, const KFrags& k, auto next) __attribute__((always_inline)) {
-        constexpr bool NEXT = decltype(next)::value;
+    // A tile's scores and values (at `stage`) into the running softmax. NEXT: the next tile's keys are at `ahead`; its scores are formed
+    // between the exponentials of this one's and returned. CACHED: the tile has no nodes.
+    auto fold = [&](int t, Scores y, int stage, int ahead, auto next, auto cached) __attribute__((always_inline)) {
+        constexpr bool NEXT = decltype(next)::value, CACHED = decltype(cached)::value;
+        static_assert(!NEXT || ROWS == 32, "");
         auto& c = y.c;
+        VFrag v[kV];
+        u32x4 k[8];
+        if constexpr (NEXT) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) k[x] = k_frag(ahead, x);
+        } else {
+#pragma unroll
+            for (int f = 0; f < kV; ++f) v[f] = v_frag(stage, f);
+        }
         // Tiles with nodes in them: what a row does not see has no weight. Bit of `vis`: the key less 4 * kg.
-        if ((t + 1) * kKeys > pos) {
+        const bool nodes = !CACHED && (t + 1) * kKeys > pos;
+        if (nodes) {
             const int at = t * kKeys + 4 * kg - pos;
             const uint32_t vis = at <= -32 ? ~0u : at >= 64 ? 0u : at >= 0 ? (uint32_t)(sees >> at) : (uint32_t)(sees << -at) | ((1u << -at) - 1u);
 #pragma unroll
             for (int r = 0; r < kScores; ++r) c[r] = vis >> ((ROWS == 32 ? 8 : 16) * (r >> 2) + (r & 3)) & 1u ? c[r] : -INFINITY;
-            // A weight of 0 times an infinity or NaN would be NaN: those enter as 0 here and are added at the end, for the rows that
-            // see them. (An exponent of all ones carries into the sign's place.)
-#pragma unroll
-            for (int f = 0; f < kV; ++f)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    typedef short i16x2 __attribute__((ext_vector_type(2)));
-                    const uint32_t w = v.f[f][j >> 1][j & 1];
-                    const uint32_t carry = (w & 0x7f807f80u) + 0x00800080u;
-                    broken |= carry;
-                    v.f[f][j >> 1][j & 1] = w & ~__builtin_bit_cast(uint32_t, __builtin_bit_cast(i16x2, carry) >> 15);
-                }
         }
         float top = c[0];
 #pragma unroll
@@ -282,9 +285,11 @@ __global__ __launch_bounds__(kWaves * 64, ROWS == 32 && WM == 1 ? 1 : 2) void mh
 #pragma unroll
         for (int s = 0; s < kScores / 2; ++s) {
             if constexpr (NEXT) {
-                // (a product, then the vector instructions of two scores, which do not wait for it: in this order)
-                static_assert(!NEXT || ROWS == 32, "");
-                x_next = mfma(__builtin_bit_cast(bf16x8, k.f[s]), __builtin_bit_cast(bf16x8, q[s]), x_next);
+                // (in this order: a product, the reads that later ones wait for, then the vector instructions of two scores, which wait for
+                // neither)
+                x_next = mfma(__builtin_bit_cast(bf16x8, k[s]), __builtin_bit_cast(bf16x8, q[s]), x_next);
+                if (s < 4) k[s + 4] = k_frag(ahead, s + 4);
+                v[s] = v_frag(stage, s);
             }
             const float p0 = fast_exp2(__builtin_fmaf(c[2 * s], a.scale_log2e, -m_run));
             const float p1 = fast_exp2(__builtin_fmaf(c[2 * s + 1], a.scale_log2e, -m_run));
@@ -299,10 +304,24 @@ __global__ __launch_bounds__(kWaves * 64, ROWS == 32 && WM == 1 ? 1 : 2) void mh
 #pragma unroll
             for (int r = 0; r < kAccSize; ++r) y_next.c[r] = x_next[r];
         }
+        if (nodes) {
+            // A weight of 0 times an infinity or NaN would be NaN: those enter as 0 here and are added at the end, for the rows that
+            // see them. (An exponent of all ones carries into the sign's place.)
+#pragma unroll
+            for (int f = 0; f < kV; ++f)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    typedef short i16x2 __attribute__((ext_vector_type(2)));
+                    const uint32_t w = v[f].half[j >> 1][j & 1];
+                    const uint32_t carry = (w & 0x7f807f80u) + 0x00800080u;
+                    broken |= carry;
+                    v[f].half[j >> 1][j & 1] = w & ~__builtin_bit_cast(uint32_t, __builtin_bit_cast(i16x2, carry) >> 15);
+                }
+        }
 #pragma unroll
         for (int f = 0; f < kV; ++f) {
             const int b = ROWS == 32 ? f >> 1 : f, s = ROWS == 32 ? f & 1 : 0;
-            const u32x4 vf = {v.f[f][0][0], v.f[f][0][1], v.f[f][1][0], v.f[f][1][1]};
+            const u32x4 vf = {v[f].half[0][0], v[f].half[0][1], v[f].half[1][0], v[f].half[1][1]};
             o[b] = mfma(__builtin_bit_cast(bf16x8, vf), __builtin_bit_cast(bf16x8, ph[s]), o[b]);
             if constexpr (EXACT) o[b] = mfma(__builtin_bit_cast(bf16x8, vf), __builtin_bit_cast(bf16x8, pl[s]), o[b]);
         }
@@ -328,18 +347,26 @@ __global__ __launch_bounds__(kWaves * 64, ROWS == 32 && WM == 1 ? 1 : 2) void mh
         Scores y;
         if (iters > 0) {
             wait_for(0, 2);
-            y = scores(read_k(0));
+            y = scores(0);
         }
-#pragma unroll 1
-        for (int it = 0; it < iters; ++it) {
+        auto step = [&](int it, int stage, auto cached) __attribute__((always_inline)) {
             if (it + 1 < iters) wait_for(it + 1, 1);
-            if (it + 3 < iters) issue(it + 3, (it + 3) & 3);
+            if (it + 3 < iters) issue(it + 3, (stage + 3) & 3);
             if (has_rows && it < my_tiles) {
-                const VFrags v = read_v(it & 3);
-                const KFrags k = read_k((it + 1) & 3);  // (behind the last tile: whatever lies there, not used)
-                y = fold(t0 + it * WK + wk, y, v, k, std::true_type{});
+                // (behind the last tile the scores are of whatever lies there, and not used)
+                y = fold(t0 + it * WK + wk, y, stage, (stage + 1) & 3, std::true_type{}, cached);
             }
-        }
+        };
+        // Four at a time where no tile has nodes: the places in the ring are constants then, and the scores change registers by name.
+        const int cached = min(max((pos / kKeys - t0) / WK, 0), iters);
+        int it = 0;
+        sees_s[wm][n] = sees;  // (not needed meanwhile, and the registers are)
+        asm volatile("" ::: "memory");
+#pragma unroll 1
+        for (; it + 4 <= cached; it += 4) static_for<0, 4>([&](auto s) __attribute__((always_inline)) { step(it + s.value, s.value, std::true_type{}); });
+        sees = sees_s[wm][n];
+#pragma unroll 1
+        for (; it < iters; ++it) step(it, it & 3, std::false_type{});
     } else {
         int stage = 0;
 #pragma unroll 1
@@ -347,10 +374,8 @@ __global__ __launch_bounds__(kWaves * 64, ROWS == 32 && WM == 1 ? 1 : 2) void mh
             wait_for(it, 0);
             if (it + 1 < iters) issue(it + 1, stage ^ 1);
             if (has_rows && it < my_tiles) {
-                KFrags k = read_k(stage);
-                asm volatile("" : "+v"(k.f[0]), "+v"(k.f[1]), "+v"(k.f[2]), "+v"(k.f[3]), "+v"(k.f[4]), "+v"(k.f[5]), "+v"(k.f[6]), "+v"(k.f[7]));
-                const VFrags v = read_v(stage);
-                fold(t0 + it * WK + wk, scores(k), v, k, std::false_type{});
+                const Scores y = scores(stage);
+                fold(t0 + it * WK + wk, y, stage, 0, std::false_type{}, std::false_type{});
             }
             stage ^= 1;
         }
