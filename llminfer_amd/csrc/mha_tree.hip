@@ -76,6 +76,15 @@ __device__ __forceinline__ int position(const TreeArgs& a) {
     return __builtin_amdgcn_readfirstlane(a.pos_dev ? max(0, min(*a.pos_dev, a.pos)) : a.pos);
 }
 
+// dma16 without the streaming hint, for tiles that several workgroups read.
+__device__ __forceinline__ void dma16_kept(const char* base, uint32_t voff, uint32_t lds_off) {
+    const uint64_t b = reinterpret_cast<uint64_t>(base);
+    const uint32_t b_lo = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b), b_hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32));
+    const uint64_t sbase = ((uint64_t)b_hi << 32) | (uint64_t)b_lo;
+    const uint32_t slds = (uint32_t)__builtin_amdgcn_readfirstlane(lds_off);
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(voff), "s"(sbase), "{m0}"(slds) : "memory");
+}
+
 // A load's base in scalar registers, for long enough (see scalar_bases).
 __device__ __forceinline__ void scalar_base(const char*& p) { asm volatile("s_nop 4" : "+s"(p)); }
 
@@ -176,7 +185,8 @@ __global__ __launch_bounds__(kWaves * 64, ROWS == 32 && WM == 1 ? 1 : 2) void mh
                 if constexpr (decltype(whole)::value) base += (int64_t)(4 * b8) * rs;
                 else off += (uint32_t)(min(4 * b8 + rho, last) - rho) * rs;  // rows past the keys repeat the last one: seen by nobody
                 scalar_base(base);
-                dma16(base, off, to + (uint32_t)(b * 1024));
+                if constexpr (EXACT) dma16(base, off, to + (uint32_t)(b * 1024));
+                else dma16_kept(base, off, to + (uint32_t)(b * 1024));
             }
         };
         if (last >= kKeys - 1) load(std::true_type{});
