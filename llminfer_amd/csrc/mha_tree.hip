@@ -328,6 +328,9 @@ __global__ __launch_bounds__(kWaves * 64, ROWS == 32 && WM == 1 ? 1 : 2) void mh
                     v[f].half[j >> 1][j & 1] = w & ~__builtin_bit_cast(uint32_t, __builtin_bit_cast(i16x2, carry) >> 15);
                 }
         }
+        // (the second product's wavefront goes first: its products keep the matrix cores busy while the other wavefront of the SIMD has its
+        // vector instructions between them. 64 nodes of 64 heads at 131000 positions 322 : 290 us, 61 of 32 heads at 32768 55.8 : 52.2.)
+        if constexpr (NEXT) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int f = 0; f < kV; ++f) {
             const int b = ROWS == 32 ? f >> 1 : f, s = ROWS == 32 ? f & 1 : 0;
@@ -335,6 +338,7 @@ __global__ __launch_bounds__(kWaves * 64, ROWS == 32 && WM == 1 ? 1 : 2) void mh
             o[b] = mfma(__builtin_bit_cast(bf16x8, vf), __builtin_bit_cast(bf16x8, ph[s]), o[b]);
             if constexpr (EXACT) o[b] = mfma(__builtin_bit_cast(bf16x8, vf), __builtin_bit_cast(bf16x8, pl[s]), o[b]);
         }
+        if constexpr (NEXT) __builtin_amdgcn_s_setprio(0);
         return y_next;
     };
     const int my_tiles = t1 - t0 > wk ? (t1 - t0 - wk + WK - 1) / WK : 0;
