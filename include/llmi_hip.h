@@ -408,9 +408,8 @@ typedef struct llmi_kv_commit_tree_args {
     void* stream;
 } llmi_kv_commit_tree_args;
 
-/* In every layer, for i = 1 .. result[0]-1: the K and V rows of slot pos + path[i] to slot pos + i. In place: an accepted
- * path ascends, so no row is overwritten before it has been moved. Entries below i or beyond node_num move nothing, every other slot
- * stays as it is. Does not change the position word: add result[0] to it behind this call. */
+/* In every layer, for i = 1 .. result[0]-1: the K and V rows that stood in slot pos + path[i] before the call to slot pos + i, in
+ * place. Entries below i or from node_num on move nothing, every other slot stays as it is. Does not change the position word: add result[0] to it behind this call. */
 int llmi_hip_kv_commit_tree(const llmi_kv_commit_tree_args* args);
 
 /* ---- pooled device allocator ------------------------------------------- */

@@ -107,7 +107,8 @@ __device__ __forceinline__ void write_out(const TreeArgs& a, int kvh, int row, i
 // WM wavefronts side by side on ROWS query rows each, 4 / WM of them on a tile each of the same rows. EXACT: a probability enters the second
 // product as the sum of two bf16 numbers (relative error 2^-17), otherwise as one (2^-8).
 template <int ROWS, int WM, bool EXACT, int STAGES>
-__global__ __launch_bounds__(kWaves * 64, ROWS == 32 && WM == 1 ? 1 : 2) void mha_tree_kernel(TreeArgs a) {
+// (two workgroups on a compute unit where its LDS holds two rings: a hint without which the accumulators go to AGPRs and back)
+__global__ __launch_bounds__(kWaves * 64, STAGES * (kWaves / WM) * kTileBytes <= 80 * 1024 ? 2 : 1) void mha_tree_kernel(TreeArgs a) {
     constexpr int WK = kWaves / WM;
     constexpr int kStageBytes = WK * kTileBytes;
     constexpr int kLoads = 16 / WM;      // 1 KiB blocks of a tile per wavefront: eight of K, eight of V
@@ -572,8 +573,14 @@ int launch_mha_tree(const llmi_mha_tree_args& args, const TreeForm& form) {
     a.part_ml = reinterpret_cast<float2*>(a.part + (size_t)n_kv * a.blocks * a.splits * (form.rows / 2) * 64);
     a.scale_log2e = 1.4426950408889634f / sqrtf((float)kHeadDim);
     const hipStream_t stream = static_cast<hipStream_t>(m.stream);
+    // Two wavefronts on each of two tiles: scores ahead from six pairs of tiles a split on, before that the longer way to the first product costs
+    // more (two stages : four, us, 16 nodes of 32 heads, 8 KV heads: 13.2 : 14.3 at 6000 positions, 16.5 : 17.1 at 10000, 19.9 : 19.5 at 14000, 33.4 : 30.4
+    // at 32768).
+    constexpr int kPairsAhead = 6;
+    const int pairs = (m.pos + args.node_num) / kKeys / (2 * a.splits);
     if (form.rows == 16) launch<16, 1, true, 2>(a, n_kv, stream);
     else if (form.row_waves == 1) launch<32, 1, true, 2>(a, n_kv, stream);
+    else if (form.row_waves == 2 && pairs < kPairsAhead) launch<32, 2, true, 2>(a, n_kv, stream);
     else if (form.row_waves == 2) launch<32, 2, true, 4>(a, n_kv, stream);
     else if (form.blocks <= 4) launch<32, 4, true, 4>(a, n_kv, stream);
     else launch<32, 4, false, 4>(a, n_kv, stream);

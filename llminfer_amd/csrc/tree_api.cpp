@@ -93,8 +93,8 @@ int llmi_hip_mha_decode_tree(const llmi_mha_tree_args* args) {
 
 size_t llmi_hip_mha_tree_workspace_bytes(int32_t head_num, int32_t head_dim, int32_t node_num) {
     if (head_num <= 0 || head_dim <= 0 || node_num <= 0 || node_num > LLMI_TREE_MAX_NODES) return 0;
-    // (how many KV heads share the query heads is not said, nor the length: whatever needs most. Sixteen rows by length are bounded
-    // by the workgroups the rule allows them)
+    // (how many KV heads share the query heads is not said, nor the length: whatever needs most. Sixteen rows by length: a workgroup
+    // takes one block)
     size_t most = 16;
     for (int group = 1; group <= kMaxGroup; ++group) {
         if (head_num % group != 0) continue;
@@ -102,7 +102,7 @@ size_t llmi_hip_mha_tree_workspace_bytes(int32_t head_num, int32_t head_dim, int
         const TreeForm f = tree_blocks(node_num * group, n_kv, INT32_MAX);
         most = std::max(most, (size_t)tree_splits(f, n_kv, INT32_MAX) * n_kv * f.blocks * tree_split_bytes(f));
     }
-    return std::max(most, kSmallGroups * tree_split_bytes({16, 1, 1, 1}));
+    return std::max(most, 256 * tree_split_bytes({16, 1, 1, 1}));
 }
 
 int llmi_hip_qk_norm_rope_append_tree(const llmi_qk_norm_rope_tree_args* a) {

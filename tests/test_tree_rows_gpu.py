@@ -136,7 +136,7 @@ def test_commit(dev, layout, n, path, n_kv, layers, pos):
 def test_commit_leaves_alone_what_it_cannot_place(dev):
     """Counts and entries out of range move nothing, and nothing beyond the nodes' slots is touched."""
     c = [cache(dev, 2, 40, 8, HEAD, 50 + i) for i in range(2)]
-    for path, count in (([0, 3, 5], 0), ([0, 3, 5], -7), ([0, -1, 0, 10, 64, 1 << 30, -(1 << 31)], 7), ([0, 0, 1, 2], 4)):
+    for path, count in (([0, 3, 5], 0), ([0, 3, 5], -7), ([0, -1, 0, 10, 64, 1 << 30, -(1 << 31)], 7), ([0, 0, 1, 2], 4), ([7, 1, 2, 3], 4)):
         mine = [x.clone() for x in c]
         commit(mine, path, count, 10, HEAD, 20)
         assert all(torch.equal(a, b) for a, b in zip(mine, c)), (path, count)
