@@ -1,5 +1,6 @@
 """llmi_hip_mha_decode_tree on the device against its definition in 64 bits: the same bf16 inputs, the fp32 result within the bound of
 tree_cases.attention_bound, the bf16 output the rounding of the fp32 result. Whatever the call must not read holds NaN."""
+import ctypes
 import math
 
 import pytest
@@ -126,6 +127,47 @@ def test_seen_values_keep_their_infinities(dev):
     assert bool((got[4:, :, 17] == math.inf).all()) and bool(torch.isfinite(got[:4]).all())
     rest = [d for d in range(D) if d != 17]
     assert bool(torch.isfinite(got[:, :, rest]).all())
+
+
+# nodes, query heads, KV heads, cached positions, query rows of a workgroup: every way the kernels take a call (blocks of 16 rows, one and
+# several; one block of 32; two, over short and long splits; four, one workgroup and several to a tile)
+FORMS = [(5, 16, 8, 50, 16), (26, 32, 8, 500, 16), (8, 32, 8, 9000, 32), (16, 32, 8, 6000, 64), (16, 32, 8, 14000, 64), (26, 32, 8, 6007, 128),
+         (61, 32, 8, 3000, 128), (64, 64, 8, 2500, 128), (33, 32, 2, 9000, 128)]
+
+
+@pytest.mark.parametrize("layout", [POS, HEAD])
+@pytest.mark.parametrize("n,n_q,n_kv,ctx,rows_of_group", FORMS)
+def test_every_form(dev, n, n_q, n_kv, ctx, rows_of_group, layout):
+    """A tree with nodes that hold NaN, infinities and the lowest value for those that do not see them, one empty word; then shorter contexts
+    from the device, which the same launch serves."""
+    bad = [i for i in range(1, n) if i % 4 == 1]
+    hidden = sum(1 << i for i in bad)
+    words = [w & ~hidden for w in words_of(parents_of(7, n))]
+    words[n - 1] = 0
+    c = Case(dev, n, n_q, n_kv, ctx, layout, words=words, seed=n)
+    args = B.MhaTreeArgs()
+    args.mha = ops.make_mha_args(c.q, c.kc, c.vc, c.q, torch.empty(24 << 20, device=dev), **{k: v for k, v in c.scalars().items() if k != "node_num"})
+    args.node_num = n
+    plan = B.MhaPlan()
+    assert B.lib().llmi_hip_mha_tree_plan(ctypes.byref(args), ctypes.byref(plan)) == 0 and plan.group_pad == rows_of_group
+    clean = c.run()
+    c.check(clean)
+    word = torch.zeros(1, dtype=torch.int32, device=dev)
+    for pos in (0, 1, ctx // 2 + 3, ctx - 1):
+        word.fill_(pos)
+        c.check(c.run(pos_device=word), ctx=pos, what="position %d" % pos)
+    for k, i in enumerate(bad):
+        for cache in (c.kc, c.vc):
+            by_head(cache[0], layout)[:, ctx + i] = [NAN, math.inf, -math.inf, -3.3895e38][k % 4]
+    assert torch.equal(c.run(), clean)
+    # ... and who sees one value that is not finite has it, in its column alone
+    sees = [i for i in range(n) if words[i] & 1]
+    by_head(c.vc[0], layout)[:, ctx, 77] = math.inf
+    got = c.run()
+    assert bool((got[sees][:, :, 77] == math.inf).all()) and torch.equal(got[:, :, :77], clean[:, :, :77]) and torch.equal(got[:, :, 78:], clean[:, :, 78:])
+    by_head(c.vc[0], layout)[:, ctx, 77] = NAN
+    got = c.run()
+    assert bool(torch.isnan(got[sees][:, :, 77]).all()) and torch.equal(got[:, :, :77], clean[:, :, :77]) and torch.equal(got[:, :, 78:], clean[:, :, 78:])
 
 
 def test_overflowing_scores(dev):

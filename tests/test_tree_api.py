@@ -119,6 +119,52 @@ def test_append_status_codes(over, row, status):
     assert B.lib().llmi_hip_qk_norm_rope_append_tree(ctypes.byref(t)) == B.STATUS[status]
 
 
+@pytest.mark.parametrize("n,n_q,n_kv,pos,rows,splits", [
+    (5, 16, 8, 57, 16, 1), (5, 16, 8, 250, 16, 1), (5, 16, 8, 252, 16, 2), (8, 32, 8, 500, 16, 4), (8, 32, 8, 4099, 16, 16), (8, 32, 8, 9000, 32, 32),
+    (16, 32, 8, 6000, 64, 32), (26, 32, 8, 500, 16, 4), (26, 32, 8, 6007, 128, 32), (61, 32, 8, 6000, 128, 16), (61, 32, 8, 32768, 128, 32),
+    (64, 64, 8, 131000, 128, 16), (64, 64, 8, 100, 16, 1), (1, 8, 1, 131000, 16, 256),
+])
+def test_plan_by_size(n, n_q, n_kv, pos, rows, splits):
+    rc, p = plan(tree_args(node_num=n, head_num=n_q, kv_dim=128 * n_kv, kv_mul=n_q // n_kv, pos=pos, max_seq_len=pos + n))
+    assert rc == 0 and (p.group_pad, p.num_splits) == (rows, splits)
+    assert p.path == (B.PATH_SINGLE_PASS if splits == 1 else B.PATH_SPLIT) and p.waves_per_group == 4
+
+
+def test_plan_invariants_over_random_arguments():
+    import random
+    rng = random.Random(12)
+    for _ in range(3000):
+        n, group, n_kv = rng.randint(1, 64), rng.randint(1, 16), rng.choice([1, 2, 3, 4, 8, 16, 40])
+        pos = int(2 ** (rng.random() * 18)) - 1
+        forced = rng.choice([0, 0, 0, 1, 2, 17, 256])
+        t = tree_args(node_num=n, head_num=group * n_kv, kv_dim=128 * n_kv, kv_mul=group, pos=pos, max_seq_len=pos + n + rng.randint(0, 9), num_splits=forced)
+        t.mha.workspace_bytes = 1 << 40
+        rc, p = plan(t)
+        tiles = -(-(pos + n) // 32)
+        rows = group * n
+        assert rc == 0 and 1 <= p.num_splits <= min(256, tiles) and p.rows_per_split * p.num_splits >= pos + n
+        assert p.group_pad in (16, 32, 64, 128) and (rows > 16 or p.group_pad == 16)
+        assert (p.num_splits == 1) == (p.workspace_needed == 0)
+        if forced:
+            assert p.num_splits == min(forced, tiles)
+            if p.num_splits > 1:
+                t.mha.workspace_bytes = p.workspace_needed - 1
+                assert plan(t)[0] == B.STATUS["WORKSPACE"]
+                t.mha.workspace_bytes += 1
+                assert plan(t)[0] == 0
+                t.mha.workspace = None
+                assert plan(t)[0] == B.STATUS["WORKSPACE"]
+        else:
+            # what workspace_bytes says is enough, whatever the length; less of it means fewer splits; none at all, one
+            assert p.workspace_needed <= ops.tree_workspace_bytes(group * n_kv, 128, n)
+            t.mha.workspace_bytes = p.workspace_needed // 2
+            rc, q = plan(t)
+            assert rc == 0 and q.num_splits <= max(1, p.num_splits // 2) and q.workspace_needed <= t.mha.workspace_bytes
+            t.mha.workspace = None
+            rc, q = plan(t)
+            assert rc == 0 and q.num_splits == 1 and q.path == B.PATH_SINGLE_PASS
+
+
 def test_workspace_sizes():
     assert ops.tree_workspace_bytes(32, 128, 8) > 0 and ops.tree_workspace_bytes(0, 128, 8) == 0 and ops.tree_workspace_bytes(32, 128, 0) == 0
     assert ops.verify_workspace_bytes(8, 1000) > 0 and ops.verify_workspace_bytes(0, 5) == 0 and ops.verify_workspace_bytes(3, 0) == 0
