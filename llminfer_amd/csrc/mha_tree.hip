@@ -476,12 +476,12 @@ __global__ __launch_bounds__(kWaves * 64, STAGES * (kWaves / WM) * kTileBytes <=
     if (wk == 0 && kg == 0) a.part_ml[at * ROWS + n] = t1 > t0 ? make_float2(m_run, l_run) : make_float2(-INFINITY, 0.0f);
 }
 
-// The splits of a block joined: a workgroup per slot, its wavefronts on every fourth split, eight of them asked for at once.
-template <int ROWS>
-__global__ __launch_bounds__(kWaves * 64) void mha_tree_join_kernel(TreeArgs a) {
+// The splits of a block joined: a workgroup per slot, its W wavefronts on every W-th split, eight of them asked for at once.
+template <int ROWS, int W>
+__global__ __launch_bounds__(W * 64) void mha_tree_join_kernel(TreeArgs a) {
     constexpr int kAhead = 8;
-    __shared__ f32x4 wave_o[kWaves][64];
-    __shared__ float wave_m[kWaves][64], wave_l[kWaves][64];
+    __shared__ f32x4 wave_o[W][64];
+    __shared__ float wave_m[W][64], wave_l[W][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int kvh = blockIdx.x, slot = blockIdx.y, block = blockIdx.z;
     const int n = lane & (ROWS - 1);
@@ -490,15 +490,15 @@ __global__ __launch_bounds__(kWaves * 64) void mha_tree_join_kernel(TreeArgs a) 
     const f32x4* part = a.part + (first * kSlots<ROWS> + slot) * 64 + lane;
     float m = -FLT_MAX, sum = 0.0f;
     f32x4 o{};
-    for (int s0 = wave; s0 < a.splits; s0 += kWaves * kAhead) {
+    for (int s0 = wave; s0 < a.splits; s0 += W * kAhead) {
         float2 x[kAhead];
         f32x4 y[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            const int s = min(s0 + kWaves * i, a.splits - 1);
+            const int s = min(s0 + W * i, a.splits - 1);
             x[i] = ml[s * ROWS];
             y[i] = part[(int64_t)s * kSlots<ROWS> * 64];
-            if (s0 + kWaves * i >= a.splits) x[i] = make_float2(-INFINITY, 0.0f);
+            if (s0 + W * i >= a.splits) x[i] = make_float2(-INFINITY, 0.0f);
         }
         float top = m;
 #pragma unroll
@@ -524,11 +524,11 @@ __global__ __launch_bounds__(kWaves * 64) void mha_tree_join_kernel(TreeArgs a) 
     if (wave != 0) return;
     float top = m;
 #pragma unroll
-    for (int i = 1; i < kWaves; ++i) top = fmaxf(top, wave_m[i][lane]);
+    for (int i = 1; i < W; ++i) top = fmaxf(top, wave_m[i][lane]);
     f32x4 all{};
     float total = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
+    for (int i = 0; i < W; ++i) {
         const float w = fast_exp2(wave_m[i][lane] - top);
         const f32x4 y = wave_o[i][lane];
         total += w * wave_l[i][lane];
@@ -542,7 +542,12 @@ template <int ROWS, int WM, bool EXACT, int STAGES>
 void launch(const TreeArgs& a, int n_kv, hipStream_t stream) {
     const dim3 grid(n_kv, a.splits, (a.blocks + WM - 1) / WM), block(kWaves * 64);
     hipLaunchKernelGGL((mha_tree_kernel<ROWS, WM, EXACT, STAGES>), grid, block, 0, stream, a);
-    if (a.splits > 1) hipLaunchKernelGGL((mha_tree_join_kernel<ROWS>), dim3(n_kv, kSlots<ROWS>, a.blocks), block, 0, stream, a);
+    if (a.splits == 1) return;
+    // (a trip to memory for all splits up to 128)
+    const dim3 join(n_kv, kSlots<ROWS>, a.blocks);
+    if (a.splits <= 32) hipLaunchKernelGGL((mha_tree_join_kernel<ROWS, 4>), join, dim3(4 * 64), 0, stream, a);
+    else if (a.splits <= 64) hipLaunchKernelGGL((mha_tree_join_kernel<ROWS, 8>), join, dim3(8 * 64), 0, stream, a);
+    else hipLaunchKernelGGL((mha_tree_join_kernel<ROWS, 16>), join, dim3(16 * 64), 0, stream, a);
 }
 
 }  // namespace

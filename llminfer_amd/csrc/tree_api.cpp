@@ -47,7 +47,12 @@ int tree_splits(const TreeForm& f, int n_kv, int64_t tiles) {
     if (tiles <= kSingleTiles) return 1;
     const int row_groups = (f.blocks + f.row_waves - 1) / f.row_waves;
     const int groups = f.row_waves == 4 && tiles * n_kv * row_groups >= 256 * 64 ? 512 : 256;
-    const int64_t splits = std::min<int64_t>(std::min(groups / (n_kv * row_groups), kMaxSplits), tiles * f.row_waves / 4);
+    // No more than a tile for each wavefront; and beyond 32, with few KV heads, only as many as have four iterations (six of single tiles): us by
+    // splits, 5 nodes of 8 heads, one KV head 10.3 : 9.7 : 11.5 with 32 : 64 : 70 at 9000 positions, 22.3 : 15.6 : 20.6 with 32 : 64 : 128 at 40000, 43.4 : 29.2
+    // : 26.8 with 64 : 128 : 256 at 131000; 16 nodes of 16 heads, two 17.0 : 16.4 : 17.7 : 19.6 with 48 : 64 : 94 : 128 at 12000; 26 nodes, one
+    // 16.3 : 17.9 : 24.5 with 32 : 64 : 128 at 9000.
+    const int64_t most = std::max<int64_t>(32, tiles / (f.row_waves == 4 ? 6 : 16 / f.row_waves));
+    const int64_t splits = std::min({(int64_t)std::min(groups / (n_kv * row_groups), kMaxSplits), tiles * f.row_waves / 4, most});
     return splits < 2 ? 1 : (int)splits;
 }
 

@@ -122,7 +122,7 @@ def test_append_status_codes(over, row, status):
 @pytest.mark.parametrize("n,n_q,n_kv,pos,rows,splits", [
     (5, 16, 8, 57, 16, 1), (5, 16, 8, 250, 16, 1), (5, 16, 8, 252, 16, 2), (8, 32, 8, 500, 16, 4), (8, 32, 8, 4099, 16, 16), (8, 32, 8, 9000, 32, 32),
     (16, 32, 8, 6000, 64, 32), (26, 32, 8, 500, 16, 4), (26, 32, 8, 6007, 128, 32), (61, 32, 8, 6000, 128, 16), (61, 32, 8, 32768, 128, 32),
-    (64, 64, 8, 131000, 128, 16), (64, 64, 8, 100, 16, 1), (1, 8, 1, 131000, 16, 256),
+    (64, 64, 8, 131000, 128, 16), (64, 64, 8, 100, 16, 1), (1, 8, 1, 131000, 16, 255),
 ])
 def test_plan_by_size(n, n_q, n_kv, pos, rows, splits):
     rc, p = plan(tree_args(node_num=n, head_num=n_q, kv_dim=128 * n_kv, kv_mul=n_q // n_kv, pos=pos, max_seq_len=pos + n))
