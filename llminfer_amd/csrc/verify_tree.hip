@@ -12,6 +12,9 @@
 // bits before the exponential), the exponential is the hardware's. A thread adds its sixteen weights of a slice in fp32, everything above that in
 // fp64: whichever of two neighbouring tokens a sum falls on then depends on the weights' own rounding alone.
 
+// What bounds it: the stream of the rows in the first launch (26 x 151936 fp32 in 6 us), dependent trips to memory in the second. 6 rows of 32000 with
+// draft logits 14 us, 26 of 151936 greedy 9.7, 64 of 151936 in bf16 sampled 18.7 (one workgroup that decides and draws: 51, 17, 191).
+
 #include <hip/hip_runtime.h>
 #include <float.h>
 #include <stdint.h>
