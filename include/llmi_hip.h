@@ -328,7 +328,8 @@ typedef struct llmi_mha_tree_args {
 /* Attention of all nodes of one layer: for node i and query head h the softmax-weighted sum of V rows as in
  * llmi_hip_mha_decode, over the cached positions 0..pos-1 and the nodes its word names (slots pos..pos+node_num-1, written
  * before). A node with no key at all (an empty word and nothing cached) gets zeros; what stands in the K and V rows a node does
- * not see leaves no trace in its output, NaN and infinities included. Allocates nothing; safe under stream capture; the workspace needs
+ * not see leaves no trace in its output, NaN and infinities included. A V row that it sees with an infinity or NaN makes that column
+ * of its output one that is not finite (an infinity at a cached position may come out as NaN). Allocates nothing; safe under stream capture; the workspace needs
  * no initialisation, and two calls that share one must not overlap in time. */
 int llmi_hip_mha_decode_tree(const llmi_mha_tree_args* args);
 /* What llmi_hip_mha_decode_tree would launch (no HIP call): path, num_splits, rows_per_split, waves_per_group and
@@ -386,9 +387,10 @@ typedef struct llmi_verify_tree_args {
  *  - with draft_logits, q = softmax(draft row / temperature): accepted if u[c] * q_v(token) < p_v(token); if not, the following token
  *    is drawn from max(p_v - q_v, 0).
  * Drawn: the first token t at which the sum of what is left over tokens 0..t exceeds u[0] times the sum over all (if nothing is left, the
- * likeliest). Weights are fp32, their sums fp64, in an order that depends on vocab alone. -inf (a filtered token) and NaN logits have no
- * weight, +inf counts as the largest finite number; behind a row without a weight nothing is accepted and the token is -1.
- * A parent or token outside its range makes its node (and those below) one that is not accepted. Allocates nothing; safe under capture. */
+ * likeliest). Weights are fp32; a thread adds its sixteen of 4096 tokens in fp32, everything above in fp64, in an order that vocab, node_num
+ * and the logits' type fix: the same call gives the same tokens. -inf (a filtered token) and NaN logits have no weight, +inf counts as the
+ * largest finite number. Behind a target row without a weight nothing is accepted and the token is -1; behind a draft row without one nothing is
+ * accepted and the token is drawn from p_v. A parent or token outside its range makes its node (and those below) one that is not accepted. Allocates nothing; safe under capture. */
 int llmi_hip_verify_tree(const llmi_verify_tree_args* args);
 size_t llmi_hip_verify_tree_workspace_bytes(int32_t node_num, int32_t vocab);
 

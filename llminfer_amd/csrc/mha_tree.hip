@@ -19,7 +19,7 @@
 // exchanged by the row's low four bits, V's 32-byte pieces rotated by the row's low three, which spreads every read over the banks.
 //
 // Keys are split over workgroups; a second launch joins the splits. What bounds it: the way to the first product and the join's launch up to a few
-// thousand positions (8 nodes of 32 heads, 8 KV heads at 4099: 10.3 us, 17 MB), memory for few rows (8 nodes at 32768: 29.5 us, 4.6 TB/s), matrix cores and
+// thousand positions (8 nodes of 32 heads, 8 KV heads at 4099: 10.3 us, 17 MB), memory for few rows (8 nodes at 32768: 29.6 us, 4.5 TB/s), matrix cores and
 // the exponentials between their products for many (64 nodes of 64 heads at 131000: 290 us, 0.95 PFLOP/s).
 
 #include <hip/hip_runtime.h>
@@ -398,14 +398,15 @@ __global__ __launch_bounds__(kWaves * 64, STAGES * (kWaves / WM) * kTileBytes <=
         }
     }
 
-    // Infinities and NaN among the values of nodes, for the rows that see them.
+    // Infinities and NaN among the values of the nodes' tiles, for the rows that see them: nodes, and (x < 0, seen by all) the cached positions
+    // that share the first node's tile.
     if (__builtin_expect(__any((broken & 0x80008000u) != 0u), 0)) {
 #pragma unroll 1
-        for (int x = 0; x < a.nodes; ++x) {
+        for (int x = -(pos % kKeys); x < a.nodes; ++x) {
             const int t = (pos + x) / kKeys;
             if (t < t0 || t >= t1 || (t - t0) % WK != wk) continue;
             const char* at = vb + (int64_t)(pos + x) * rs;
-            const bool seen = sees >> x & 1;
+            const bool seen = x < 0 || (sees >> x & 1);
 #pragma unroll
             for (int slot = 0; slot < kS; ++slot) {
                 const u32x2 w = *reinterpret_cast<const u32x2*>(at + 2 * slot_column<ROWS>(slot, lane));

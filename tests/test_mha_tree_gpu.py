@@ -170,6 +170,24 @@ def test_every_form(dev, n, n_q, n_kv, ctx, rows_of_group, layout):
     assert bool(torch.isnan(got[sees][:, :, 77]).all()) and torch.equal(got[:, :, :77], clean[:, :, :77]) and torch.equal(got[:, :, 78:], clean[:, :, 78:])
 
 
+@pytest.mark.parametrize("poison", [NAN, math.inf, -math.inf])
+@pytest.mark.parametrize("n,n_q,n_kv,ctx,rows_of_group", FORMS)
+def test_cached_values_that_are_not_finite(dev, n, n_q, n_kv, ctx, rows_of_group, poison):
+    """Every node sees the cached positions: a V row there with an infinity or NaN shows in that column of every output and in no other, in the
+    tile that cached positions share with the nodes (the last one) as in those before."""
+    assert ctx % 32 != 0
+    c = Case(dev, n, n_q, n_kv, ctx, seed=n)
+    clean = c.run()
+    v = by_head(c.vc[0], c.layout)
+    for at in (ctx - 1, ctx - ctx % 32, ctx // 3):
+        kept = v[:, at, 77].clone()
+        v[:, at, 77] = poison
+        got = c.run()
+        v[:, at, 77] = kept
+        assert not bool(torch.isfinite(got[:, :, 77]).any()), "position %d" % at
+        assert torch.equal(got[:, :, :77], clean[:, :, :77]) and torch.equal(got[:, :, 78:], clean[:, :, 78:]), "position %d" % at
+
+
 def test_overflowing_scores(dev):
     """Scores below the least fp32 number have no weight; a node with no other key gets zeros."""
     c = Case(dev, 8, 16, 8, 0, kind="star")

@@ -168,6 +168,31 @@ def test_nothing_left(dev):
     assert run(dev, target, np.array([0, 4444], np.int32), [-1, 0], np.full(2, 1.5, np.float32), 1.0, draft) == ([0], 4444)
 
 
+def test_a_draft_row_without_weight(dev):
+    """It cannot have given the token: refused, and the following one is the target's own."""
+    # (4096 equal weights: every sum is exact)
+    target = np.zeros((3, 4096), np.float32)
+    target[0, 4000] = 40.0
+    for empty in (-INF, math.nan):
+        draft = target.copy()
+        draft[0] = empty
+        assert run(dev, target, np.array([0, 4000, 7], np.int32), [-1, 0, 1], np.full(3, 0.5, np.float32), 1.0, draft) == ([0], 4000)
+        # (the second row is one: its node is not reached past)
+        draft = target.copy()
+        draft[1] = empty
+        assert run(dev, target, np.array([0, 4000, 7], np.int32), [-1, 0, 1], np.array([0.5, 0.5, 0.0], np.float32), 1.0, draft) == ([0, 1], 2048)
+
+
+def test_greedy_takes_no_random_numbers(dev):
+    target, _, tokens, parents, _ = make(11, 20, 9000)
+    ws = torch.empty(ops.verify_workspace_bytes(20, 9000) // 4, device=dev)
+    path, result = torch.zeros(20, dtype=torch.int32, device=dev), torch.zeros(2, dtype=torch.int32, device=dev)
+    ops.verify_tree(torch.from_numpy(target).to(dev), torch.from_numpy(tokens).to(dev), None, path, result, ws,
+                    parents=torch.tensor(parents, dtype=torch.int32, device=dev), temperature=0.0)
+    count, token = result.tolist()
+    assert (path.tolist()[:count], token) == verify_oracle(target, tokens, parents, None, 0.0)
+
+
 @pytest.mark.parametrize("with_draft", [False, True])
 def test_the_target_is_what_is_sampled(dev, with_draft):
     """The first token behind the root over many random numbers, against the target's distribution: frequencies within five
