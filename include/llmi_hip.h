@@ -385,7 +385,8 @@ typedef struct llmi_verify_tree_args {
  *  - without draft_logits child c of node v is accepted if u[c] * (1 - p_v of the tokens refused before it) < p_v(token of c), never
  *    if its token has been refused before; if none is, the following token is drawn from p_v without the refused tokens;
  *  - with draft_logits, q = softmax(draft row / temperature): accepted if u[c] * q_v(token) < p_v(token); if not, the following token
- *    is drawn from max(p_v - q_v, 0).
+ *    is drawn from max(p_v - q_v, 0). Behind a node whose child's token is outside the vocabulary nothing has been tried: the following token is
+ *    drawn from p_v, and the draft's row is not used. So a chain shorter than node_num is filled up with tokens of -1.
  * Drawn: the first token t at which the sum of what is left over tokens 0..t exceeds u[0] times the sum over all (if nothing is left, the
  * likeliest). Weights are fp32; a thread adds its sixteen of 4096 tokens in fp32, everything above in fp64, in an order that vocab, node_num
  * and the logits' type fix: the same call gives the same tokens. -inf (a filtered token) and NaN logits have no weight, +inf counts as the

@@ -203,6 +203,7 @@ struct Walk {
     int32_t refused[kNodes];
     uint32_t alike[kThreads / 64][kNodes];  // sixteen nodes each: same parent (low half), same token
     int32_t last, refused_n, count;
+    int32_t tried;  // a draft's token was tried behind the last node, and refused
 };
 
 // All rows' slices joined, `lanes` lanes a row; then the nodes. `writes`: this workgroup writes the path.
@@ -317,12 +318,13 @@ __device__ __forceinline__ void walk(const VerifyArgs& a, Walk& w, bool writes) 
         }
         const int count = __popcll(on), last = 63 - __clzll(on);
         const bool gone = valid && parent == last && !again;
-        const uint64_t gone_set = a.draft ? 0ull : __ballot(gone);
+        const uint64_t tried_set = __ballot(gone), gone_set = a.draft ? 0ull : tried_set;
         if (!a.draft && gone) w.refused[__popcll(gone_set & ((1ull << i) - 1))] = token;
         if (i == 0) {
             w.last = last;
             w.count = count;
             w.refused_n = __popcll(gone_set);
+            w.tried = tried_set != 0;
         }
         if (writes) {
             if (on >> i & 1) a.path[__popcll(on & ((1ull << i) - 1))] = i;
@@ -333,13 +335,14 @@ __device__ __forceinline__ void walk(const VerifyArgs& a, Walk& w, bool writes) 
     __syncthreads();
 }
 
-// What is left of a thread's weights at the last accepted node.
+// What is left of a thread's weights at the last accepted node. (The draft's distribution is taken away where a token that came from it has been
+// refused. Behind the last node of a chain, and behind one whose child's token is outside the vocabulary, a chain shorter than its rows, none has.)
 template <typename T>
 __device__ __forceinline__ void left_of(const VerifyArgs& a, const Walk& w, int slice, float (&v)[kEach], double (&left)[kEach]) {
     const int last = w.last;
     const float m = w.tops[last].max;
     load_slice(static_cast<const T*>(a.target) + last * a.target_stride, slice, a.vocab, v);
-    if (a.draft && last < a.nodes - 1) {
+    if (a.draft && w.tried) {
         float q[kEach];
         load_slice(static_cast<const T*>(a.draft) + last * a.draft_stride, slice, a.vocab, q);
         const float m_q = w.tops[a.nodes + last].max;
