@@ -329,7 +329,7 @@ typedef struct llmi_mha_tree_args {
  * llmi_hip_mha_decode, over the cached positions 0..pos-1 and the nodes its word names (slots pos..pos+node_num-1, written
  * before). A node with no key at all (an empty word and nothing cached) gets zeros; what stands in the K and V rows a node does
  * not see leaves no trace in its output, NaN and infinities included. A V row that it sees with an infinity or NaN makes that column
- * of its output one that is not finite (an infinity at a cached position may come out as NaN). Allocates nothing; safe under stream capture; the workspace needs
+ * of its output one that is not finite (an infinity at a cached position, or with a weight of 0 in fp32, may come out as NaN). Allocates nothing; safe under stream capture; the workspace needs
  * no initialisation, and two calls that share one must not overlap in time. */
 int llmi_hip_mha_decode_tree(const llmi_mha_tree_args* args);
 /* What llmi_hip_mha_decode_tree would launch (no HIP call): path, num_splits, rows_per_split, waves_per_group and

@@ -515,9 +515,9 @@ __global__ __launch_bounds__(W * 64) void mha_tree_join_kernel(TreeArgs a) {
         for (int i = 0; i < kAhead; ++i) {
             const float w = fast_exp2(x[i].x - m);
             sum += w * x[i].y;
-            // (a split without keys has left no part)
+            // (a split without keys has left no part; a weight of 0 alone does not say that: an infinity or NaN counts with it too)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = w == 0.0f ? o[e] : o[e] + w * y[i][e];
+            for (int e = 0; e < 4; ++e) o[e] = x[i].x == -INFINITY ? o[e] : o[e] + w * y[i][e];
         }
     }
     wave_o[wave][lane] = o;
