@@ -329,8 +329,11 @@ typedef struct llmi_mha_tree_args {
  * llmi_hip_mha_decode, over the cached positions 0..pos-1 and the nodes its word names (slots pos..pos+node_num-1, written
  * before). A node with no key at all (an empty word and nothing cached) gets zeros; what stands in the K and V rows a node does
  * not see leaves no trace in its output, NaN and infinities included. A V row that it sees with an infinity or NaN makes that column
- * of its output one that is not finite (an infinity at a cached position, or with a weight of 0 in fp32, may come out as NaN). Allocates nothing; safe under stream capture; the workspace needs
- * no initialisation, and two calls that share one must not overlap in time. */
+ * of its output one that is not finite (an infinity at a cached position, or with a weight of 0 in fp32, may come out as NaN).
+ * Scores, maxima, sums and accumulators are fp32; a weight enters the sum over V as the sum of two bf16 numbers (2^-16 of it lost at most). Without an
+ * output_f32, where a KV head has more than 128 query rows (node x head) and the context is not short (llmi_mha_plan.group_pad 128), it enters as one (2^-8): the
+ * outputs are bf16 themselves. Asking for output_f32 takes the slower form with two there, and output is the rounding of it.
+ * Allocates nothing; safe under stream capture; the workspace needs no initialisation, and two calls that share one must not overlap in time. */
 int llmi_hip_mha_decode_tree(const llmi_mha_tree_args* args);
 /* What llmi_hip_mha_decode_tree would launch (no HIP call): path, num_splits, rows_per_split, waves_per_group and
  * workspace_needed as for llmi_hip_mha_plan; group_pad is the query rows (node x head) of a KV head that one workgroup takes. */

@@ -78,7 +78,7 @@ __device__ __forceinline__ int position(const TreeArgs& a) {
     return __builtin_amdgcn_readfirstlane(a.pos_dev ? max(0, min(*a.pos_dev, a.pos)) : a.pos);
 }
 
-// dma16 without the streaming hint, for tiles that several workgroups read.
+// dma16 without the streaming hint, for tiles that several workgroups read one behind the other.
 __device__ __forceinline__ void dma16_kept(const char* base, uint32_t voff, uint32_t lds_off) {
     const uint64_t b = reinterpret_cast<uint64_t>(base);
     const uint32_t b_lo = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b), b_hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32));
@@ -107,8 +107,8 @@ __device__ __forceinline__ void write_out(const TreeArgs& a, int kvh, int row, i
 }
 
 // WM wavefronts side by side on ROWS query rows each, 4 / WM of them on a tile each of the same rows. EXACT: a probability enters the second
-// product as the sum of two bf16 numbers (relative error 2^-17), otherwise as one (2^-8).
-template <int ROWS, int WM, bool EXACT, int STAGES>
+// product as the sum of two bf16 numbers (relative error 2^-16), otherwise as one (2^-8). KEPT: loads without the streaming hint.
+template <int ROWS, int WM, bool EXACT, int STAGES, bool KEPT>
 // (two workgroups on a compute unit where its LDS holds two rings: a hint without which the accumulators go to AGPRs and back)
 __global__ __launch_bounds__(kWaves * 64, STAGES * (kWaves / WM) * kTileBytes <= 80 * 1024 ? 2 : 1) void mha_tree_kernel(TreeArgs a) {
     constexpr int WK = kWaves / WM;
@@ -188,7 +188,7 @@ __global__ __launch_bounds__(kWaves * 64, STAGES * (kWaves / WM) * kTileBytes <=
                 if constexpr (decltype(whole)::value) base += (int64_t)(4 * b8) * rs;
                 else off += (uint32_t)(min(4 * b8 + rho, last) - rho) * rs;  // rows past the keys repeat the last one: seen by nobody
                 scalar_base(base);
-                if constexpr (EXACT) dma16(base, off, to + (uint32_t)(b * 1024));
+                if constexpr (!KEPT) dma16(base, off, to + (uint32_t)(b * 1024));
                 else dma16_kept(base, off, to + (uint32_t)(b * 1024));
             }
         };
@@ -541,10 +541,10 @@ __global__ __launch_bounds__(W * 64) void mha_tree_join_kernel(TreeArgs a) {
     write_out(a, kvh, block * ROWS + n, slot_column<ROWS>(slot, lane), all, total);
 }
 
-template <int ROWS, int WM, bool EXACT, int STAGES>
+template <int ROWS, int WM, bool EXACT, int STAGES, bool KEPT>
 void launch(const TreeArgs& a, int n_kv, hipStream_t stream) {
     const dim3 grid(n_kv, a.splits, (a.blocks + WM - 1) / WM), block(kWaves * 64);
-    hipLaunchKernelGGL((mha_tree_kernel<ROWS, WM, EXACT, STAGES>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((mha_tree_kernel<ROWS, WM, EXACT, STAGES, KEPT>), grid, block, 0, stream, a);
     if (a.splits == 1) return;
     // (a trip to memory for all splits up to 128)
     const dim3 join(n_kv, kSlots<ROWS>, a.blocks);
@@ -586,12 +586,16 @@ int launch_mha_tree(const llmi_mha_tree_args& args, const TreeForm& form) {
     // at 32768).
     constexpr int kPairsAhead = 6;
     const int pairs = (m.pos + args.node_num) / kKeys / (2 * a.splits);
-    if (form.rows == 16) launch<16, 1, true, 2>(a, n_kv, stream);
-    else if (form.row_waves == 1) launch<32, 1, true, 2>(a, n_kv, stream);
-    else if (form.row_waves == 2 && pairs < kPairsAhead) launch<32, 2, true, 2>(a, n_kv, stream);
-    else if (form.row_waves == 2) launch<32, 2, true, 4>(a, n_kv, stream);
-    else if (form.blocks <= 4) launch<32, 4, true, 4>(a, n_kv, stream);
-    else launch<32, 4, false, 4>(a, n_kv, stream);
+    if (form.rows == 16) launch<16, 1, true, 2, false>(a, n_kv, stream);
+    else if (form.row_waves == 1) launch<32, 1, true, 2, false>(a, n_kv, stream);
+    else if (form.row_waves == 2 && pairs < kPairsAhead) launch<32, 2, true, 2, false>(a, n_kv, stream);
+    else if (form.row_waves == 2) launch<32, 2, true, 4, false>(a, n_kv, stream);
+    else if (form.blocks <= 4) launch<32, 4, true, 4, false>(a, n_kv, stream);
+    // Beyond 128 query rows the matrix cores are the bound: with one bf16 number a probability, half as many of the second product's instructions; a
+    // bf16 output rounds as much by itself. Whoever asks for the fp32 output gets both. us, one : two numbers: 64 nodes of 64 heads, 8 KV heads 35.5 : 41.1
+    // at 8000 positions, 293 : 393 at 131000, 61 nodes of 32 heads 20.7 : 22.6 at 6000, 56.4 : 67.5 at 32768.
+    else if (a.out_f32) launch<32, 4, true, 4, true>(a, n_kv, stream);
+    else launch<32, 4, false, 4, true>(a, n_kv, stream);
     return check_launch();
 }
 
