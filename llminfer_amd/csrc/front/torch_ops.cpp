@@ -455,6 +455,16 @@ LLMI_ENTRY(qkv_gemv) {
 // ---- drafted tokens ----
 // These calls know how long their rows are, and look: a tensor that is shorter than what the call would touch, or that lies on another
 // device than the one the launch goes to, is refused.
+// (Sizes that only a wrong argument makes are products past 64 bits: those stay larger than any tensor.)
+int64_t product(std::initializer_list<int64_t> factors) {
+    int64_t p = 1;
+    for (int64_t f : factors)
+        if (f == 0) return 0;
+    for (int64_t f : factors)
+        if (__builtin_mul_overflow(p, f, &p)) return INT64_MAX;
+    return p;
+}
+
 struct Looked {
     PyObject* const* vals;
     bool ok = true;
@@ -495,7 +505,7 @@ struct Looked {
         *stride = 0;
         if (!ok || absent(key)) return nullptr;
         if (!THPVariable_Check(vals[key]) || !tensor(key).is_cuda() || !type_fits(tensor(key), kind) || tensor(key).dim() != 2)
-            return whole<void>(key, kind, rows * width);
+            return whole<void>(key, kind, product({rows, width}));
         const at::Tensor& t = tensor(key);
         if (!here(key)) return nullptr;
         if (t.size(0) < rows || t.size(1) != width || (width > 1 && t.stride(1) != 1) || (rows > 1 && t.stride(0) < width)) {
@@ -534,8 +544,8 @@ LLMI_ENTRY(mha_decode_tree) {
     if (!ok) return nullptr;
     Looked look(vals);
     t.node_num = int32(vals, k_node_num, 0, &look.ok);
-    const int64_t rows = look.positive(k_node_num) * look.positive(k_head_num) * look.positive(k_head_dim);
-    const int64_t cached = (look.positive(k_layer_id) + 1) * look.positive(k_max_seq_len) * look.positive(k_kv_dim);
+    const int64_t rows = product({look.positive(k_node_num), look.positive(k_head_num), look.positive(k_head_dim)});
+    const int64_t cached = product({look.positive(k_layer_id) + 1, look.positive(k_max_seq_len), look.positive(k_kv_dim)});
     look.whole<void>(k_query, Kind::bf16, rows);
     look.whole<void>(k_key_cache, Kind::bf16, cached);
     look.whole<void>(k_value_cache, Kind::bf16, cached);
@@ -568,9 +578,9 @@ LLMI_ENTRY(qk_norm_rope_append_tree) {
     a.kv_layout = int32(vals, k_kv_layout, LLMI_KV_LAYOUT_POS_MAJOR, &look.ok);
     a.eps = look.number(k_eps, 1e-6f);
     if (!look.ok) return nullptr;
-    const int64_t n = look.positive(k_node_num), dim = look.positive(k_head_num) * look.positive(k_head_dim), kv_dim = look.positive(k_kv_dim);
-    const int64_t cached = (look.positive(k_layer_id) + 1) * look.positive(k_max_seq_len) * kv_dim;
-    const int64_t table = look.positive(k_max_seq_len) * (look.positive(k_head_dim) / 2);
+    const int64_t n = look.positive(k_node_num), dim = product({look.positive(k_head_num), look.positive(k_head_dim)}), kv_dim = look.positive(k_kv_dim);
+    const int64_t cached = product({look.positive(k_layer_id) + 1, look.positive(k_max_seq_len), kv_dim});
+    const int64_t table = product({look.positive(k_max_seq_len), look.positive(k_head_dim) / 2});
     a.query = look.rows(k_query, Kind::bf16, n, dim, &t.query_stride);
     a.query_src = look.rows(k_query_src, Kind::bf16, n, dim, &t.query_src_stride);
     a.key_new = look.rows(k_key_new, Kind::bf16, n, kv_dim, &t.key_new_stride);
@@ -640,7 +650,7 @@ LLMI_ENTRY(kv_commit_tree) {
     a.max_seq_len = int32(vals, k_max_seq_len, 0, &look.ok);
     a.kv_layout = int32(vals, k_kv_layout, LLMI_KV_LAYOUT_POS_MAJOR, &look.ok);
     if (!look.ok) return nullptr;
-    const int64_t cached = look.positive(k_layer_num) * look.positive(k_max_seq_len) * look.positive(k_kv_dim);
+    const int64_t cached = product({look.positive(k_layer_num), look.positive(k_max_seq_len), look.positive(k_kv_dim)});
     a.key_cache = look.whole<void>(k_key_cache, Kind::bf16, cached);
     a.value_cache = look.whole<void>(k_value_cache, Kind::bf16, cached);
     a.path = look.whole<const int32_t>(k_path, Kind::i32, look.positive(k_node_num));
