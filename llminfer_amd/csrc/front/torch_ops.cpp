@@ -14,6 +14,8 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cfloat>
+#include <cmath>
 #include <cstdint>
 #include <initializer_list>
 
@@ -520,7 +522,8 @@ struct Looked {
         if (!ok || !vals[key]) return unset;
         const double v = PyFloat_AsDouble(vals[key]);
         if (PyErr_Occurred()) ok = false;
-        return (float)v;
+        // (a number that fp32 has only as 0 is not 0: no temperature of that size is greedy)
+        return v != 0.0 && (float)v == 0.0f ? std::copysign(FLT_TRUE_MIN, (float)v) : (float)v;
     }
     int64_t positive(Key key) {
         const int32_t v = int32(vals, key, 0, &ok);
