@@ -56,14 +56,17 @@ int tree_splits(const TreeForm& f, int n_kv, int64_t tiles) {
     return splits < 2 ? 1 : (int)splits;
 }
 
+// (64 bits: a bound near the type's largest position has more keys than that with its nodes' tile filled up)
+int64_t tiles_of(const llmi_mha_tree_args* a) { return ((int64_t)a->mha.pos + a->node_num + kTreeKeys - 1) / kTreeKeys; }
+
 int make_form(const llmi_mha_tree_args* a, TreeForm* f) {
     if (int rc = validate_tree(a)) return rc;
     const llmi_mha_args& m = a->mha;
     const int n_kv = m.kv_dim / m.head_dim;
-    const int tiles = (m.pos + a->node_num + kTreeKeys - 1) / kTreeKeys;
+    const int64_t tiles = tiles_of(a);
     *f = tree_blocks(a->node_num * m.kv_mul, n_kv, tiles);
     const size_t room = m.workspace ? m.workspace_bytes / ((size_t)n_kv * f->blocks * tree_split_bytes(*f)) : 0;
-    f->splits = m.num_splits ? std::min(m.num_splits, tiles) : (int)std::min<size_t>(tree_splits(*f, n_kv, tiles), room);
+    f->splits = m.num_splits ? (int)std::min<int64_t>(m.num_splits, tiles) : (int)std::min<size_t>(tree_splits(*f, n_kv, tiles), room);
     if (f->splits < 2) f->splits = 1;
     return f->splits > 1 && (size_t)f->splits > room ? LLMI_ERR_WORKSPACE : LLMI_OK;
 }
@@ -79,11 +82,11 @@ int llmi_hip_mha_tree_plan(const llmi_mha_tree_args* args, llmi_mha_plan* plan) 
     if (!plan) return LLMI_ERR_NULL_POINTER;
     TreeForm f;
     if (int rc = make_form(args, &f)) return rc;
-    const int tiles = (args->mha.pos + args->node_num + kTreeKeys - 1) / kTreeKeys;
+    const int64_t tiles = tiles_of(args);
     *plan = llmi_mha_plan{};
     plan->path = f.splits > 1 ? LLMI_PATH_SPLIT : LLMI_PATH_SINGLE_PASS;
     plan->num_splits = f.splits;
-    plan->rows_per_split = (tiles + f.splits - 1) / f.splits * kTreeKeys;
+    plan->rows_per_split = (int32_t)std::min<int64_t>((tiles + f.splits - 1) / f.splits * kTreeKeys, INT32_MAX);
     plan->waves_per_group = 4;
     plan->group_pad = f.rows * f.row_waves;
     plan->workspace_needed = f.splits > 1 ? (size_t)(args->mha.kv_dim / 128) * f.blocks * f.splits * tree_split_bytes(f) : 0;
