@@ -16,11 +16,13 @@
 //             P^T  lane L: those eight: place 8*(L/16) + j is key 16*(j/4) + 4*(L/16) + j%4
 //             V^T  lane L: column 16*b + L%16 (b = 0..7), keys in that order;  O^T  lane L: query row L%16, columns 16*b + 4*(L/16) + r
 // Tiles lie in LDS as rows of 256 bytes, filled by LDS-DMA loads whose lanes fetch from where the swizzle wants it: K's 16-byte chunks are
-// exchanged by the row's low four bits, V's 32-byte pieces rotated by the row's low three, which spreads every read over the banks.
+// exchanged by the row's low four bits, V's 32-byte pieces rotated by the row's low three. K's reads are spread over the banks by that, and V's in
+// the 16-row form. In the 32-row form half a wavefront of the transposing read takes two neighbouring pieces of four keys, at the places 0 1 2 3 and 1 2 3 4:
+// two cycles a half in place of one (counters: 2.0 conflict cycles a read of V, a third of all LDS cycles).
 //
 // Keys are split over workgroups; a second launch joins the splits. What bounds it: the way to the first product and the join's launch up to a few
 // thousand positions (8 nodes of 32 heads, 8 KV heads at 4099: 10.3 us, 17 MB), memory for few rows (8 nodes at 32768: 29.6 us, 4.5 TB/s), matrix cores and
-// the exponentials between their products for many (64 nodes of 64 heads at 131000: 290 us, 0.95 PFLOP/s).
+// the exponentials between their products for many (64 nodes of 64 heads at 131000: 293 us, 0.94 PFLOP/s).
 
 #include <hip/hip_runtime.h>
 #include <float.h>
@@ -78,7 +80,8 @@ __device__ __forceinline__ int position(const TreeArgs& a) {
     return __builtin_amdgcn_readfirstlane(a.pos_dev ? max(0, min(*a.pos_dev, a.pos)) : a.pos);
 }
 
-// dma16 without the streaming hint, for tiles that several workgroups read one behind the other.
+// dma16 without the streaming hint: for the form whose tiles are always read by several workgroups. (Several blocks of 16 rows read a tile
+// several times too, with the hint: not measured the other way.)
 __device__ __forceinline__ void dma16_kept(const char* base, uint32_t voff, uint32_t lds_off) {
     const uint64_t b = reinterpret_cast<uint64_t>(base);
     const uint32_t b_lo = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b), b_hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32));
@@ -346,7 +349,7 @@ __global__ __launch_bounds__(kWaves * 64, STAGES * (kWaves / WM) * kTileBytes <=
     };
     const int my_tiles = t1 - t0 > wk ? (t1 - t0 - wk + WK - 1) / WK : 0;
     // This wavefront's tile `it` has landed, up to `newer` ones behind it stay in flight; then every wavefront's, and all have read what is
-    // refilled next.
+    // refilled next. (Needed where wavefronts share tiles; with WM == 1 each has its own, and they wait for one another all the same.)
     auto wait_for = [&](int it, int newer) __attribute__((always_inline)) {
         newer = min(newer, my_tiles - 1 - it);
         if (newer >= 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * kLoads) : "memory");
