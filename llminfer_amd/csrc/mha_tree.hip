@@ -80,8 +80,10 @@ __device__ __forceinline__ int position(const TreeArgs& a) {
     return __builtin_amdgcn_readfirstlane(a.pos_dev ? max(0, min(*a.pos_dev, a.pos)) : a.pos);
 }
 
-// dma16 without the streaming hint: for the form whose tiles are always read by several workgroups. (Several blocks of 16 rows read a tile
-// several times too, with the hint: not measured the other way.)
+// dma16 without the streaming hint: for the form of 32 rows whose tiles several workgroups read. Several blocks of 16 rows have the hint though they
+// share tiles as well; us, with it : without, 8 KV heads: 8 nodes of 32 heads 7.3 : 7.3 at 250 positions, 8.5 : 8.7 at 2000, 10.2 : 10.2 at 4099, 26 nodes 8.5 : 8.3 at
+// 500, 61 nodes 10.1 : 9.9 at 500, 5 nodes of 64 heads 10.3 : 10.1 at 3000; 16 nodes of 16 heads, 4 KV heads 13.2 : 11.7 at 8000. So two blocks lose a little without it and
+// more of them gain.
 __device__ __forceinline__ void dma16_kept(const char* base, uint32_t voff, uint32_t lds_off) {
     const uint64_t b = reinterpret_cast<uint64_t>(base);
     const uint32_t b_lo = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b), b_hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32));
