@@ -36,6 +36,8 @@
  *   llmi_hip_mha_decode_tree, llmi_hip_qk_norm_rope_append_tree, llmi_hip_verify_tree,
  *   llmi_hip_kv_commit_tree       (new) one step of speculative decoding: several drafted tokens
  *                                 checked in one pass of the model
+ *   llmi_hip_mha_decode_kv8, llmi_hip_mha_decode_append_kv8, llmi_hip_qk_norm_rope_append_kv8,
+ *   llmi_hip_kv8_store, llmi_hip_kv8_load  (new) a KV cache of 8-bit codes with a scale per row
  *   llmi_pool_* / llmi_hip_pool_* base::CUDADeviceAllocator::allocate / release
  *                                 code/source/base/alloc_cu.cpp:7-119
  *   llmi_hip_memcpy / memset_zero base::DeviceAllocator::memcpy / memset_zero
@@ -417,6 +419,118 @@ typedef struct llmi_kv_commit_tree_args {
 /* In every layer, for i = 1 .. result[0]-1: the K and V rows that stood in slot pos + path[i] before the call to slot pos + i, in
  * place. Entries below i or from node_num on move nothing, every other slot stays as it is. Does not change the position word: add result[0] to it behind this call. */
 int llmi_hip_kv_commit_tree(const llmi_kv_commit_tree_args* args);
+
+/* ---- an 8-bit KV cache -------------------------------------------------------
+ * No counterpart in the reference, whose cache has the model's own type. A row -- the 128 values of a KV head's K or V at one
+ * position, as the bf16 cache holds them -- is kept as 128 codes of 8 bits and a scale s: the smallest number of eight significant bits with
+ * s * top >= the row's largest magnitude, and at least 2^-64 (so a row whose largest magnitude is under top * 2^-64 loses
+ * precision, down to 0). top is 448 for E4M3 codes (1 sign, 4 exponent, 3 mantissa bits), 127 for whole numbers. A code is x / s rounded to
+ * nearest even and stands for code * s. A row with an infinity or NaN is kept as a row of NaN (s = NaN, codes 0).
+ * One buffer holds K, V and scales of all layers, llmi_hip_kv8_bytes() bytes, 16-byte aligned: [layer][KV head][record of 32 positions],
+ * 260 bytes a position and KV head where the bf16 cache has 512. A record is 8320 bytes; with p the position in it, t = p / 16,
+ * g = p / 4 % 4, i = p % 4, and channel c:
+ *   K code at    2048 * t + 256 * (c / 16) + 16 * (p % 16) + c % 16
+ *   V code at    4096 + 1024 * (c / 32) + 256 * g + 16 * (c % 16) + 8 * (c / 16 % 2) + 4 * t + i
+ *   K scale at   8192 + 16 * g + 8 * t + 2 * i, bf16;  V scale 64 bytes behind it
+ * so records can be moved about whole (a prefix kept or dropped at a multiple of 32 positions). Nothing reads what belongs to positions that have
+ * not been written, and the buffer needs no initialisation. max_seq_len is the positions per layer the buffer was sized for. */
+enum { LLMI_KV8_E4M3 = 0, LLMI_KV8_INT8 = 1 };
+#define LLMI_KV8_RECORD_POSITIONS 32
+#define LLMI_KV8_RECORD_BYTES 8320
+
+/* Bytes of the buffer; 0 for sizes that are not possible. */
+size_t llmi_hip_kv8_bytes(int32_t layer_num, int32_t max_seq_len, int32_t kv_dim, int32_t head_dim);
+
+typedef struct llmi_kv8_copy_args {
+    void* key_cache;          /* device bf16, base of the whole cache (layer_num layers), 16-byte aligned                  */
+    void* value_cache;
+    void* cache8;             /* device, the 8-bit cache of the same layers and positions                                 */
+    int32_t layer_num;
+    int32_t first_pos;        /* positions first_pos .. first_pos + num_pos - 1 of every layer and KV head                */
+    int32_t num_pos;
+    int32_t kv_dim;
+    int32_t head_dim;         /* must be 128 */
+    int32_t max_seq_len;      /* of both caches                                                                          */
+    int32_t kv_layout;        /* of the bf16 cache                                                                       */
+    int32_t format;           /* LLMI_KV8_*                                                                              */
+    void* stream;
+} llmi_kv8_copy_args;
+
+/* Rows of a bf16 cache into the 8-bit one (a prompt that was prefilled in bf16, say). Every other position of both stays as it is. */
+int llmi_hip_kv8_store(const llmi_kv8_copy_args* args);
+/* Back: code * s, rounded to bf16 once. Every other position of both stays as it is. */
+int llmi_hip_kv8_load(const llmi_kv8_copy_args* args);
+
+typedef struct llmi_qk_norm_rope_kv8_args {
+    void* query;              /* device bf16 [row_num][head_num*128]: receives the normalised + rotated queries           */
+    const void* query_src;    /* device bf16 raw queries, or NULL = transform `query` in place                            */
+    const void* key_new;      /* device bf16 [row_num][kv_dim]: the tokens' raw K rows                                    */
+    const void* value_new;    /* device bf16 [row_num][kv_dim]                                                            */
+    void* cache8;             /* rows (layer_id, pos .. pos + row_num - 1) are written                                    */
+    const void* norm_weight;  /* device bf16 [2*128]: q_norm then k_norm                                                  */
+    const float* sin_cache;   /* device fp32 [max_seq_len][64]                                                            */
+    const float* cos_cache;
+    const int32_t* pos_device; /* optional, device int32: the first position read at run time, clamped to 0..pos          */
+    int32_t layer_id;
+    int32_t pos;              /* position of the first token                                                              */
+    int32_t row_num;          /* tokens, >= 1                                                                             */
+    int32_t kv_dim;
+    int32_t head_num;
+    int32_t head_dim;         /* must be 128 */
+    int32_t max_seq_len;
+    int32_t format;           /* LLMI_KV8_*                                                                               */
+    float eps;
+    /* elements between one token's row and the next; multiples of 8; 0 = rows lie one behind the other */
+    int64_t query_stride, query_src_stride, key_new_stride, value_new_stride;
+    void* stream;
+} llmi_qk_norm_rope_kv8_args;
+
+/* llmi_hip_qk_norm_rope_append for consecutive tokens and an 8-bit cache: K rows are normalised, rotated and rounded to bf16 as there (what the bf16
+ * cache would hold; the bits of llmi_hip_mha_decode_append), then quantised; V rows are quantised as they are. One launch, no allocation. */
+int llmi_hip_qk_norm_rope_append_kv8(const llmi_qk_norm_rope_kv8_args* args);
+
+typedef struct llmi_mha_kv8_args {
+    const void* query;        /* device, bf16 [head_num*128]                                          */
+    void* cache8;             /* device, base of the 8-bit cache (all layers)                         */
+    void* workspace;          /* device, 16-byte aligned; may be NULL: one workgroup per KV head then */
+    size_t workspace_bytes;   /* llmi_hip_mha_workspace_bytes() is enough for any length              */
+    void* output;             /* device, bf16 [head_num*128]                                          */
+    float* output_f32;        /* optional device fp32 [head_num*128]: the result before its rounding  */
+    int32_t layer_id;
+    int32_t pos;              /* attends to positions 0..pos                                          */
+    int32_t kv_dim;
+    int32_t kv_mul;           /* query heads per KV head, 1..16                                       */
+    int32_t head_num;
+    int32_t head_dim;         /* must be 128                                                          */
+    int32_t max_seq_len;
+    int32_t format;           /* LLMI_KV8_*                                                           */
+    int32_t num_splits;       /* 0 = auto; otherwise the workgroups a KV head's positions are dealt to at most */
+    void* stream;
+    const int32_t* pos_device; /* optional, device int32: the position read at run time, clamped to 0..pos; `pos` sizes the launch */
+} llmi_mha_kv8_args;
+
+/* llmi_hip_mha_decode over an 8-bit cache: K and V are what the codes stand for, scores, maxima, sums and accumulators fp32, a weight times V's
+ * scale enters the sum over V as the sum of two bf16 numbers (2^-16 of it lost at most). One launch whose last workgroup of a KV head waits (bounded:
+ * llmi_hip_set_poll_limit) for the others'. Allocates nothing; safe under stream capture; the workspace needs no initialisation, and two calls that
+ * share one must not overlap in time. */
+int llmi_hip_mha_decode_kv8(const llmi_mha_kv8_args* args);
+/* What it would launch (no HIP call): as llmi_hip_mha_plan; group_pad is 16. */
+int llmi_hip_mha_kv8_plan(const llmi_mha_kv8_args* args, llmi_mha_plan* plan);
+
+typedef struct llmi_mha_kv8_append_args {
+    llmi_mha_kv8_args mha;    /* as for llmi_hip_mha_decode_kv8, except: query is the RAW query of the new token, and the row (layer_id, pos) of
+                                 the cache is written                                                 */
+    const void* key_new;      /* device bf16 [kv_dim]: the new token's raw K row                      */
+    const void* value_new;    /* device bf16 [kv_dim]                                                 */
+    const void* norm_weight;  /* device bf16 [2*128]: q_norm then k_norm                              */
+    const float* sin_cache;   /* device fp32 [max_seq_len][64]                                        */
+    const float* cos_cache;
+    float eps;
+} llmi_mha_kv8_append_args;
+
+/* llmi_hip_qk_norm_rope_append_kv8 for one token, then llmi_hip_mha_decode_kv8, as one launch: the same cache bytes, the new token taken as its codes
+ * stand for it. The normalised query is not written back. */
+int llmi_hip_mha_decode_append_kv8(const llmi_mha_kv8_append_args* args);
 
 /* ---- pooled device allocator ------------------------------------------- */
 

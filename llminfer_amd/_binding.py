@@ -114,6 +114,40 @@ class KvCommitTreeArgs(ctypes.Structure):
     ]
 
 
+class Kv8CopyArgs(ctypes.Structure):
+    _fields_ = [
+        ("key_cache", c_void_p), ("value_cache", c_void_p), ("cache8", c_void_p),
+        ("layer_num", c_i32), ("first_pos", c_i32), ("num_pos", c_i32), ("kv_dim", c_i32), ("head_dim", c_i32), ("max_seq_len", c_i32),
+        ("kv_layout", c_i32), ("format", c_i32), ("stream", c_void_p),
+    ]
+
+
+class QkNormRopeKv8Args(ctypes.Structure):
+    _fields_ = [
+        ("query", c_void_p), ("query_src", c_void_p), ("key_new", c_void_p), ("value_new", c_void_p), ("cache8", c_void_p),
+        ("norm_weight", c_void_p), ("sin_cache", c_void_p), ("cos_cache", c_void_p), ("pos_device", c_void_p),
+        ("layer_id", c_i32), ("pos", c_i32), ("row_num", c_i32), ("kv_dim", c_i32), ("head_num", c_i32), ("head_dim", c_i32),
+        ("max_seq_len", c_i32), ("format", c_i32), ("eps", ctypes.c_float),
+        ("query_stride", ctypes.c_int64), ("query_src_stride", ctypes.c_int64), ("key_new_stride", ctypes.c_int64),
+        ("value_new_stride", ctypes.c_int64), ("stream", c_void_p),
+    ]
+
+
+class MhaKv8Args(ctypes.Structure):
+    _fields_ = [
+        ("query", c_void_p), ("cache8", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("output", c_void_p),
+        ("output_f32", c_void_p), ("layer_id", c_i32), ("pos", c_i32), ("kv_dim", c_i32), ("kv_mul", c_i32), ("head_num", c_i32),
+        ("head_dim", c_i32), ("max_seq_len", c_i32), ("format", c_i32), ("num_splits", c_i32), ("stream", c_void_p), ("pos_device", c_void_p),
+    ]
+
+
+class MhaKv8AppendArgs(ctypes.Structure):
+    _fields_ = [("mha", MhaKv8Args), ("key_new", c_void_p), ("value_new", c_void_p), ("norm_weight", c_void_p), ("sin_cache", c_void_p),
+                ("cos_cache", c_void_p), ("eps", ctypes.c_float)]
+
+
+KV8_E4M3, KV8_INT8 = 0, 1
+KV8_RECORD_POSITIONS, KV8_RECORD_BYTES = 32, 8320
 TREE_MAX_NODES = 64
 LOGITS_F32, LOGITS_BF16 = 0, 1
 
@@ -156,6 +190,13 @@ SYMBOLS = {
     "llmi_hip_verify_tree": (ctypes.c_int, [ctypes.POINTER(VerifyTreeArgs)]),
     "llmi_hip_verify_tree_workspace_bytes": (c_size_t, [c_i32, c_i32]),
     "llmi_hip_kv_commit_tree": (ctypes.c_int, [ctypes.POINTER(KvCommitTreeArgs)]),
+    "llmi_hip_kv8_bytes": (c_size_t, [c_i32, c_i32, c_i32, c_i32]),
+    "llmi_hip_kv8_store": (ctypes.c_int, [ctypes.POINTER(Kv8CopyArgs)]),
+    "llmi_hip_kv8_load": (ctypes.c_int, [ctypes.POINTER(Kv8CopyArgs)]),
+    "llmi_hip_qk_norm_rope_append_kv8": (ctypes.c_int, [ctypes.POINTER(QkNormRopeKv8Args)]),
+    "llmi_hip_mha_decode_kv8": (ctypes.c_int, [ctypes.POINTER(MhaKv8Args)]),
+    "llmi_hip_mha_kv8_plan": (ctypes.c_int, [ctypes.POINTER(MhaKv8Args), ctypes.POINTER(MhaPlan)]),
+    "llmi_hip_mha_decode_append_kv8": (ctypes.c_int, [ctypes.POINTER(MhaKv8AppendArgs)]),
     "llmi_hip_gemv": (ctypes.c_int, [ctypes.POINTER(GemvArgs)]),
     "llmi_hip_qkv_gemv": (ctypes.c_int, [ctypes.POINTER(QkvGemvArgs)]),
     "llmi_pool_create": (c_void_p, [BACKING_ALLOC_FN, BACKING_FREE_FN, c_void_p]),

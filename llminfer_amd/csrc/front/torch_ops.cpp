@@ -31,7 +31,7 @@ namespace {
     X(residual) X(one_launch) X(layer_count) X(query_stride) X(key_new_stride) X(value_new_stride) X(norm_weight_stride)         \
     X(output_stride) X(query_src) X(input) X(weight) X(mode) X(key) X(value) X(src_pos_major) X(dst_head_major) X(layer_num)     \
     X(num_pos) X(tree_mask) X(node_num) X(depth) X(target_logits) X(draft_logits) X(tokens) X(parents) X(uniform) X(path)         \
-    X(result) X(temperature)
+    X(result) X(temperature) X(cache8) X(kv8_format) X(first_pos) X(row_num)
 
 enum Key : int {
 #define X(name) k_##name,
@@ -131,21 +131,27 @@ struct Abi {
     int (*qk_norm_rope_append_tree)(const llmi_qk_norm_rope_tree_args*);
     int (*verify_tree)(const llmi_verify_tree_args*);
     int (*kv_commit_tree)(const llmi_kv_commit_tree_args*);
+    int (*kv8_store)(const llmi_kv8_copy_args*);
+    int (*kv8_load)(const llmi_kv8_copy_args*);
+    int (*qk_norm_rope_append_kv8)(const llmi_qk_norm_rope_kv8_args*);
+    int (*mha_decode_kv8)(const llmi_mha_kv8_args*);
+    int (*mha_decode_append_kv8)(const llmi_mha_kv8_append_args*);
 } g_abi;
 PyObject *g_get_device, *g_get_stream;   // torch's current device, and its current stream as a number
 PyObject *g_check_dev, *g_check_status;  // ops._check_dev, _binding.check: they raise
-PyObject *g_bf16_types, *g_f32_types, *g_i32_types, *g_i64_types;  // what _check_dev is told to expect
+PyObject *g_bf16_types, *g_f32_types, *g_i32_types, *g_i64_types, *g_u8_types;  // what _check_dev is told to expect
 
 // ---- conversions ----
-enum class Kind { bf16, f32, i32, i64 };
+enum class Kind { bf16, f32, i32, i64, u8 };
 
 PyObject* types_of(Kind kind) {
-    return kind == Kind::f32 ? g_f32_types : kind == Kind::i32 ? g_i32_types : kind == Kind::i64 ? g_i64_types : g_bf16_types;
+    return kind == Kind::f32 ? g_f32_types : kind == Kind::i32 ? g_i32_types : kind == Kind::i64 ? g_i64_types : kind == Kind::u8 ? g_u8_types : g_bf16_types;
 }
 
 inline bool type_fits(const at::Tensor& t, Kind kind) {
     const at::ScalarType s = t.scalar_type();
     if (kind == Kind::i32) return s == at::kInt;
+    if (kind == Kind::u8) return s == at::kByte;
     if (kind == Kind::i64) return s == at::kLong || s == at::ScalarType::UInt64;
     return kind == Kind::f32 ? s == at::kFloat : s == at::kBFloat16 || s == at::kShort || s == at::ScalarType::UInt16;
 }
@@ -664,10 +670,149 @@ LLMI_ENTRY(kv_commit_tree) {
     Py_RETURN_NONE;
 }
 
-// bind(functions, get_device, get_stream, check_dev, check_status, bf16_types, f32_types, i32_types, i64_types); functions: C ABI name -> address
+// ---- an 8-bit KV cache ----
+// Bytes of the cache up to and with `layers` layers of it, larger than any tensor where they pass 64 bits.
+int64_t kv8_size(Looked& look, int64_t layers) {
+    const int64_t records = (look.positive(k_max_seq_len) + LLMI_KV8_RECORD_POSITIONS - 1) / LLMI_KV8_RECORD_POSITIONS;
+    return product({layers, look.positive(k_kv_dim) / 128, records, LLMI_KV8_RECORD_BYTES});
+}
+
+constexpr Key kKv8StorePos[] = {k_key_cache, k_value_cache, k_cache8}, kKv8LoadPos[] = {k_cache8, k_key_cache, k_value_cache};
+constexpr uint64_t kKv8CopyKeywords = bits({k_layer_num, k_num_pos, k_first_pos, k_kv_dim, k_head_dim, k_max_seq_len, k_kv_layout, k_kv8_format, k_stream});
+constexpr uint64_t kKv8CopyRequired = bits({k_key_cache, k_value_cache, k_cache8, k_layer_num, k_num_pos, k_kv_dim, k_head_dim, k_max_seq_len});
+const Signature kKv8StoreSig = {"kv8_store", kKv8StorePos, 3, kKv8CopyKeywords, kKv8CopyRequired};
+const Signature kKv8LoadSig = {"kv8_load", kKv8LoadPos, 3, kKv8CopyKeywords, kKv8CopyRequired};
+
+bool fill_kv8_copy(PyObject* const* vals, llmi_kv8_copy_args* a) {
+    Looked look(vals);
+    a->layer_num = int32(vals, k_layer_num, 0, &look.ok);
+    a->first_pos = int32(vals, k_first_pos, 0, &look.ok);
+    a->num_pos = int32(vals, k_num_pos, 0, &look.ok);
+    a->kv_dim = int32(vals, k_kv_dim, 0, &look.ok);
+    a->head_dim = int32(vals, k_head_dim, 0, &look.ok);
+    a->max_seq_len = int32(vals, k_max_seq_len, 0, &look.ok);
+    a->kv_layout = int32(vals, k_kv_layout, LLMI_KV_LAYOUT_POS_MAJOR, &look.ok);
+    a->format = int32(vals, k_kv8_format, LLMI_KV8_E4M3, &look.ok);
+    if (!look.ok) return false;
+    const int64_t layers = look.positive(k_layer_num), rows = product({layers, look.positive(k_max_seq_len), look.positive(k_kv_dim)});
+    a->key_cache = look.whole<void>(k_key_cache, Kind::bf16, rows);
+    a->value_cache = look.whole<void>(k_value_cache, Kind::bf16, rows);
+    a->cache8 = look.whole<void>(k_cache8, Kind::u8, kv8_size(look, layers));
+    a->stream = stream_of(vals, &look.ok);
+    return look.ok;
+}
+
+LLMI_ENTRY(kv8_store) {
+    LLMI_PARSE(kKv8StoreSig);
+    llmi_kv8_copy_args a{};
+    if (!fill_kv8_copy(vals, &a) || !call("llmi_hip_kv8_store", [&] { return g_abi.kv8_store(&a); })) return nullptr;
+    return Py_NewRef(vals[k_cache8]);
+}
+
+LLMI_ENTRY(kv8_load) {
+    LLMI_PARSE(kKv8LoadSig);
+    llmi_kv8_copy_args a{};
+    if (!fill_kv8_copy(vals, &a) || !call("llmi_hip_kv8_load", [&] { return g_abi.kv8_load(&a); })) return nullptr;
+    Py_RETURN_NONE;
+}
+
+constexpr Key kNormRopeKv8Pos[] = {k_query, k_key_new, k_value_new, k_cache8, k_norm_weight, k_sin_cache, k_cos_cache};
+const Signature kNormRopeKv8Sig = {
+    "qk_norm_rope_append_kv8", kNormRopeKv8Pos, 7,
+    bits({k_row_num, k_layer_id, k_pos, k_kv_dim, k_head_num, k_head_dim, k_max_seq_len, k_kv8_format, k_eps, k_query_src, k_pos_device, k_stream}),
+    bits({k_query, k_key_new, k_value_new, k_cache8, k_norm_weight, k_sin_cache, k_cos_cache, k_row_num, k_layer_id, k_pos, k_kv_dim, k_head_num,
+          k_head_dim, k_max_seq_len})};
+LLMI_ENTRY(qk_norm_rope_append_kv8) {
+    LLMI_PARSE(kNormRopeKv8Sig);
+    Looked look(vals);
+    llmi_qk_norm_rope_kv8_args a{};
+    a.layer_id = int32(vals, k_layer_id, 0, &look.ok);
+    a.pos = int32(vals, k_pos, 0, &look.ok);
+    a.row_num = int32(vals, k_row_num, 0, &look.ok);
+    a.kv_dim = int32(vals, k_kv_dim, 0, &look.ok);
+    a.head_num = int32(vals, k_head_num, 0, &look.ok);
+    a.head_dim = int32(vals, k_head_dim, 0, &look.ok);
+    a.max_seq_len = int32(vals, k_max_seq_len, 0, &look.ok);
+    a.format = int32(vals, k_kv8_format, LLMI_KV8_E4M3, &look.ok);
+    a.eps = look.number(k_eps, 1e-6f);
+    if (!look.ok) return nullptr;
+    const int64_t n = look.positive(k_row_num), dim = product({look.positive(k_head_num), look.positive(k_head_dim)}), kv_dim = look.positive(k_kv_dim);
+    const int64_t table = product({look.positive(k_max_seq_len), look.positive(k_head_dim) / 2});
+    a.query = look.rows(k_query, Kind::bf16, n, dim, &a.query_stride);
+    a.query_src = look.rows(k_query_src, Kind::bf16, n, dim, &a.query_src_stride);
+    a.key_new = look.rows(k_key_new, Kind::bf16, n, kv_dim, &a.key_new_stride);
+    a.value_new = look.rows(k_value_new, Kind::bf16, n, kv_dim, &a.value_new_stride);
+    a.cache8 = look.whole<void>(k_cache8, Kind::u8, kv8_size(look, look.positive(k_layer_id) + 1));
+    a.norm_weight = look.whole<const void>(k_norm_weight, Kind::bf16, 2 * look.positive(k_head_dim));
+    a.sin_cache = look.whole<const float>(k_sin_cache, Kind::f32, table);
+    a.cos_cache = look.whole<const float>(k_cos_cache, Kind::f32, table);
+    a.pos_device = look.position();
+    a.stream = stream_of(vals, &look.ok);
+    if (!look.ok || !call("llmi_hip_qk_norm_rope_append_kv8", [&] { return g_abi.qk_norm_rope_append_kv8(&a); })) return nullptr;
+    Py_RETURN_NONE;
+}
+
+constexpr uint64_t kMhaKv8Keywords =
+    bits({k_stream, k_layer_id, k_pos, k_kv_dim, k_kv_mul, k_head_num, k_head_dim, k_max_seq_len, k_kv8_format, k_num_splits, k_output_f32, k_pos_device});
+void fill_mha_kv8(Looked& look, Key query, llmi_mha_kv8_args* a) {
+    PyObject* const* vals = look.vals;
+    a->layer_id = int32(vals, k_layer_id, 0, &look.ok);
+    a->pos = int32(vals, k_pos, 0, &look.ok);
+    a->kv_dim = int32(vals, k_kv_dim, 0, &look.ok);
+    a->kv_mul = int32(vals, k_kv_mul, 0, &look.ok);
+    a->head_num = int32(vals, k_head_num, 0, &look.ok);
+    a->head_dim = int32(vals, k_head_dim, 0, &look.ok);
+    a->max_seq_len = int32(vals, k_max_seq_len, 0, &look.ok);
+    a->format = int32(vals, k_kv8_format, LLMI_KV8_E4M3, &look.ok);
+    a->num_splits = int32(vals, k_num_splits, 0, &look.ok);
+    if (!look.ok) return;
+    const int64_t dim = product({look.positive(k_head_num), look.positive(k_head_dim)});
+    a->query = look.whole<const void>(query, Kind::bf16, dim);
+    a->cache8 = look.whole<void>(k_cache8, Kind::u8, kv8_size(look, look.positive(k_layer_id) + 1));
+    a->output = look.whole<void>(k_output, Kind::bf16, dim);
+    a->output_f32 = look.whole<float>(k_output_f32, Kind::f32, dim);
+    a->workspace = look.whole<void>(k_workspace, Kind::f32, 0);
+    if (a->workspace) a->workspace_bytes = look.tensor(k_workspace).nbytes();
+    a->pos_device = look.position();
+    a->stream = stream_of(vals, &look.ok);
+}
+
+constexpr Key kDecodeKv8Pos[] = {k_query, k_cache8, k_output, k_workspace};
+const Signature kDecodeKv8Sig = {"mha_decode_kv8", kDecodeKv8Pos, 4, kMhaKv8Keywords, kMhaRequired | bits({k_query, k_cache8, k_output, k_workspace})};
+LLMI_ENTRY(mha_decode_kv8) {
+    LLMI_PARSE(kDecodeKv8Sig);
+    Looked look(vals);
+    llmi_mha_kv8_args a{};
+    fill_mha_kv8(look, k_query, &a);
+    if (!look.ok || !call("llmi_hip_mha_decode_kv8", [&] { return g_abi.mha_decode_kv8(&a); })) return nullptr;
+    return Py_NewRef(vals[k_output]);
+}
+
+constexpr Key kAppendKv8Pos[] = {k_query_raw, k_key_new, k_value_new, k_norm_weight, k_sin_cache, k_cos_cache, k_cache8, k_output, k_workspace};
+const Signature kAppendKv8Sig = {
+    "mha_decode_append_kv8", kAppendKv8Pos, 9, kMhaKv8Keywords | bits({k_eps}),
+    kMhaRequired | bits({k_query_raw, k_key_new, k_value_new, k_norm_weight, k_sin_cache, k_cos_cache, k_cache8, k_output, k_workspace})};
+LLMI_ENTRY(mha_decode_append_kv8) {
+    LLMI_PARSE(kAppendKv8Sig);
+    Looked look(vals);
+    llmi_mha_kv8_append_args t{};
+    fill_mha_kv8(look, k_query_raw, &t.mha);
+    t.eps = look.number(k_eps, 1e-6f);
+    if (!look.ok) return nullptr;
+    const int64_t kv_dim = look.positive(k_kv_dim), table = product({look.positive(k_max_seq_len), look.positive(k_head_dim) / 2});
+    t.key_new = look.whole<const void>(k_key_new, Kind::bf16, kv_dim);
+    t.value_new = look.whole<const void>(k_value_new, Kind::bf16, kv_dim);
+    t.norm_weight = look.whole<const void>(k_norm_weight, Kind::bf16, 2 * look.positive(k_head_dim));
+    t.sin_cache = look.whole<const float>(k_sin_cache, Kind::f32, table);
+    t.cos_cache = look.whole<const float>(k_cos_cache, Kind::f32, table);
+    if (!look.ok || !call("llmi_hip_mha_decode_append_kv8", [&] { return g_abi.mha_decode_append_kv8(&t); })) return nullptr;
+    return Py_NewRef(vals[k_output]);
+}
+
+// bind(functions, get_device, get_stream, check_dev, check_status, bf16_types, f32_types, i32_types, i64_types, u8_types); functions: C ABI name -> address
 PyObject* bind(PyObject*, PyObject* args) {
-    PyObject *functions, *objs[8];
-    if (!PyArg_ParseTuple(args, "O!OOOOOOOO", &PyDict_Type, &functions, &objs[0], &objs[1], &objs[2], &objs[3], &objs[4], &objs[5], &objs[6], &objs[7]))
+    PyObject *functions, *objs[9];
+    if (!PyArg_ParseTuple(args, "O!OOOOOOOOO", &PyDict_Type, &functions, &objs[0], &objs[1], &objs[2], &objs[3], &objs[4], &objs[5], &objs[6], &objs[7], &objs[8]))
         return nullptr;
     struct {
         const char* name;
@@ -685,7 +830,12 @@ PyObject* bind(PyObject*, PyObject* args) {
                   {"llmi_hip_mha_decode_tree", &g_abi.mha_decode_tree},
                   {"llmi_hip_qk_norm_rope_append_tree", &g_abi.qk_norm_rope_append_tree},
                   {"llmi_hip_verify_tree", &g_abi.verify_tree},
-                  {"llmi_hip_kv_commit_tree", &g_abi.kv_commit_tree}};
+                  {"llmi_hip_kv_commit_tree", &g_abi.kv_commit_tree},
+                  {"llmi_hip_kv8_store", &g_abi.kv8_store},
+                  {"llmi_hip_kv8_load", &g_abi.kv8_load},
+                  {"llmi_hip_qk_norm_rope_append_kv8", &g_abi.qk_norm_rope_append_kv8},
+                  {"llmi_hip_mha_decode_kv8", &g_abi.mha_decode_kv8},
+                  {"llmi_hip_mha_decode_append_kv8", &g_abi.mha_decode_append_kv8}};
     for (const auto& w : wanted) {
         PyObject* n = PyDict_GetItemString(functions, w.name);  // borrowed
         void* p = n ? PyLong_AsVoidPtr(n) : nullptr;
@@ -696,8 +846,8 @@ PyObject* bind(PyObject*, PyObject* args) {
         }
         *static_cast<void**>(w.slot) = p;
     }
-    PyObject** const keep[] = {&g_get_device, &g_get_stream, &g_check_dev, &g_check_status, &g_bf16_types, &g_f32_types, &g_i32_types, &g_i64_types};
-    for (int i = 0; i < 8; ++i) {
+    PyObject** const keep[] = {&g_get_device, &g_get_stream, &g_check_dev, &g_check_status, &g_bf16_types, &g_f32_types, &g_i32_types, &g_i64_types, &g_u8_types};
+    for (int i = 0; i < 9; ++i) {
         Py_INCREF(objs[i]);
         Py_XSETREF(*keep[i], objs[i]);
     }
@@ -766,6 +916,26 @@ PyMethodDef g_methods[] = {
                 "($module, key_cache, value_cache, path, result, *, node_num, layer_num, pos, kv_dim, head_dim, max_seq_len, kv_layout=0, "
                 "pos_device=None, stream=None)",
                 "The accepted nodes' K and V rows to consecutive slots from pos on, in all layers (llmi_hip_kv_commit_tree)."),
+    LLMI_METHOD(kv8_store, "($module, key_cache, value_cache, cache8, *, layer_num, num_pos, kv_dim, head_dim, max_seq_len, first_pos=0, kv_layout=0, "
+                           "kv8_format=0, stream=None)",
+                "Positions first_pos .. first_pos + num_pos - 1 of a bf16 cache, all layers, into the 8-bit cache `cache8` (uint8, kv8_bytes() of\n"
+                "them) as E4M3 (0) or whole-number (1) codes with a scale per row (llmi_hip_kv8_store); returns cache8."),
+    LLMI_METHOD(kv8_load, "($module, cache8, key_cache, value_cache, *, layer_num, num_pos, kv_dim, head_dim, max_seq_len, first_pos=0, kv_layout=0, "
+                          "kv8_format=0, stream=None)",
+                "The same positions back into a bf16 cache (llmi_hip_kv8_load)."),
+    LLMI_METHOD(qk_norm_rope_append_kv8,
+                "($module, query, key_new, value_new, cache8, norm_weight, sin_cache, cos_cache, *, row_num, layer_id, pos, kv_dim, head_num, head_dim, "
+                "max_seq_len, kv8_format=0, eps=1e-06, query_src=None, pos_device=None, stream=None)",
+                "QK-Norm + RoPE of row_num tokens from position pos on, their K and V rows quantised into the 8-bit cache\n"
+                "(llmi_hip_qk_norm_rope_append_kv8). The rows of query, query_src, key_new and value_new may be slices of wider ones."),
+    LLMI_METHOD(mha_decode_kv8,
+                "($module, query, cache8, output, workspace, *, stream=None, layer_id, pos, kv_dim, kv_mul, head_num, head_dim, max_seq_len, "
+                "kv8_format=0, num_splits=0, output_f32=None, pos_device=None)",
+                "Decode attention for one layer / one token over an 8-bit cache (llmi_hip_mha_decode_kv8); returns the output."),
+    LLMI_METHOD(mha_decode_append_kv8,
+                "($module, query_raw, key_new, value_new, norm_weight, sin_cache, cos_cache, cache8, output, workspace, *, eps=1e-06, stream=None, "
+                "layer_id, pos, kv_dim, kv_mul, head_num, head_dim, max_seq_len, kv8_format=0, num_splits=0, output_f32=None, pos_device=None)",
+                "qk_norm_rope_append_kv8 for one token and mha_decode_kv8 as one kernel (llmi_hip_mha_decode_append_kv8); returns the output."),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_torch_ops", "Native calls of llminfer_amd.ops.", -1, g_methods};

@@ -1,0 +1,150 @@
+// C ABI of the calls for an 8-bit KV cache (include/llmi_hip.h): argument validation and the split rule of its attention. The kernels
+// live in mha_kv8.hip and kv8_rows.hip.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "llmi_hip.h"
+#include "llmi_internal.h"
+
+namespace llmi {
+namespace {
+
+// KV heads are a grid dimension.
+constexpr int kMostKvHeads = 65535;
+
+inline bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+bool is_format(int32_t f) { return f == LLMI_KV8_E4M3 || f == LLMI_KV8_INT8; }
+
+int validate_dims(int32_t head_dim, int32_t kv_dim, int32_t max_seq_len, int32_t format) {
+    if (head_dim != 128) return LLMI_ERR_HEAD_DIM;
+    if (kv_dim <= 0 || kv_dim % head_dim != 0) return LLMI_ERR_KV_DIM;
+    if (kv_dim / head_dim > kMostKvHeads || max_seq_len <= 0 || !is_format(format)) return LLMI_ERR_INVALID_ARG;
+    return LLMI_OK;
+}
+
+int validate(const llmi_mha_kv8_args* a) {
+    if (!a) return LLMI_ERR_NULL_POINTER;
+    if (!a->query || !a->cache8 || !a->output) return LLMI_ERR_NULL_POINTER;
+    if (int rc = validate_dims(a->head_dim, a->kv_dim, a->max_seq_len, a->format)) return rc;
+    if (a->kv_mul < 1 || a->kv_mul > kMaxGroup || a->head_num != a->kv_mul * (a->kv_dim / a->head_dim)) return LLMI_ERR_HEAD_GROUP;
+    if (a->layer_id < 0 || a->num_splits < 0 || a->num_splits > kMaxSplits) return LLMI_ERR_INVALID_ARG;
+    if (a->pos < 0 || a->pos >= a->max_seq_len) return LLMI_ERR_POS_RANGE;
+    if (!aligned(a->query, 16) || !aligned(a->cache8, 16) || !aligned(a->output, 16) || !aligned(a->workspace, 16) || !aligned(a->output_f32, 4) ||
+        !aligned(a->pos_device, 4))
+        return LLMI_ERR_ALIGNMENT;
+    return LLMI_OK;
+}
+
+size_t split_bytes(const llmi_mha_kv8_args* a) { return (size_t)a->head_num * (128 * sizeof(float) + 2 * sizeof(unsigned long long)); }
+
+// The workgroups a KV head's records are dealt to: a record for each wavefront, up to two workgroups per compute unit.
+int make_splits(const llmi_mha_kv8_args* a, int new_rows, int* splits) {
+    if (int rc = validate(a)) return rc;
+    const int64_t keys = (int64_t)a->pos + 1 - new_rows, tiles = (keys + 31) / 32;
+    const int64_t most = std::max<int64_t>(1, (tiles + kKv8Waves - 1) / kKv8Waves);
+    // (partial outputs are addressed with 31 bits)
+    const size_t room = a->workspace ? std::min(a->workspace_bytes > 16 ? a->workspace_bytes - 16 : 0, (size_t)INT32_MAX) / split_bytes(a) : 0;
+    int64_t want = a->num_splits;
+    if (want == 0) {
+        want = std::min<int64_t>(std::max(512 / (a->kv_dim / 128), 1), kMaxSplits);
+        want = std::min<int64_t>({want, most, (int64_t)room});
+    } else {
+        want = std::min(want, most);
+        if (want > 1 && (size_t)want > room) return LLMI_ERR_WORKSPACE;
+    }
+    *splits = (int)std::max<int64_t>(want, 1);
+    return LLMI_OK;
+}
+
+int validate_copy(const llmi_kv8_copy_args* a) {
+    if (!a) return LLMI_ERR_NULL_POINTER;
+    if (!a->key_cache || !a->value_cache || !a->cache8) return LLMI_ERR_NULL_POINTER;
+    if (int rc = validate_dims(a->head_dim, a->kv_dim, a->max_seq_len, a->format)) return rc;
+    if (a->layer_num < 0) return LLMI_ERR_INVALID_ARG;
+    if (a->first_pos < 0 || a->num_pos < 0 || a->first_pos > a->max_seq_len || a->num_pos > a->max_seq_len - a->first_pos) return LLMI_ERR_POS_RANGE;
+    if (a->kv_layout != LLMI_KV_LAYOUT_POS_MAJOR && a->kv_layout != LLMI_KV_LAYOUT_HEAD_MAJOR) return LLMI_ERR_LAYOUT;
+    if (!aligned(a->key_cache, 16) || !aligned(a->value_cache, 16) || !aligned(a->cache8, 16)) return LLMI_ERR_ALIGNMENT;
+    return LLMI_OK;
+}
+
+}  // namespace
+}  // namespace llmi
+
+using namespace llmi;
+
+extern "C" {
+
+size_t llmi_hip_kv8_bytes(int32_t layer_num, int32_t max_seq_len, int32_t kv_dim, int32_t head_dim) {
+    if (layer_num <= 0 || max_seq_len <= 0 || head_dim != 128 || kv_dim <= 0 || kv_dim % 128 != 0) return 0;
+    size_t n = (size_t)kv8_records(max_seq_len) * kKv8Record;
+    if (__builtin_mul_overflow(n, (size_t)(kv_dim / 128), &n) || __builtin_mul_overflow(n, (size_t)layer_num, &n)) return 0;
+    return n;
+}
+
+int llmi_hip_kv8_store(const llmi_kv8_copy_args* args) {
+    if (int rc = validate_copy(args)) return rc;
+    return launch_kv8_store(*args);
+}
+
+int llmi_hip_kv8_load(const llmi_kv8_copy_args* args) {
+    if (int rc = validate_copy(args)) return rc;
+    return launch_kv8_load(*args);
+}
+
+int llmi_hip_qk_norm_rope_append_kv8(const llmi_qk_norm_rope_kv8_args* a) {
+    if (!a) return LLMI_ERR_NULL_POINTER;
+    if (!a->query || !a->key_new || !a->value_new || !a->cache8 || !a->norm_weight || !a->sin_cache || !a->cos_cache) return LLMI_ERR_NULL_POINTER;
+    if (int rc = validate_dims(a->head_dim, a->kv_dim, a->max_seq_len, a->format)) return rc;
+    if (a->head_num <= 0 || a->head_num > kMaxGroup * kMostKvHeads || a->layer_id < 0 || a->row_num < 1 || !(a->eps >= 0.0f)) return LLMI_ERR_INVALID_ARG;
+    if (a->pos < 0 || a->row_num > a->max_seq_len || a->pos > a->max_seq_len - a->row_num) return LLMI_ERR_POS_RANGE;
+    const void* rows[] = {a->query, a->query_src, a->key_new, a->value_new, a->cache8, a->norm_weight, a->sin_cache, a->cos_cache};
+    for (const void* q : rows)
+        if (!aligned(q, 16)) return LLMI_ERR_ALIGNMENT;
+    const int64_t strides[] = {a->query_stride, a->query_src_stride, a->key_new_stride, a->value_new_stride};
+    const int64_t least[] = {(int64_t)a->head_num * 128, (int64_t)a->head_num * 128, a->kv_dim, a->kv_dim};
+    for (int i = 0; i < 4; ++i) {
+        if (strides[i] == 0) continue;
+        if (strides[i] % 8 != 0) return LLMI_ERR_ALIGNMENT;
+        if (strides[i] < least[i] && a->row_num > 1) return LLMI_ERR_INVALID_ARG;
+    }
+    if (!aligned(a->pos_device, 4)) return LLMI_ERR_ALIGNMENT;
+    return launch_qk_norm_rope_append_kv8(*a);
+}
+
+int llmi_hip_mha_kv8_plan(const llmi_mha_kv8_args* args, llmi_mha_plan* plan) {
+    if (!plan) return LLMI_ERR_NULL_POINTER;
+    int splits;
+    if (int rc = make_splits(args, 0, &splits)) return rc;
+    const int64_t tiles = ((int64_t)args->pos + 32) / 32, turn = (int64_t)splits * kKv8Waves;
+    *plan = llmi_mha_plan{};
+    plan->path = splits > 1 ? LLMI_PATH_SPLIT_FUSED : LLMI_PATH_SINGLE_PASS;
+    plan->num_splits = splits;
+    plan->rows_per_split = (int32_t)std::min<int64_t>((tiles + turn - 1) / turn * kKv8Waves * 32, INT32_MAX);
+    plan->waves_per_group = kKv8Waves;
+    plan->group_pad = 16;
+    plan->workspace_needed = splits > 1 ? split_bytes(args) * (size_t)splits + 16 : 0;
+    return LLMI_OK;
+}
+
+int llmi_hip_mha_decode_kv8(const llmi_mha_kv8_args* args) {
+    int splits;
+    if (int rc = make_splits(args, 0, &splits)) return rc;
+    return launch_mha_kv8(*args, nullptr, splits);
+}
+
+int llmi_hip_mha_decode_append_kv8(const llmi_mha_kv8_append_args* a) {
+    if (!a) return LLMI_ERR_NULL_POINTER;
+    int splits;
+    if (int rc = make_splits(&a->mha, 1, &splits)) return rc;
+    if (!a->key_new || !a->value_new || !a->norm_weight || !a->sin_cache || !a->cos_cache) return LLMI_ERR_NULL_POINTER;
+    if (!aligned(a->key_new, 16) || !aligned(a->value_new, 16) || !aligned(a->norm_weight, 16) || !aligned(a->sin_cache, 16) || !aligned(a->cos_cache, 16))
+        return LLMI_ERR_ALIGNMENT;
+    if (!(a->eps >= 0.0f)) return LLMI_ERR_INVALID_ARG;
+    return launch_mha_kv8(a->mha, a, splits);
+}
+
+}  // extern "C"

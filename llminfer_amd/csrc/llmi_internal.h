@@ -142,6 +142,15 @@ int launch_qk_norm_rope_append_tree(const llmi_qk_norm_rope_tree_args& args);
 size_t verify_tree_workspace_bytes(int32_t node_num, int32_t vocab);
 int launch_verify_tree(const llmi_verify_tree_args& args);
 int launch_kv_commit_tree(const llmi_kv_commit_tree_args& args);
+// The 8-bit cache (kv8.h, kv8_api.cpp).
+constexpr int kKv8Record = LLMI_KV8_RECORD_BYTES;
+constexpr int kKv8Waves = 4;  // wavefronts of an attention workgroup
+inline int64_t kv8_records(int32_t max_seq_len) { return ((int64_t)max_seq_len + LLMI_KV8_RECORD_POSITIONS - 1) / LLMI_KV8_RECORD_POSITIONS; }
+int launch_mha_kv8(const llmi_mha_kv8_args& args, const llmi_mha_kv8_append_args* append, int splits);
+hipError_t poll_timeouts_kv8(unsigned int* n);
+int launch_qk_norm_rope_append_kv8(const llmi_qk_norm_rope_kv8_args& args);
+int launch_kv8_store(const llmi_kv8_copy_args& args);
+int launch_kv8_load(const llmi_kv8_copy_args& args);
 int launch_kv_restride(const void* src, void* dst, int32_t layer_num, int32_t max_seq_len,
                        int32_t kv_dim, int32_t head_dim, int32_t num_pos, hipStream_t stream);
 

@@ -110,7 +110,7 @@ int static_scratch(void** ptr, size_t* bytes) {
 int read_poll_timeouts(unsigned long long* count) {
     // (every translation unit that instantiates the kernels counts on its own device word)
     hipError_t (*const parts[])(unsigned int*) = {poll_timeouts_group1, poll_timeouts_group2, poll_timeouts_group4,
-                                                  poll_timeouts_group8, poll_timeouts_group16, poll_timeouts_stack, poll_timeouts_heads};
+                                                  poll_timeouts_group8, poll_timeouts_group16, poll_timeouts_stack, poll_timeouts_heads, poll_timeouts_kv8};
     unsigned long long total = 0;
     for (auto part : parts) {
         unsigned int n = 0;
