@@ -109,19 +109,20 @@ struct NewRow {
     uint32_t neighbour[2];    // the dwords of the pair's other lane: what four_pairs_squared adds up
     u32x2 sn, cs;
 };
-__device__ __forceinline__ NewRow load_row32(const uint16_t* row, const uint16_t* w, const float* sin_row, const float* cos_row, int p) {
-    NewRow y;
-    const uint32_t* r = reinterpret_cast<const uint32_t*>(row);
-    const uint32_t* n = reinterpret_cast<const uint32_t*>(w);
+// (addresses as numbers, so that they can be chosen by selects: global loads all the same, a flat one would wait for LDS too)
+__device__ __forceinline__ void load_row32(NewRow& y, uint64_t row, uint64_t w, int p) {
+    typedef const __attribute__((address_space(1))) uint32_t* Words;
+    const Words r = reinterpret_cast<Words>(row), n = reinterpret_cast<Words>(w);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         y.x[h] = r[p + 32 * h];
         y.neighbour[h] = r[(p ^ 1) + 32 * h];
         y.w[h] = n[p + 32 * h];
     }
+}
+__device__ __forceinline__ void load_tables32(NewRow& y, const float* sin_row, const float* cos_row, int p) {
     y.sn = reinterpret_cast<const u32x2*>(sin_row)[p];
     y.cs = reinterpret_cast<const u32x2*>(cos_row)[p];
-    return y;
 }
 // RMS norm and rotation of such a row, rounded to bf16: the bits of norm_rope_row32.
 __device__ __forceinline__ void norm_rope_regs32(const NewRow& y, int p, float eps, uint32_t& lo, uint32_t& hi) {

@@ -41,22 +41,32 @@ int validate(const llmi_mha_kv8_args* a) {
 
 size_t split_bytes(const llmi_mha_kv8_args* a) { return (size_t)a->head_num * (128 * sizeof(float) + 2 * sizeof(unsigned long long)); }
 
-// The workgroups a KV head's records are dealt to: a record for each wavefront, up to two workgroups per compute unit.
-int make_splits(const llmi_mha_kv8_args* a, int new_rows, int* splits) {
+// A KV head's query heads are joined by different workgroups where those, which wait for each other, fit the chip with room to spare.
+constexpr int kMostJoining = 128;
+
+// The workgroups a KV head's records are dealt to: one up to ten records (kKv8Single), then a record each up to one workgroup per compute unit. us by
+// splits, 32 Q / 8 KV heads, E4M3: 4.54 : 4.83 : 4.71 with 1 : 5 : 10 at 301 positions, 5.24 : 4.95 : 4.73 with 1 : 5 : 13 at 401, 5.52 : 4.85 : 4.71 with
+// 1 : 8 : 16 at 512, 4.90 : 4.75 with 16 : 32 at 1024, 5.68 : 6.55 with 32 : 64 at 4096, 7.31 : 7.96 at 8192, 14.2 : 15.9 at 32768, 42.7 : 45.6 at 131001.
+// Eight wavefronts a workgroup where four would have more than a record each alone, more than five in a split (each wavefront has one record on
+// its way; more in flight on a compute unit are slower: two a wavefront 43.9 : 42.4 us at 131001, 15.3 : 14.2 at 32768, three 18.6). us with 4 : 8: 3.08 : 3.16 at
+// 128 positions, 4.61 : 4.19 at 256, 5.48 : 4.54 at 301 (one split); 5.73 : 5.81 at 4096, 7.02 : 6.64 at 6008, 15.7 : 14.3 at 32768, 46.2 : 42.4 at 131001, whole
+// numbers, 64 Q heads 6.16 : 6.33 at 4096, 7.59 : 7.25 at 6008, 51.8 : 44.0 at 131001.
+int make_form(const llmi_mha_kv8_args* a, int new_rows, Kv8Form* form) {
     if (int rc = validate(a)) return rc;
     const int64_t keys = (int64_t)a->pos + 1 - new_rows, tiles = (keys + 31) / 32;
-    const int64_t most = std::max<int64_t>(1, (tiles + kKv8Waves - 1) / kKv8Waves);
     // (partial outputs are addressed with 31 bits)
     const size_t room = a->workspace ? std::min(a->workspace_bytes > 16 ? a->workspace_bytes - 16 : 0, (size_t)INT32_MAX) / split_bytes(a) : 0;
     int64_t want = a->num_splits;
     if (want == 0) {
-        want = std::min<int64_t>(std::max(512 / (a->kv_dim / 128), 1), kMaxSplits);
-        want = std::min<int64_t>({want, most, (int64_t)room});
+        want = std::min<int64_t>({std::max(256 / (a->kv_dim / 128), 1), kMaxSplits, (int64_t)room});
+        want = kv8_active_splits(tiles, (int)want);
     } else {
-        want = std::min(want, most);
+        want = std::min(want, tiles);
         if (want > 1 && (size_t)want > room) return LLMI_ERR_WORKSPACE;
     }
-    *splits = (int)std::max<int64_t>(want, 1);
+    form->splits = (int)std::max<int64_t>(want, 1);
+    form->waves = tiles > (form->splits == 1 ? 4 : 5 * (int64_t)form->splits) ? 8 : 4;
+    form->spread_min = a->head_num <= kMostJoining ? 2 : INT32_MAX;
     return LLMI_OK;
 }
 
@@ -117,34 +127,35 @@ int llmi_hip_qk_norm_rope_append_kv8(const llmi_qk_norm_rope_kv8_args* a) {
 
 int llmi_hip_mha_kv8_plan(const llmi_mha_kv8_args* args, llmi_mha_plan* plan) {
     if (!plan) return LLMI_ERR_NULL_POINTER;
-    int splits;
-    if (int rc = make_splits(args, 0, &splits)) return rc;
-    const int64_t tiles = ((int64_t)args->pos + 32) / 32, turn = (int64_t)splits * kKv8Waves;
+    Kv8Form form;
+    if (int rc = make_form(args, 0, &form)) return rc;
+    const int splits = form.splits;
+    const int64_t tiles = ((int64_t)args->pos + 32) / 32, per = (tiles + splits - 1) / splits;
     *plan = llmi_mha_plan{};
     plan->path = splits > 1 ? LLMI_PATH_SPLIT_FUSED : LLMI_PATH_SINGLE_PASS;
     plan->num_splits = splits;
-    plan->rows_per_split = (int32_t)std::min<int64_t>((tiles + turn - 1) / turn * kKv8Waves * 32, INT32_MAX);
-    plan->waves_per_group = kKv8Waves;
+    plan->rows_per_split = (int32_t)std::min<int64_t>(per * 32, INT32_MAX);
+    plan->waves_per_group = form.waves;
     plan->group_pad = 16;
     plan->workspace_needed = splits > 1 ? split_bytes(args) * (size_t)splits + 16 : 0;
     return LLMI_OK;
 }
 
 int llmi_hip_mha_decode_kv8(const llmi_mha_kv8_args* args) {
-    int splits;
-    if (int rc = make_splits(args, 0, &splits)) return rc;
-    return launch_mha_kv8(*args, nullptr, splits);
+    Kv8Form form;
+    if (int rc = make_form(args, 0, &form)) return rc;
+    return launch_mha_kv8(*args, nullptr, form);
 }
 
 int llmi_hip_mha_decode_append_kv8(const llmi_mha_kv8_append_args* a) {
     if (!a) return LLMI_ERR_NULL_POINTER;
-    int splits;
-    if (int rc = make_splits(&a->mha, 1, &splits)) return rc;
+    Kv8Form form;
+    if (int rc = make_form(&a->mha, 1, &form)) return rc;
     if (!a->key_new || !a->value_new || !a->norm_weight || !a->sin_cache || !a->cos_cache) return LLMI_ERR_NULL_POINTER;
     if (!aligned(a->key_new, 16) || !aligned(a->value_new, 16) || !aligned(a->norm_weight, 16) || !aligned(a->sin_cache, 16) || !aligned(a->cos_cache, 16))
         return LLMI_ERR_ALIGNMENT;
     if (!(a->eps >= 0.0f)) return LLMI_ERR_INVALID_ARG;
-    return launch_mha_kv8(a->mha, a, splits);
+    return launch_mha_kv8(a->mha, a, form);
 }
 
 }  // extern "C"

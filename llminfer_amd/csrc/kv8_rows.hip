@@ -41,7 +41,9 @@ __global__ __launch_bounds__(kRowThreads) void kv8_append_kernel(RowsArgs a) {
         const uint16_t* src = is_query ? a.query_src + row * a.query_src_stride + b * kHeadDim
                               : is_v   ? a.value_new + row * a.value_new_stride + kh * kHeadDim
                                        : a.key_new + row * a.key_new_stride + kh * kHeadDim;
-        const NewRow y = load_row32(src, a.weight + (is_query ? 0 : kHeadDim), a.sin_cache + (int64_t)pos * 64, a.cos_cache + (int64_t)pos * 64, p);
+        NewRow y;
+        load_row32(y, reinterpret_cast<uint64_t>(src), reinterpret_cast<uint64_t>(a.weight + (is_query ? 0 : kHeadDim)), p);
+        load_tables32(y, a.sin_cache + (int64_t)pos * 64, a.cos_cache + (int64_t)pos * 64, p);
         uint32_t lo, hi;
         norm_rope_regs32(y, p, a.eps, lo, hi);
         if (is_query) {

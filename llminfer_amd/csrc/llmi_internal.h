@@ -144,9 +144,18 @@ int launch_verify_tree(const llmi_verify_tree_args& args);
 int launch_kv_commit_tree(const llmi_kv_commit_tree_args& args);
 // The 8-bit cache (kv8.h, kv8_api.cpp).
 constexpr int kKv8Record = LLMI_KV8_RECORD_BYTES;
-constexpr int kKv8Waves = 4;  // wavefronts of an attention workgroup
 inline int64_t kv8_records(int32_t max_seq_len) { return ((int64_t)max_seq_len + LLMI_KV8_RECORD_POSITIONS - 1) / LLMI_KV8_RECORD_POSITIONS; }
-int launch_mha_kv8(const llmi_mha_kv8_args& args, const llmi_mha_kv8_append_args* append, int splits);
+// The splits that a KV head's records are dealt to where there may be `splits`: one for short contexts, else a record each at least.
+constexpr int kKv8Single = 10;
+LLMI_HOST_DEVICE constexpr int kv8_active_splits(int64_t tiles, int splits) {
+    return tiles <= kKv8Single || splits < 2 ? 1 : tiles < splits ? (int)tiles : splits;
+}
+// How the attention takes a call (rules and measurements: kv8_api.cpp): splits of a KV head, wavefronts of a workgroup (4 or 8), fewest splits at
+// which a KV head's query heads are joined by different workgroups.
+struct Kv8Form {
+    int splits, waves, spread_min;
+};
+int launch_mha_kv8(const llmi_mha_kv8_args& args, const llmi_mha_kv8_append_args* append, const Kv8Form& form);
 hipError_t poll_timeouts_kv8(unsigned int* n);
 int launch_qk_norm_rope_append_kv8(const llmi_qk_norm_rope_kv8_args& args);
 int launch_kv8_store(const llmi_kv8_copy_args& args);

@@ -41,6 +41,8 @@ struct Kv8Args {
     int64_t records;              // per KV head
     uint32_t tag;
     int32_t pos, group, n_q, splits, max_polls;
+    int32_t run, longer;          // records per split, and how many splits take one more (position known on the host)
+    int32_t spread_min;           // fewest splits at which a KV head's query heads are joined by different workgroups
     float scale_log2e;            // log2(e) / sqrt(128)
     // the new token's
     const uint16_t* k_new;
@@ -52,31 +54,34 @@ struct Kv8Args {
 };
 
 struct Record {
-    u32x4 k[4], v[4], ks, vs;
+    u32x4 k[4], v[4], ks, vs;  // codes, the lane's eight scales
 };
 
 // Streaming loads: nobody reads a record twice.
 constexpr int kStream = 2;
-__device__ __forceinline__ Record load_record(const char* at, uint32_t bytes, uint32_t lane) {
-    // (a record that there is not: zeros, and nothing read)
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(at), 0, bytes, 0x00020000);
+// (a record that there is not: zeros, and nothing read)
+__device__ __forceinline__ Record load_record(const char* at, bool there, uint32_t lane) {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(at), 0, there ? kKv8Record : 0, 0x00020000);
+    auto load = [&](uint32_t lane_at, int offset) __attribute__((always_inline)) {
+        return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, lane_at, offset, kStream));
+    };
     Record y;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y.k[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, lane * 16u, i * 1024, kStream));
-    y.ks = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (lane >> 4) * 16u, kScaleBytes, kStream));
-    y.vs = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (lane >> 4) * 16u, kScaleBytes + 64, kStream));
+    for (int i = 0; i < 4; ++i) y.k[i] = load(lane * 16u, i * 1024);
+    y.ks = load((lane >> 4) * 16u, kScaleBytes);
+    y.vs = load((lane >> 4) * 16u, kScaleBytes + 64);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y.v[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, lane * 16u, kVBytes + i * 1024, kStream));
+    for (int i = 0; i < 4; ++i) y.v[i] = load(lane * 16u, kVBytes + i * 1024);
     return y;
 }
 
 template <int FORMAT, int NW, bool APPEND>
 __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
-    constexpr int kAhead = 2;  // records in flight
     __shared__ __attribute__((aligned(16))) float parts[NW][kHeads][kHeadDim];
     __shared__ float part_m[kHeads][NW], part_l[kHeads][NW];
-    __shared__ float weights[NW][kMaxSplits];
+    __shared__ __attribute__((aligned(16))) float weights[NW][2][32];
     __shared__ float fin[kHeads][2];
+    __shared__ bool arrived[NW];
     __shared__ __attribute__((aligned(16))) uint16_t rows[APPEND ? kHeads : 1][kHeadDim];
     __shared__ __attribute__((aligned(16))) uint8_t new_codes[APPEND ? 2 : 1][kHeadDim];
     __shared__ float new_scale[2];
@@ -85,59 +90,98 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
     const int n = lane & 15, g = lane >> 4;
     const int kvh = blockIdx.x, split = blockIdx.y;
 
-    const int pos = __builtin_amdgcn_readfirstlane(a.pos_dev ? max(0, min(*a.pos_dev, a.pos)) : a.pos);
+    // The new token's rows, half a wavefront each: the query heads, and (the last split files them) K and V behind them. What does not depend on the
+    // position is asked for in front of it, everything else in front of the records.
+    const int p32 = lane & 31;
+    const int half = (int)(threadIdx.x >> 5);
+    const int work_rows = a.group + 2;
+    NewRow row;
+    auto ask_row = [&](int at) __attribute__((always_inline)) {
+        const bool is_new = at >= a.group;
+        const uint64_t new_row = reinterpret_cast<uint64_t>(at > a.group ? a.v_new : a.k_new) + (uint64_t)(uint32_t)(kvh * 256);
+        const uint64_t q_row = reinterpret_cast<uint64_t>(a.q) + (uint64_t)(uint32_t)((kvh * a.group + at) * 256);
+        load_row32(row, is_new ? new_row : q_row, reinterpret_cast<uint64_t>(a.norm_w) + (is_new ? 256u : 0u), p32);
+    };
+    // (half wavefronts without a row take the last one again: a branch around the loads would make their wait one for all of the records' too)
+    if constexpr (APPEND) ask_row(min(half, work_rows - 1));
+    int pos = a.pos, active = a.splits, run = a.run, longer = a.longer;
+    if (a.pos_dev) {
+        // (constant address space: a scalar load; nothing in the launch writes the position)
+        const auto word = reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(a.pos_dev));
+        pos = max(0, min(*word, a.pos));
+        const int tiles = (int)(((int64_t)pos + (APPEND ? 0 : 1) + 31) >> 5);
+        active = kv8_active_splits(tiles, a.splits);
+        if (split >= active) return;
+        // (a quotient in two steps of 24 bits, then one up or down: two orders shorter than the compiler's division, and on the way to the first load)
+        const float inverse = 1.0f / (float)active;
+        run = (int)((float)tiles * inverse);
+        run += (int)((float)(tiles - run * active) * inverse);
+        longer = tiles - run * active;
+        if (longer < 0) {
+            --run;
+            longer += active;
+        } else if (longer >= active) {
+            ++run;
+            longer -= active;
+        }
+    }
     const int64_t keys = (int64_t)pos + (APPEND ? 0 : 1);  // positions that come from the cache
-    const int tiles = (int)((keys + 31) >> 5);
-    const int active = max(1, min(a.splits, (tiles + NW - 1) / NW));
-    if (split >= active) return;
     const bool last = split == active - 1;
+    // A split's records are a run of consecutive ones (runs differ by one at most), its wavefronts take them in turn.
+    const int mine = run + (split < longer ? 1 : 0);
+    const int first_tile = split * run + min(split, longer);
+    const int last_tile = (int)((keys + 31) >> 5) - 1;
     const char* head = a.cache + (int64_t)kvh * a.records * kKv8Record;
-    const int step = active * NW, t0 = split * NW + wave;
-    const int count = t0 < tiles ? (tiles - t0 + step - 1) / step : 0;
+    const char* from = head + (int64_t)(first_tile + wave) * kKv8Record;
+    const int count = wave < mine ? (mine - wave + NW - 1) / NW : 0;
     auto fetch = [&](int i) __attribute__((always_inline)) {
-        const int64_t t = t0 + (int64_t)i * step;
-        return load_record(head + (i < count ? t : 0) * kKv8Record, i < count ? (uint32_t)kKv8Record : 0u, (uint32_t)lane);
+        return load_record(from + (i < count ? (int64_t)i * (NW * kKv8Record) : 0), i < count, (uint32_t)lane);
     };
 
-    // The new token's rows, half a wavefront each: the query heads, in the last split K and V behind them.
-    const int half = threadIdx.x >> 5, p32 = lane & 31;
-    const int work_rows = a.group + (last ? 2 : 0);
+    // The query heads: step s of the first product has channels 64 (s/2) + 16 g + 8 (s%2) .. + 7 in lane group g. (Columns behind the group repeat its
+    // last head: nobody reads their outputs.)
+    u32x4 q[4];
+    const int hq = min(n, a.group - 1);
+    if constexpr (!APPEND) {
+        const uint16_t* src = a.q + (int64_t)(kvh * a.group + hq) * kHeadDim;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) q[s] = *reinterpret_cast<const u32x4*>(src + 64 * (s >> 1) + 16 * g + 8 * (s & 1));
+    }
+    auto ask_tables = [&]() __attribute__((always_inline)) { load_tables32(row, a.sin_cache + (int64_t)pos * 64, a.cos_cache + (int64_t)pos * 64, p32); };
+    if constexpr (APPEND) ask_tables();
+    asm volatile("" ::: "memory");
+    Record r = fetch(0);
     if constexpr (APPEND) {
-        for (int row = half; row < work_rows; row += 2 * NW) {
-            const bool is_new = row >= a.group, is_v = row > a.group;
-            const uint16_t* src = is_v ? a.v_new + kvh * kHeadDim : is_new ? a.k_new + kvh * kHeadDim : a.q + (int64_t)(kvh * a.group + row) * kHeadDim;
-            const NewRow y = load_row32(src, a.norm_w + (is_new ? kHeadDim : 0), a.sin_cache + (int64_t)pos * 64, a.cos_cache + (int64_t)pos * 64, p32);
+        auto finish_row = [&](int at) __attribute__((always_inline)) {
+            const bool is_new = at >= a.group, is_v = at > a.group;
             uint32_t lo, hi;
-            norm_rope_regs32(y, p32, a.eps, lo, hi);
+            norm_rope_regs32(row, p32, a.eps, lo, hi);
             if (is_v) {
-                lo = y.x[0];
-                hi = y.x[1];
+                lo = row.x[0];
+                hi = row.x[1];
             }
-            if (is_new) {
+            if (!is_new) {
+                reinterpret_cast<uint32_t*>(rows[at])[p32] = lo;
+                reinterpret_cast<uint32_t*>(rows[at])[p32 + 32] = hi;
+            } else if (last) {
                 float s;
                 const uint32_t codes = quantise_row32<FORMAT>(lo, hi, s);
                 file_row32(const_cast<char*>(head) + (int64_t)(pos >> 5) * kKv8Record, pos & 31, is_v, p32, codes, s);
                 reinterpret_cast<uint16_t*>(new_codes[is_v])[p32] = (uint16_t)codes;
                 reinterpret_cast<uint16_t*>(new_codes[is_v])[p32 + 32] = (uint16_t)(codes >> 16);
                 if (p32 == 0) new_scale[is_v] = s;
-            } else {
-                reinterpret_cast<uint32_t*>(rows[row])[p32] = lo;
-                reinterpret_cast<uint32_t*>(rows[row])[p32 + 32] = hi;
             }
+        };
+        if (half < work_rows) finish_row(half);
+        // (apart from the first one: a loop's wait would be for its newest loads, the record's too)
+        for (int at = half + 2 * NW; at < work_rows; at += 2 * NW) {
+            ask_row(at);
+            ask_tables();
+            finish_row(at);
         }
-    }
-    Record ring[kAhead];
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (the records stay on their way)
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) ring[i] = fetch(i);
-    if constexpr (APPEND) __syncthreads();
-
-    // The query heads: step s of the first product has channels 64 (s/2) + 16 g + 8 (s%2) .. + 7 in lane group g.
-    u32x4 q[4];
-    {
-        const int hq = min(n, a.group - 1);
-        const uint16_t* src = APPEND ? rows[hq] : a.q + (int64_t)(kvh * a.group + hq) * kHeadDim;
-#pragma unroll
-        for (int s = 0; s < 4; ++s) q[s] = *reinterpret_cast<const u32x4*>(src + 64 * (s >> 1) + 16 * g + 8 * (s & 1));
+        for (int s = 0; s < 4; ++s) q[s] = *reinterpret_cast<const u32x4*>(rows[hq] + 64 * (s >> 1) + 16 * g + 8 * (s & 1));
     }
     float m_run = -FLT_MAX, l_run = 0.0f;  // (a finite maximum: scores of -inf get weight 0, not NaN)
     f32x4 o[8];
@@ -145,8 +189,8 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
     for (int b = 0; b < 8; ++b) o[b] = f32x4{};
 
     if constexpr (APPEND) {
-        // The new token, as its codes stand for it, with weight 1.
-        if (last && wave == 0) {
+        // The new token, as its codes stand for it, with weight 1: the wavefront that has the fewest records starts from it.
+        if (last && wave == NW - 1) {
             const float ks = new_scale[0], vs = new_scale[1];
             f32x4 c{};
             // (all sixteen positions of the product are the new one)
@@ -169,8 +213,8 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
         }
     }
 
-    auto fold = [&](Record& r, int64_t t) __attribute__((always_inline)) {
-        float c[8];
+    auto fold = [&](int t) __attribute__((always_inline)) {
+        float c[8], vs[8];  // of position 16 (e / 4) + 4 g + e % 4: scores in the exp2 domain, V's scales
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             f32x4 x{};
@@ -182,14 +226,13 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) c[4 * u + e] = x[e];
         }
-        float vs[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const uint32_t kw = r.ks[e >> 1], vw = r.vs[e >> 1];
             c[e] *= ((e & 1) ? bf16_hi(kw) : bf16_lo(kw)) * a.scale_log2e;
             vs[e] = (e & 1) ? bf16_hi(vw) : bf16_lo(vw);
         }
-        if (t == tiles - 1 && (keys & 31)) {
+        if (t == last_tile && (keys & 31)) {
             // The last record, not full: what lies behind the last position has no weight whatever it is.
             const int left = (int)(keys & 31) - 4 * g;
 #pragma unroll
@@ -235,18 +278,14 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
         }
 #pragma unroll
         for (int b = 0; b < 8; ++b) {
-            const bf16x8 v = kv8_operand<FORMAT>(r.v[b >> 1][2 * (b & 1)], r.v[b >> 1][2 * (b & 1) + 1]);
-            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, ph), o[b], 0, 0, 0);
-            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, pl), o[b], 0, 0, 0);
+            const bf16x8 x = kv8_operand<FORMAT>(r.v[b >> 1][2 * (b & 1)], r.v[b >> 1][2 * (b & 1) + 1]);
+            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(bf16x8, ph), o[b], 0, 0, 0);
+            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(bf16x8, pl), o[b], 0, 0, 0);
         }
     };
-    for (int i = 0; i < count; i += kAhead) {
-#pragma unroll
-        for (int d = 0; d < kAhead; ++d) {
-            if (i + d >= count) break;
-            fold(ring[d], t0 + (int64_t)(i + d) * step);
-            ring[d] = fetch(i + d + kAhead);
-        }
+    for (int i = 0; i < count; ++i) {
+        fold(first_tile + wave + i * NW);
+        r = fetch(i + 1);
     }
 
     // The workgroup's wavefronts.
@@ -270,7 +309,16 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
             for (int e = 0; e < 4; ++e) a.out_f32[(int64_t)hq * kHeadDim + 4 * c4 + e] = x[e];
         }
     };
-    for (int u = threadIdx.x; u < a.group * 32; u += NW * 64) {
+    // Who joins a head's splits: the workgroup of the last one all of them, or, where there are enough, the last splits' workgroups a head each, so
+    // that the parts are read back by several compute units.
+    const bool spread = active >= a.spread_min && active >= a.group;
+    const int my_head = spread && active - 1 - split < a.group ? active - 1 - split : -1;
+    constexpr int kUnits = kHeads * 32 / (NW * 64);
+    float unit_m[kUnits], unit_l[kUnits];
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+        const int u = (int)threadIdx.x + i * NW * 64;
+        if (u >= a.group * 32) break;
         const int h = u >> 5, c4 = u & 31, hq = kvh * a.group + h;
         float m = part_m[h][0];
 #pragma unroll
@@ -285,119 +333,167 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] += f * y[e];
         }
+        unit_m[i] = m;
+        unit_l[i] = sum;
         if (active == 1) {
             const float r = 1.0f / sum;
             write_out(hq, c4, f32x4{x[0] * r, x[1] * r, x[2] * r, x[3] * r});
-            continue;
-        }
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), part_rsrc, (uint32_t)(((hq * S + split) * kHeadDim + 4 * c4) * 4), 0, kCacheDevice);
-        if (last) {
-            if (c4 == 0) {
-                fin[h][0] = m;
-                fin[h][1] = sum;
-            }
-            continue;
-        }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (a head's 32 columns are half a wavefront's)
-        if (c4 == 0) {
-            unsigned long long* to = a.arrivals + ((int64_t)hq * S + split) * 2;
-            const unsigned long long tag = a.tag;
-            __hip_atomic_store(to, tag | (unsigned long long)__builtin_bit_cast(uint32_t, m) << 32, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __hip_atomic_store(to + 1, tag | (unsigned long long)__builtin_bit_cast(uint32_t, sum) << 32, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        } else {
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), part_rsrc, (uint32_t)(((hq * S + split) * kHeadDim + 4 * c4) * 4), 0, kCacheDevice);
         }
     }
-    if (active == 1 || !last) return;
-
-    // The last split's workgroup: a wavefront a head.
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (active == 1) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (a head's 32 columns are half a wavefront's: no barrier)
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+        const int u = (int)threadIdx.x + i * NW * 64;
+        if (u >= a.group * 32) break;
+        const int h = u >> 5;
+        if ((u & 31) != 0) continue;
+        if (spread ? h == my_head : last) {
+            fin[h][0] = unit_m[i];
+            fin[h][1] = unit_l[i];
+        } else {
+            unsigned long long* to = a.arrivals + ((int64_t)(kvh * a.group + h) * S + split) * 2;
+            const unsigned long long tag = a.tag;
+            __hip_atomic_store(to, tag | (unsigned long long)__builtin_bit_cast(uint32_t, unit_m[i]) << 32, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(to + 1, tag | (unsigned long long)__builtin_bit_cast(uint32_t, unit_l[i]) << 32, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    }
+    if (spread ? my_head < 0 : !last) return;
     __syncthreads();
-    for (int h = wave; h < a.group; h += NW) {
+
+    // A wavefront's part of a head's join: splits s0 .. s0 + n - 1 (64 at most), a lane each for the records, a lane for four columns of every
+    // second split for the parts.
+    struct Part {
+        float m, sum;
+        f32x4 x;
+        bool in;
+    };
+    const int c4 = lane & 31, part = lane >> 5;
+    auto gather = [&](int h, int s0, int n) __attribute__((always_inline)) {
+        constexpr int kBatch = 16;
         const int hq = kvh * a.group + h;
-        constexpr int kSlots = kMaxSplits / 64;
-        float ms[kSlots], ls[kSlots];
-        unsigned long long* from = a.arrivals + (int64_t)hq * S * 2;
-        bool in = false;
-        for (int spin = 0; spin < a.max_polls && !in; ++spin) {
+        unsigned long long* rec = a.arrivals + ((int64_t)hq * S + s0 + lane) * 2;
+        Part y;
+        float m = -FLT_MAX, l = 0.0f;
+        const bool mine_is = lane < n && s0 + lane == split, polls = lane < n && !mine_is;
+        if (mine_is) {
+            m = fin[h][0];
+            l = fin[h][1];
+        }
+        y.in = false;
+        for (int spin = 0; spin < a.max_polls && !y.in; ++spin) {
             bool ok = true;
-#pragma unroll
-            for (int j = 0; j < kSlots; ++j) {
-                const int s = lane + 64 * j;
-                ms[j] = -FLT_MAX;
-                ls[j] = 0.0f;
-                if (s >= active) continue;
-                if (s == split) {
-                    ms[j] = fin[h][0];
-                    ls[j] = fin[h][1];
-                    continue;
-                }
-                const unsigned long long r0 = __hip_atomic_load(from + 2 * s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                const unsigned long long r1 = __hip_atomic_load(from + 2 * s + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                ok = ok && (uint32_t)r0 == a.tag && (uint32_t)r1 == a.tag;
-                ms[j] = __builtin_bit_cast(float, (uint32_t)(r0 >> 32));
-                ls[j] = __builtin_bit_cast(float, (uint32_t)(r1 >> 32));
+            if (polls) {
+                const unsigned long long r0 = __hip_atomic_load(rec, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                const unsigned long long r1 = __hip_atomic_load(rec + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                ok = (uint32_t)r0 == a.tag && (uint32_t)r1 == a.tag;
+                m = __builtin_bit_cast(float, (uint32_t)(r0 >> 32));
+                l = __builtin_bit_cast(float, (uint32_t)(r1 >> 32));
             }
-            in = __all(ok);
+            y.in = __all(ok);
         }
-        if (!in && lane == 0) atomicAdd(&g_poll_timeouts, 1u);
-        float m = -FLT_MAX;
-        if (in) {
+        // (rows behind the last split: zeros, and nothing read)
+        const __amdgpu_buffer_rsrc_t rows_rsrc =
+            __builtin_amdgcn_make_buffer_rsrc(a.ws + (int64_t)(hq * S + s0) * kHeadDim, 0, max(n, 0) * (kHeadDim * 4), 0x00020000);
+        const uint32_t at = (uint32_t)(part * (kHeadDim * 4) + c4 * 16);
+        f32x4 v[kBatch];
 #pragma unroll
-            for (int j = 0; j < kSlots; ++j) m = fmaxf(m, ms[j]);
+        for (int j = 0; j < kBatch; ++j) v[j] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rows_rsrc, at, j * 1024, kCacheDevice));
+        if (polls && y.in) {
+            // (a replay of a captured launch carries the same tag)
+            __hip_atomic_store(rec, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(rec + 1, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-        m = wave_max(m);
-        float sum = 0.0f;
-        if (in) {
-#pragma unroll
-            for (int j = 0; j < kSlots; ++j) {
-                const int s = lane + 64 * j;
-                if (s >= active) continue;
-                const float f = fast_exp2(ms[j] - m);
-                weights[wave][s] = f;
-                sum += f * ls[j];
-                if (s == split) continue;
-                // (a replay of a captured launch carries the same tag)
-                __hip_atomic_store(from + 2 * s, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                __hip_atomic_store(from + 2 * s + 1, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
-        }
-        sum = wave_sum(sum);
+        y.m = wave_max(m);
+        const float f = lane < n ? fast_exp2(m - y.m) : 0.0f;
+        weights[wave][lane & 1][lane >> 1] = f;  // (a half wavefront's side by side)
+        y.sum = wave_sum(f * l);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_wave_barrier();
-        const int c4 = lane & 31, part = lane >> 5;
-        f32x4 x{};
-        constexpr int kBatch = 8;
-        for (int s0 = part; s0 < active; s0 += 2 * kBatch) {
-            f32x4 y[kBatch];
+        f32x4 w[kBatch / 4];
+        auto weigh = [&](int j0) __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 0; j < kBatch; ++j) {
-                const int s = min(s0 + 2 * j, active - 1);
-                y[j] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(part_rsrc, (uint32_t)(((hq * S + s) * kHeadDim + 4 * c4) * 4), 0, kCacheDevice));
-            }
+            for (int j = 0; j < kBatch / 4; ++j) w[j] = *reinterpret_cast<const f32x4*>(&weights[wave][part][j0 + 4 * j]);
+        };
+        auto add = [&]() __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 0; j < kBatch; ++j) {
-                const int s = s0 + 2 * j;
-                const float f = weights[wave][min(s, active - 1)];
+            for (int j = 0; j < kBatch; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = s < active ? x[e] + f * y[j][e] : x[e];
-            }
+                for (int e = 0; e < 4; ++e) y.x[e] = __builtin_fmaf(w[j >> 2][j & 3], v[j][e], y.x[e]);
+        };
+        y.x = f32x4{};
+        weigh(0);
+        add();
+        if (n > 2 * kBatch) {
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) v[j] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rows_rsrc, at, (kBatch + j) * 1024, kCacheDevice));
+            weigh(kBatch);
+            add();
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = halves_sum(x[e]);
-        const float r = in ? 1.0f / sum : __builtin_bit_cast(float, 0x7fc00000u);
-        if (part == 0) write_out(hq, c4, f32x4{x[0] * r, x[1] * r, x[2] * r, x[3] * r});
+        for (int e = 0; e < 4; ++e) y.x[e] = halves_sum(y.x[e]);
+        return y;
+    };
+    if (active <= 64) {
+        // a wavefront a head
+        if (spread && wave != 0) return;
+        for (int h = spread ? my_head : wave; h < a.group; h += NW) {
+            const Part y = gather(h, 0, active);
+            if (!y.in && lane == 0) atomicAdd(&g_poll_timeouts, 1u);
+            const float r = y.in ? 1.0f / y.sum : __builtin_bit_cast(float, 0x7fc00000u);
+            if (part == 0) write_out(kvh * a.group + h, c4, f32x4{y.x[0] * r, y.x[1] * r, y.x[2] * r, y.x[3] * r});
+            if (spread) break;
+        }
+        return;
+    }
+    // All wavefronts a head: a share of the splits each.
+    const int share = (active + NW - 1) / NW;
+    for (int h = spread ? my_head : 0; h < a.group; ++h) {
+        const Part y = gather(h, wave * share, min(share, active - wave * share));
+        __syncthreads();  // (the parts' place is read for the last time in the turn before)
+        if (part == 0) *reinterpret_cast<f32x4*>(&parts[wave][0][4 * c4]) = y.x;
+        if (lane == 0) {
+            part_m[0][wave] = y.m;
+            part_l[0][wave] = y.sum;
+            arrived[wave] = y.in;
+        }
+        __syncthreads();
+        if (threadIdx.x < 32) {
+            float m = part_m[0][0], sum = 0.0f;
+            f32x4 x{};
+#pragma unroll
+            for (int w = 1; w < NW; ++w) m = fmaxf(m, part_m[0][w]);
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                const float f = fast_exp2(part_m[0][w] - m);
+                sum += f * part_l[0][w];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] += f * parts[w][0][4 * c4 + e];
+            }
+            bool in = true;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) in = in && arrived[w];
+            if (!in && lane == 0) atomicAdd(&g_poll_timeouts, 1u);
+            const float r = in ? 1.0f / sum : __builtin_bit_cast(float, 0x7fc00000u);
+            write_out(kvh * a.group + h, c4, f32x4{x[0] * r, x[1] * r, x[2] * r, x[3] * r});
+        }
+        if (spread) break;
     }
 }
 
 template <int FORMAT, bool APPEND>
-void launch(const Kv8Args& a, int n_kv, hipStream_t stream) {
-    hipLaunchKernelGGL((mha_kv8_kernel<FORMAT, kKv8Waves, APPEND>), dim3(n_kv, a.splits), dim3(kKv8Waves * 64), 0, stream, a);
+void launch(const Kv8Args& a, int n_kv, int waves, hipStream_t stream) {
+    if (waves == 8) hipLaunchKernelGGL((mha_kv8_kernel<FORMAT, 8, APPEND>), dim3(n_kv, a.splits), dim3(8 * 64), 0, stream, a);
+    else hipLaunchKernelGGL((mha_kv8_kernel<FORMAT, 4, APPEND>), dim3(n_kv, a.splits), dim3(4 * 64), 0, stream, a);
 }
 
 }  // namespace
 
 hipError_t poll_timeouts_kv8(unsigned int* n) { return hipMemcpyFromSymbol(n, HIP_SYMBOL(g_poll_timeouts), sizeof(*n)); }
 
-int launch_mha_kv8(const llmi_mha_kv8_args& m, const llmi_mha_kv8_append_args* append, int splits) {
+int launch_mha_kv8(const llmi_mha_kv8_args& m, const llmi_mha_kv8_append_args* append, const Kv8Form& form) {
     Kv8Args a{};
     const int n_kv = m.kv_dim / kHeadDim;
     a.q = static_cast<const uint16_t*>(m.query);
@@ -409,12 +505,16 @@ int launch_mha_kv8(const llmi_mha_kv8_args& m, const llmi_mha_kv8_append_args* a
     a.pos = m.pos;
     a.group = m.kv_mul;
     a.n_q = m.head_num;
-    a.splits = splits;
+    a.splits = form.splits;
     a.max_polls = poll_limit();
+    const int tiles = (int)(((int64_t)m.pos + (append ? 0 : 1) + 31) >> 5);
+    a.run = tiles / form.splits;
+    a.longer = tiles % form.splits;
+    a.spread_min = form.spread_min;
     a.scale_log2e = 1.4426950408889634f / sqrtf((float)kHeadDim);
-    if (splits > 1) {
+    if (form.splits > 1) {
         a.ws = static_cast<float*>(m.workspace);
-        a.arrivals = reinterpret_cast<unsigned long long*>(static_cast<char*>(m.workspace) + fused_workspace(m.head_num, kHeadDim, splits, false).partial_bytes);
+        a.arrivals = reinterpret_cast<unsigned long long*>(static_cast<char*>(m.workspace) + fused_workspace(m.head_num, kHeadDim, form.splits, false).partial_bytes);
         a.tag = record_tag(next_epoch());
     }
     if (append) {
@@ -427,8 +527,8 @@ int launch_mha_kv8(const llmi_mha_kv8_args& m, const llmi_mha_kv8_append_args* a
     }
     const hipStream_t stream = static_cast<hipStream_t>(m.stream);
     const bool e4m3 = m.format == LLMI_KV8_E4M3;
-    if (append) e4m3 ? launch<LLMI_KV8_E4M3, true>(a, n_kv, stream) : launch<LLMI_KV8_INT8, true>(a, n_kv, stream);
-    else e4m3 ? launch<LLMI_KV8_E4M3, false>(a, n_kv, stream) : launch<LLMI_KV8_INT8, false>(a, n_kv, stream);
+    if (append) e4m3 ? launch<LLMI_KV8_E4M3, true>(a, n_kv, form.waves, stream) : launch<LLMI_KV8_INT8, true>(a, n_kv, form.waves, stream);
+    else e4m3 ? launch<LLMI_KV8_E4M3, false>(a, n_kv, form.waves, stream) : launch<LLMI_KV8_INT8, false>(a, n_kv, form.waves, stream);
     return check_launch();
 }
 

@@ -156,7 +156,7 @@ def test_plan_over_random_arguments():
             assert rc == B.STATUS["WORKSPACE"] and splits > 1
             continue
         assert p.workspace_needed <= max(room, 16) and p.workspace_needed < 1 << 31 and 1 <= p.num_splits <= 256
-        assert p.num_splits <= max(1, -(-tiles // p.waves_per_group)) and (splits == 0 or p.num_splits <= splits)
+        assert p.num_splits <= tiles and (splits == 0 or p.num_splits <= splits) and p.waves_per_group in (4, 8)
         assert min(p.rows_per_split, 1 << 30) * p.num_splits >= min(pos + 1, 1 << 30)
         assert (p.path == B.PATH_SINGLE_PASS) == (p.num_splits == 1)
 
