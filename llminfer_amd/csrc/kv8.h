@@ -50,10 +50,9 @@ __device__ __forceinline__ float kv8_quotient(float x, float s, float r) {
     return __builtin_fmaf(-__builtin_fmaf(y, s, -x), r, y);
 }
 
-// Four values' codes, the first in the low byte. Of a scale of NaN: zeros.
+// Four values' codes, the first in the low byte; r = 1 / s. Of a scale of NaN: zeros.
 template <int FORMAT>
-__device__ __forceinline__ uint32_t kv8_codes(float x0, float x1, float x2, float x3, float s) {
-    const float r = 1.0f / s;
+__device__ __forceinline__ uint32_t kv8_codes(float x0, float x1, float x2, float x3, float s, float r) {
     const float y0 = kv8_quotient(x0, s, r), y1 = kv8_quotient(x1, s, r), y2 = kv8_quotient(x2, s, r), y3 = kv8_quotient(x3, s, r);
     uint32_t w;
     if constexpr (FORMAT == LLMI_KV8_E4M3) {
@@ -102,6 +101,19 @@ __device__ __forceinline__ uint32_t row32_max(uint32_t x) {
 }
 // The larger magnitude of two bf16 numbers, as bits.
 __device__ __forceinline__ uint32_t pair_magnitude(uint32_t w) { return max_u32(w & 0x7fffu, (w >> 16) & 0x7fffu); }
+
+// Four words whose bytes are a 4 x 4 matrix, transposed: byte j of word i to byte i of word j.
+__device__ __forceinline__ void transpose_bytes(const uint32_t (&a)[4], uint32_t (&b)[4]) {
+    const uint32_t p = __builtin_amdgcn_perm(a[1], a[0], 0x05010400u), q = __builtin_amdgcn_perm(a[1], a[0], 0x07030602u);  // rows 0, 1: columns 0 and 1, 2 and 3
+    const uint32_t r = __builtin_amdgcn_perm(a[3], a[2], 0x05010400u), s = __builtin_amdgcn_perm(a[3], a[2], 0x07030602u);
+    b[0] = __builtin_amdgcn_perm(r, p, 0x05040100u);
+    b[1] = __builtin_amdgcn_perm(r, p, 0x07060302u);
+    b[2] = __builtin_amdgcn_perm(s, q, 0x05040100u);
+    b[3] = __builtin_amdgcn_perm(s, q, 0x07060302u);
+}
+// x of lane I of the caller's four neighbours.
+template <int I>
+__device__ __forceinline__ float quad_lane(float x) { return dpp_partner<I * 0x55>(x); }
 
 // A row on 32 lanes: lane p has dwords p and p + 32 of it (channels 2p, 2p + 1, 64 + 2p, 64 + 2p + 1).
 struct NewRow {
@@ -158,7 +170,7 @@ __device__ __forceinline__ void norm_rope_regs32(const NewRow& y, int p, float e
 template <int FORMAT>
 __device__ __forceinline__ uint32_t quantise_row32(uint32_t lo, uint32_t hi, float& s) {
     s = kv8_scale<FORMAT>(row32_max(max_u32(pair_magnitude(lo), pair_magnitude(hi))));
-    return kv8_codes<FORMAT>(bf16_lo(lo), bf16_hi(lo), bf16_lo(hi), bf16_hi(hi), s);
+    return kv8_codes<FORMAT>(bf16_lo(lo), bf16_hi(lo), bf16_lo(hi), bf16_hi(hi), s, 1.0f / s);
 }
 // ... and filed in its record.
 __device__ __forceinline__ void file_row32(char* record, int pos, bool is_v, int p, uint32_t codes, float s) {

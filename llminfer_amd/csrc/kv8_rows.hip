@@ -68,98 +68,171 @@ struct CopyArgs {
     int64_t layer_elems, row_stride, head_stride;  // elements
     int64_t records;     // per KV head
     int32_t first, count, n_kv, layers;
+    int32_t touched;     // records of a KV head that have positions of the call
+    bool by_head;
 };
 
-// A workgroup per record of a KV head, K in the first half of the threads' turns, V in the second: sixteen lanes a row of 256 bytes.
+// A workgroup per record of a KV head. Wavefront w has sixteen positions, 16 (w % 2) and on, of K (w < 2) or V; lane L of it the channels 8 (L % 16) .. + 7
+// of four of them, 4 (L / 16) .. + 3: rows are read (written) whole, 256 bytes over sixteen lanes, a lane's four positions are the bytes of V's words (two
+// rounds of v_perm), and what a row needs once (scale, reciprocal) is worked out for one row a lane and handed round the four neighbours. The record
+// passes through LDS, where its blocks of 256 bytes are 272 apart: eight times fewer bank conflicts. Both ways past the caches, as in kv_restride.
 constexpr int kCopyThreads = 256;
-template <int FORMAT>
+template <bool STREAM>
+__device__ __forceinline__ u32x4 load_chunk(const u32x4* p) {
+    return STREAM ? __builtin_nontemporal_load(p) : *p;
+}
+constexpr int kLdsScales = 32 * 272;
+__device__ __forceinline__ int in_lds(int byte) { return byte + (byte >> 8) * 16; }  // (of codes)
+struct CopyPlace {
+    int kh, record, from, to;     // positions from .. to - 1 of the record are the call's
+    int which, p0, c0;            // the lane's first position and channel
+};
+__device__ __forceinline__ CopyPlace copy_place(const CopyArgs& a) {
+    CopyPlace x;
+    // (neighbours where the bf16 cache has its rows side by side)
+    const uint32_t b = blockIdx.x, along = a.by_head ? (uint32_t)a.touched : (uint32_t)a.n_kv, far = b / along, near = b - far * along;
+    x.kh = (int)(a.by_head ? far : near);
+    x.record = (a.first >> 5) + (int)(a.by_head ? near : far);
+    x.from = max(a.first - x.record * 32, 0);
+    x.to = (int)min((int64_t)a.first + a.count - (int64_t)x.record * 32, (int64_t)32);
+    const int wave = (int)(threadIdx.x >> 6), lane = (int)(threadIdx.x & 63);
+    x.which = wave >> 1;
+    x.p0 = 16 * (wave & 1) + 4 * (lane >> 4);
+    x.c0 = 8 * (lane & 15);
+    return x;
+}
+
+template <int FORMAT, bool STREAM>
 __global__ __launch_bounds__(kCopyThreads) void kv8_store_kernel(CopyArgs a) {
-    __shared__ __attribute__((aligned(16))) char rec[kKv8Record];
-    const int kh = blockIdx.y;
-    const int record = (a.first >> 5) + (int)blockIdx.x;
-    const int p0 = record * 32;
-    const int from = max(a.first - p0, 0), to = (int)min((int64_t)a.first + a.count - p0, (int64_t)32);  // its positions that are filed
-    const int lane16 = threadIdx.x & 15;
-    for (int layer = blockIdx.z; layer < a.layers; layer += gridDim.z) {
-        __syncthreads();
+    __shared__ __attribute__((aligned(16))) char rec[kLdsScales + 128];
+    const CopyPlace at = copy_place(a);
+    const int kh = at.kh;
+    const int l4 = (int)(threadIdx.x & 3);
+    const uint16_t* src = (at.which ? a.rows[1] : a.rows[0]) + (int64_t)at.record * 32 * a.row_stride + kh * a.head_stride + at.c0;
+    int32_t row[4];
 #pragma unroll
-        for (int turn = 0; turn < 4; ++turn) {
-            const int which = turn >> 1;
-            const int p = (turn & 1) * 16 + (int)(threadIdx.x >> 4);
-            const int pc = max(from, min(p, to - 1));  // (rows that are not filed repeat one that is)
-            const u32x4 w = *reinterpret_cast<const u32x4*>(a.rows[which] + layer * a.layer_elems + (p0 + (int64_t)pc) * a.row_stride + kh * a.head_stride + lane16 * 8);
-            uint32_t top = 0;
+    for (int i = 0; i < 4; ++i) row[i] = max(at.from, min(at.p0 + i, at.to - 1));  // (rows that are not filed repeat one that is)
+    for (int layer = blockIdx.y; layer < a.layers; layer += gridDim.y) {
+        if (layer != (int)blockIdx.y) __syncthreads();
+        u32x4 w[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) top = max_u32(top, pair_magnitude(w[e]));
-            const float s = kv8_scale<FORMAT>(row16_max(top));
-            uint32_t c[2];
+        for (int i = 0; i < 4; ++i) w[i] = load_chunk<STREAM>(reinterpret_cast<const u32x4*>(src + layer * a.layer_elems + (int64_t)row[i] * a.row_stride));
+        uint32_t top[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            top[i] = row16_max(max_u32(max_u32(pair_magnitude(w[i][0]), pair_magnitude(w[i][1])), max_u32(pair_magnitude(w[i][2]), pair_magnitude(w[i][3]))));
+        const float s_mine = kv8_scale<FORMAT>(l4 < 2 ? (l4 == 0 ? top[0] : top[1]) : (l4 == 2 ? top[2] : top[3])), r_mine = 1.0f / s_mine;
+        const float s[4] = {quad_lane<0>(s_mine), quad_lane<1>(s_mine), quad_lane<2>(s_mine), quad_lane<3>(s_mine)};
+        const float r[4] = {quad_lane<0>(r_mine), quad_lane<1>(r_mine), quad_lane<2>(r_mine), quad_lane<3>(r_mine)};
+        uint32_t c[2][4];  // four channels' codes of the four rows
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const uint32_t w0 = w[2 * e], w1 = w[2 * e + 1];
-                c[e] = kv8_codes<FORMAT>(bf16_lo(w0), bf16_hi(w0), bf16_lo(w1), bf16_hi(w1), s);
+                const uint32_t w0 = w[i][2 * e], w1 = w[i][2 * e + 1];
+                c[e][i] = kv8_codes<FORMAT>(bf16_lo(w0), bf16_hi(w0), bf16_lo(w1), bf16_hi(w1), s[i], r[i]);
             }
-            if (which == 0) {
-                *reinterpret_cast<u32x2*>(rec + k_byte(p, lane16 * 8)) = u32x2{c[0], c[1]};
-            } else {
+        if (at.which == 0) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) rec[v_byte(p, lane16 * 8 + e)] = (char)(c[e >> 2] >> (8 * (e & 3)));
+            for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x2*>(rec + in_lds(k_byte(at.p0 + i, at.c0))) = u32x2{c[0][i], c[1][i]};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                uint32_t v[4];
+                transpose_bytes(c[e], v);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) *reinterpret_cast<uint32_t*>(rec + in_lds(v_byte(at.p0, at.c0 + 4 * e + j))) = v[j];
             }
-            if (lane16 == 0) *reinterpret_cast<uint16_t*>(rec + k_scale_byte(p) + 64 * which) = (uint16_t)(__builtin_bit_cast(uint32_t, s) >> 16);
         }
+        if ((threadIdx.x & 12) == 0)
+            *reinterpret_cast<uint16_t*>(rec + kLdsScales - kScaleBytes + k_scale_byte(at.p0 + l4) + 64 * at.which) = (uint16_t)(__builtin_bit_cast(uint32_t, s_mine) >> 16);
         __syncthreads();
-        char* dst = a.cache + (((int64_t)layer * a.n_kv + kh) * a.records + record) * kKv8Record;
-        if (from == 0 && to == 32) {
-            for (int i = threadIdx.x; i < kKv8Record / 16; i += kCopyThreads) reinterpret_cast<u32x4*>(dst)[i] = reinterpret_cast<const u32x4*>(rec)[i];
+        char* dst = a.cache + (((int64_t)layer * a.n_kv + kh) * a.records + at.record) * kKv8Record;
+        if (at.from == 0 && at.to == 32) {
+            for (int i = threadIdx.x; i < kKv8Record / 16; i += kCopyThreads)
+                __builtin_nontemporal_store(*reinterpret_cast<const u32x4*>(rec + (i < 512 ? in_lds(16 * i) : kLdsScales - kScaleBytes + 16 * i)), reinterpret_cast<u32x4*>(dst) + i);
             continue;
         }
-        // A record that is filed in part: what belongs to its other positions stays as it is.
-        for (int i = threadIdx.x; i < (to - from) * kHeadDim; i += kCopyThreads) {
-            const int p = from + i / kHeadDim, c = i % kHeadDim;
-            dst[k_byte(p, c)] = rec[k_byte(p, c)];
-            dst[v_byte(p, c)] = rec[v_byte(p, c)];
-            if (c < 2) {
-                const int at = k_scale_byte(p) + 64 * c;
-                *reinterpret_cast<uint16_t*>(dst + at) = *reinterpret_cast<const uint16_t*>(rec + at);
+        // A record that is filed in part: what belongs to its other positions stays as it is. Sixteen bytes of K are a position's, words of V
+        // belong to four, halfwords of scales to one.
+        const auto filed = [&](int p) __attribute__((always_inline)) { return p >= at.from && p < at.to; };
+        for (int i = threadIdx.x; i < kKv8Record / 16; i += kCopyThreads) {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(rec + (i < 512 ? in_lds(16 * i) : kLdsScales - kScaleBytes + 16 * i));
+            if (i < 256) {
+                if (filed(16 * (i >> 7) + (i & 15))) reinterpret_cast<u32x4*>(dst)[i] = x;
+            } else if (i < 512) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int p = 16 * (e & 1) + 4 * ((i >> 4) & 3);
+                    char* word = dst + 16 * i + 4 * e;
+                    if (p >= at.from && p + 3 < at.to) {
+                        *reinterpret_cast<uint32_t*>(word) = x[e];
+                        continue;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (filed(p + j)) word[j] = (char)(x[e] >> (8 * j));
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (filed(16 * (e >> 2) + 4 * (i & 3) + (e & 3))) reinterpret_cast<uint16_t*>(dst)[8 * i + e] = (uint16_t)(x[e >> 1] >> (16 * (e & 1)));
             }
         }
     }
 }
 
-template <int FORMAT>
+template <int FORMAT, bool STREAM>
 __global__ __launch_bounds__(kCopyThreads) void kv8_load_kernel(CopyArgs a) {
-    __shared__ __attribute__((aligned(16))) char rec[kKv8Record];
-    const int kh = blockIdx.y;
-    const int record = (a.first >> 5) + (int)blockIdx.x;
-    const int p0 = record * 32;
-    const int from = max(a.first - p0, 0), to = (int)min((int64_t)a.first + a.count - p0, (int64_t)32);
-    const int lane16 = threadIdx.x & 15;
-    for (int layer = blockIdx.z; layer < a.layers; layer += gridDim.z) {
+    __shared__ __attribute__((aligned(16))) char rec[kLdsScales + 128];
+    const CopyPlace at = copy_place(a);
+    const int kh = at.kh;
+    uint16_t* dst = (at.which ? a.rows[1] : a.rows[0]) + (int64_t)at.record * 32 * a.row_stride + kh * a.head_stride + at.c0;
+    for (int layer = blockIdx.y; layer < a.layers; layer += gridDim.y) {
+        if (layer != (int)blockIdx.y) __syncthreads();
+        const char* src = a.cache + (((int64_t)layer * a.n_kv + kh) * a.records + at.record) * kKv8Record;
+        {
+            // (all of a thread's loads before the first is waited for)
+            const int i = (int)threadIdx.x;
+            const u32x4* from = reinterpret_cast<const u32x4*>(src);
+            const u32x4 x0 = load_chunk<STREAM>(from + i), x1 = load_chunk<STREAM>(from + i + 256);
+            u32x4 x2{};
+            if (i < 8) x2 = load_chunk<STREAM>(from + i + 512);
+            *reinterpret_cast<u32x4*>(rec + in_lds(16 * i)) = x0;
+            *reinterpret_cast<u32x4*>(rec + in_lds(16 * i + 4096)) = x1;
+            if (i < 8) *reinterpret_cast<u32x4*>(rec + kLdsScales + 16 * i) = x2;
+        }
         __syncthreads();
-        const char* src = a.cache + (((int64_t)layer * a.n_kv + kh) * a.records + record) * kKv8Record;
-        for (int i = threadIdx.x; i < kKv8Record / 16; i += kCopyThreads) reinterpret_cast<u32x4*>(rec)[i] = reinterpret_cast<const u32x4*>(src)[i];
-        __syncthreads();
+        uint32_t c[2][4];
+        if (at.which == 0) {
 #pragma unroll
-        for (int turn = 0; turn < 4; ++turn) {
-            const int which = turn >> 1;
-            const int p = (turn & 1) * 16 + (int)(threadIdx.x >> 4);
-            uint32_t c[2] = {0u, 0u};
-            if (which == 0) {
-                const u32x2 w = *reinterpret_cast<const u32x2*>(rec + k_byte(p, lane16 * 8));
-                c[0] = w[0];
-                c[1] = w[1];
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) c[e >> 2] |= (uint32_t)(uint8_t)rec[v_byte(p, lane16 * 8 + e)] << (8 * (e & 3));
+            for (int i = 0; i < 4; ++i) {
+                const u32x2 w = *reinterpret_cast<const u32x2*>(rec + in_lds(k_byte(at.p0 + i, at.c0)));
+                c[0][i] = w[0];
+                c[1][i] = w[1];
             }
-            const float s = __builtin_bit_cast(float, (uint32_t)*reinterpret_cast<const uint16_t*>(rec + k_scale_byte(p) + 64 * which) << 16);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                uint32_t v[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint32_t*>(rec + in_lds(v_byte(at.p0, at.c0 + 4 * e + j)));
+                transpose_bytes(v, c[e]);
+            }
+        }
+        const u32x2 scales = *reinterpret_cast<const u32x2*>(rec + kLdsScales - kScaleBytes + k_scale_byte(at.p0) + 64 * at.which);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t sw = scales[i >> 1];
+            const float s = (i & 1) ? bf16_hi(sw) : bf16_lo(sw);
             u32x4 y;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const uint32_t pair = (e & 1) ? kv8_pair<FORMAT, true>(c[e >> 1]) : kv8_pair<FORMAT, false>(c[e >> 1]);
+                const uint32_t pair = (e & 1) ? kv8_pair<FORMAT, true>(c[e >> 1][i]) : kv8_pair<FORMAT, false>(c[e >> 1][i]);
                 y[e] = pack_bf16(bf16_lo(pair) * s, bf16_hi(pair) * s);
             }
-            if (p >= from && p < to)
-                *reinterpret_cast<u32x4*>(a.rows[which] + layer * a.layer_elems + (p0 + (int64_t)p) * a.row_stride + kh * a.head_stride + lane16 * 8) = y;
+            const int p = at.p0 + i;
+            if (p >= at.from && p < at.to) __builtin_nontemporal_store(y, reinterpret_cast<u32x4*>(dst + layer * a.layer_elems + (int64_t)p * a.row_stride));
         }
     }
 }
@@ -178,12 +251,23 @@ CopyArgs copy_args(const llmi_kv8_copy_args& args) {
     a.count = args.num_pos;
     a.n_kv = args.kv_dim / kHeadDim;
     a.layers = args.layer_num;
+    a.touched = (int32_t)(((int64_t)args.first_pos + args.num_pos - 1) / 32 - args.first_pos / 32 + 1);
+    a.by_head = by_head;
     return a;
 }
 
-dim3 copy_grid(const llmi_kv8_copy_args& args) {
-    const unsigned records = (unsigned)(((int64_t)args.first_pos + args.num_pos - 1) / 32 - args.first_pos / 32 + 1);
-    return dim3(records, (unsigned)(args.kv_dim / kHeadDim), (unsigned)(args.layer_num < 65535 ? args.layer_num : 65535));
+dim3 copy_grid(const CopyArgs& a) { return dim3((unsigned)a.touched * (unsigned)a.n_kv, (unsigned)(a.layers < 65535 ? a.layers : 65535)); }
+
+// Whether what the call reads is more than the memory-side cache may still hold of what was written last (a prompt's prefill, the last step's rows): past
+// the caches then. us, cached loads : past them: 57 MB stored 15.5 : 17.4, 557 MB 146.6 : 134.9; 12 MB read back 6.8 : 7.6, 283 MB 148.0 : 145.7.
+// (What is written goes past them at every size: 57 MB stored 16.6 : 15.5, 12 MB read back 8.6 : 6.8 with cached stores : without, large ones 155.0 : 146.6, 157.6 : 148.0.)
+constexpr int64_t kStreamFrom = 128 << 20;
+bool streams(const llmi_kv8_copy_args& args, int64_t row_bytes) { return (int64_t)args.layer_num * args.num_pos * (args.kv_dim / kHeadDim) * row_bytes > kStreamFrom; }
+
+using CopyKernel = void (*)(CopyArgs);
+void launch_copy(const CopyArgs& a, hipStream_t stream, int format, bool past, CopyKernel e4m3, CopyKernel e4m3_past, CopyKernel whole, CopyKernel whole_past) {
+    const CopyKernel kernel = format == LLMI_KV8_E4M3 ? (past ? e4m3_past : e4m3) : (past ? whole_past : whole);
+    hipLaunchKernelGGL(kernel, copy_grid(a), dim3(kCopyThreads), 0, stream, a);
 }
 
 }  // namespace
@@ -192,8 +276,8 @@ int launch_kv8_store(const llmi_kv8_copy_args& args) {
     if (args.layer_num == 0 || args.num_pos == 0) return LLMI_OK;
     const CopyArgs a = copy_args(args);
     const hipStream_t stream = static_cast<hipStream_t>(args.stream);
-    if (args.format == LLMI_KV8_E4M3) hipLaunchKernelGGL((kv8_store_kernel<LLMI_KV8_E4M3>), copy_grid(args), dim3(kCopyThreads), 0, stream, a);
-    else hipLaunchKernelGGL((kv8_store_kernel<LLMI_KV8_INT8>), copy_grid(args), dim3(kCopyThreads), 0, stream, a);
+    launch_copy(a, stream, args.format, streams(args, 2 * 256), kv8_store_kernel<LLMI_KV8_E4M3, false>, kv8_store_kernel<LLMI_KV8_E4M3, true>, kv8_store_kernel<LLMI_KV8_INT8, false>,
+                kv8_store_kernel<LLMI_KV8_INT8, true>);
     return check_launch();
 }
 
@@ -201,8 +285,8 @@ int launch_kv8_load(const llmi_kv8_copy_args& args) {
     if (args.layer_num == 0 || args.num_pos == 0) return LLMI_OK;
     const CopyArgs a = copy_args(args);
     const hipStream_t stream = static_cast<hipStream_t>(args.stream);
-    if (args.format == LLMI_KV8_E4M3) hipLaunchKernelGGL((kv8_load_kernel<LLMI_KV8_E4M3>), copy_grid(args), dim3(kCopyThreads), 0, stream, a);
-    else hipLaunchKernelGGL((kv8_load_kernel<LLMI_KV8_INT8>), copy_grid(args), dim3(kCopyThreads), 0, stream, a);
+    launch_copy(a, stream, args.format, streams(args, 2 * 130), kv8_load_kernel<LLMI_KV8_E4M3, false>, kv8_load_kernel<LLMI_KV8_E4M3, true>, kv8_load_kernel<LLMI_KV8_INT8, false>,
+                kv8_load_kernel<LLMI_KV8_INT8, true>);
     return check_launch();
 }
 
