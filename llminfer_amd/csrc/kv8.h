@@ -166,6 +166,25 @@ __device__ __forceinline__ void norm_rope_regs32(const NewRow& y, int p, float e
     lo = pack_bf16(l0, l1);
     hi = pack_bf16(h0, h1);
 }
+// The same on 16 lanes, a DPP row: lane p has channels 4p .. 4p + 3 and the four 64 behind them. The bits of norm_rope_row32 (see four_pairs_squared).
+__device__ __forceinline__ void norm_rope_regs16(u32x2& lo, u32x2& hi, u32x2 wl, u32x2 wh, f32x4 sn, f32x4 cs, float eps) {
+    const uint32_t xl0 = lo[0], xl1 = lo[1], xh0 = hi[0], xh1 = hi[1], wl0 = wl[0], wl1 = wl[1], wh0 = wh[0], wh1 = wh[1];
+    const float a[4] = {bf16_lo(xl0), bf16_hi(xl0), bf16_lo(xl1), bf16_hi(xl1)};
+    const float b[4] = {bf16_lo(xh0), bf16_hi(xh0), bf16_lo(xh1), bf16_hi(xh1)};
+    const float wa[4] = {bf16_lo(wl0), bf16_hi(wl0), bf16_lo(wl1), bf16_hi(wl1)};
+    const float wb[4] = {bf16_lo(wh0), bf16_hi(wh0), bf16_lo(wh1), bf16_hi(wh1)};
+    float ss = four_pairs_squared(a, b);
+    ss += dpp_partner<0xB1>(ss);
+    ss += dpp_partner<0x4E>(ss);
+    ss += dpp_partner<0x141>(ss);
+    ss += dpp_partner<0x140>(ss);
+    const float r = inverse_rms(ss, eps);
+    float ol[4], oh[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) rotate_pair(a[e], b[e], wa[e], wb[e], r, sn[e], cs[e], ol[e], oh[e]);
+    lo = u32x2{pack_bf16(ol[0], ol[1]), pack_bf16(ol[2], ol[3])};
+    hi = u32x2{pack_bf16(oh[0], oh[1]), pack_bf16(oh[2], oh[3])};
+}
 // Such a row quantised: its scale, and the codes of lo's and hi's channels in the word's bytes 0, 1 and 2, 3.
 template <int FORMAT>
 __device__ __forceinline__ uint32_t quantise_row32(uint32_t lo, uint32_t hi, float& s) {

@@ -23,6 +23,7 @@ struct RowsArgs {
     const int32_t* pos_dev;  // optional
     int64_t records;   // per KV head
     int32_t pos, rows, head_num, n_kv;
+    uint32_t record_groups;  // many rows: workgroups that have a record
     float eps;
 };
 
@@ -83,6 +84,43 @@ __device__ __forceinline__ u32x4 load_chunk(const u32x4* p) {
 }
 constexpr int kLdsScales = 32 * 272;
 __device__ __forceinline__ int in_lds(int byte) { return byte + (byte >> 8) * 16; }  // (of codes)
+// A record from LDS to where it belongs, positions from .. to - 1 of it.
+__device__ __forceinline__ void write_record(char* dst, const char* rec, int from, int to) {
+    const auto chunk = [&](int i) __attribute__((always_inline)) {
+        return *reinterpret_cast<const u32x4*>(rec + (i < 512 ? in_lds(16 * i) : kLdsScales - kScaleBytes + 16 * i));
+    };
+    if (from == 0 && to == 32) {
+        for (int i = threadIdx.x; i < kKv8Record / 16; i += kCopyThreads) __builtin_nontemporal_store(chunk(i), reinterpret_cast<u32x4*>(dst) + i);
+        return;
+    }
+    // In part: what belongs to its other positions stays as it is. Sixteen bytes of K are a position's, words of V belong to four, halfwords of
+    // scales to one.
+    const auto filed = [&](int p) __attribute__((always_inline)) { return p >= from && p < to; };
+    for (int i = threadIdx.x; i < kKv8Record / 16; i += kCopyThreads) {
+        const u32x4 x = chunk(i);
+        if (i < 256) {
+            if (filed(16 * (i >> 7) + (i & 15))) reinterpret_cast<u32x4*>(dst)[i] = x;
+        } else if (i < 512) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int p = 16 * (e & 1) + 4 * ((i >> 4) & 3);
+                char* word = dst + 16 * i + 4 * e;
+                if (p >= from && p + 3 < to) {
+                    *reinterpret_cast<uint32_t*>(word) = x[e];
+                    continue;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (filed(p + j)) word[j] = (char)(x[e] >> (8 * j));
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (filed(16 * (e >> 2) + 4 * (i & 3) + (e & 3))) reinterpret_cast<uint16_t*>(dst)[8 * i + e] = (uint16_t)(x[e >> 1] >> (16 * (e & 1)));
+        }
+    }
+}
+
 struct CopyPlace {
     int kh, record, from, to;     // positions from .. to - 1 of the record are the call's
     int which, p0, c0;            // the lane's first position and channel
@@ -147,38 +185,7 @@ __global__ __launch_bounds__(kCopyThreads) void kv8_store_kernel(CopyArgs a) {
         if ((threadIdx.x & 12) == 0)
             *reinterpret_cast<uint16_t*>(rec + kLdsScales - kScaleBytes + k_scale_byte(at.p0 + l4) + 64 * at.which) = (uint16_t)(__builtin_bit_cast(uint32_t, s_mine) >> 16);
         __syncthreads();
-        char* dst = a.cache + (((int64_t)layer * a.n_kv + kh) * a.records + at.record) * kKv8Record;
-        if (at.from == 0 && at.to == 32) {
-            for (int i = threadIdx.x; i < kKv8Record / 16; i += kCopyThreads)
-                __builtin_nontemporal_store(*reinterpret_cast<const u32x4*>(rec + (i < 512 ? in_lds(16 * i) : kLdsScales - kScaleBytes + 16 * i)), reinterpret_cast<u32x4*>(dst) + i);
-            continue;
-        }
-        // A record that is filed in part: what belongs to its other positions stays as it is. Sixteen bytes of K are a position's, words of V
-        // belong to four, halfwords of scales to one.
-        const auto filed = [&](int p) __attribute__((always_inline)) { return p >= at.from && p < at.to; };
-        for (int i = threadIdx.x; i < kKv8Record / 16; i += kCopyThreads) {
-            const u32x4 x = *reinterpret_cast<const u32x4*>(rec + (i < 512 ? in_lds(16 * i) : kLdsScales - kScaleBytes + 16 * i));
-            if (i < 256) {
-                if (filed(16 * (i >> 7) + (i & 15))) reinterpret_cast<u32x4*>(dst)[i] = x;
-            } else if (i < 512) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int p = 16 * (e & 1) + 4 * ((i >> 4) & 3);
-                    char* word = dst + 16 * i + 4 * e;
-                    if (p >= at.from && p + 3 < at.to) {
-                        *reinterpret_cast<uint32_t*>(word) = x[e];
-                        continue;
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (filed(p + j)) word[j] = (char)(x[e] >> (8 * j));
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (filed(16 * (e >> 2) + 4 * (i & 3) + (e & 3))) reinterpret_cast<uint16_t*>(dst)[8 * i + e] = (uint16_t)(x[e >> 1] >> (16 * (e & 1)));
-            }
-        }
+        write_record(a.cache + (((int64_t)layer * a.n_kv + kh) * a.records + at.record) * kKv8Record, rec, at.from, at.to);
     }
 }
 
@@ -237,6 +244,83 @@ __global__ __launch_bounds__(kCopyThreads) void kv8_load_kernel(CopyArgs a) {
     }
 }
 
+// The rows of many tokens. The first workgroups, whose way is the longest, have a record of a KV head each as kv8_store has: wavefront w sixteen positions
+// of K (w < 2) or V, a lane four of them; the others a token's queries each, sixteen lanes a row, the weights, sines and cosines in registers for all of a
+// wavefront's.
+template <int FORMAT>
+__global__ __launch_bounds__(kCopyThreads) void kv8_append_many_kernel(RowsArgs a) {
+    __shared__ __attribute__((aligned(16))) char rec[kLdsScales + 128];
+    const int lane = (int)(threadIdx.x & 63), wave = (int)(threadIdx.x >> 6), l16 = lane & 15, l4 = lane & 3;
+    const int base = a.pos_dev ? max(0, min(*a.pos_dev, a.pos)) : a.pos;
+    const u32x2* weight = reinterpret_cast<const u32x2*>(a.weight);
+    if (blockIdx.x >= a.record_groups) {
+        const int row = (int)(blockIdx.x - a.record_groups);
+        const int64_t table = (int64_t)(base + row) * 64 + 4 * l16;
+        const u32x2 wl = weight[l16], wh = weight[l16 + 16];
+        const f32x4 sn = *reinterpret_cast<const f32x4*>(a.sin_cache + table), cs = *reinterpret_cast<const f32x4*>(a.cos_cache + table);
+        const u32x2* src = reinterpret_cast<const u32x2*>(a.query_src + row * a.query_src_stride);
+        u32x2* dst = reinterpret_cast<u32x2*>(a.query + row * a.query_stride);
+        for (int h = (int)(threadIdx.x >> 4); h < a.head_num; h += kCopyThreads / 16) {
+            u32x2 lo = src[h * 32 + l16], hi = src[h * 32 + 16 + l16];
+            norm_rope_regs16(lo, hi, wl, wh, sn, cs, a.eps);
+            dst[h * 32 + l16] = lo;
+            dst[h * 32 + 16 + l16] = hi;
+        }
+        return;
+    }
+    const int b = (int)blockIdx.x, record = base / 32 + b / a.n_kv, kh = b % a.n_kv;
+    const int from = max(base - record * 32, 0), to = min(base + a.rows - record * 32, 32);  // (max_seq_len bounds both sums)
+    if (to <= 0) return;  // (a position read on the device needs a record less than the launch has room for, perhaps)
+    const bool is_v = wave >> 1;
+    const int p0 = 16 * (wave & 1) + 4 * (lane >> 4), c0 = 4 * l16;
+    u32x2 lo[4], hi[4];
+    int64_t row[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        row[i] = record * 32 + max(from, min(p0 + i, to - 1)) - base;  // (rows that are not filed repeat one that is)
+        const uint16_t* src = (is_v ? a.value_new + row[i] * a.value_new_stride : a.key_new + row[i] * a.key_new_stride) + kh * kHeadDim;
+        lo[i] = reinterpret_cast<const u32x2*>(src)[l16];
+        hi[i] = reinterpret_cast<const u32x2*>(src)[l16 + 16];
+    }
+    if (!is_v) {
+        const u32x2 wl = weight[32 + l16], wh = weight[48 + l16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t table = (base + row[i]) * 64 + 4 * l16;
+            norm_rope_regs16(lo[i], hi[i], wl, wh, *reinterpret_cast<const f32x4*>(a.sin_cache + table), *reinterpret_cast<const f32x4*>(a.cos_cache + table), a.eps);
+        }
+    }
+    uint32_t top[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        top[i] = row16_max(max_u32(max_u32(pair_magnitude(lo[i][0]), pair_magnitude(lo[i][1])), max_u32(pair_magnitude(hi[i][0]), pair_magnitude(hi[i][1]))));
+    const float s_mine = kv8_scale<FORMAT>(l4 < 2 ? (l4 == 0 ? top[0] : top[1]) : (l4 == 2 ? top[2] : top[3])), r_mine = 1.0f / s_mine;
+    const float s[4] = {quad_lane<0>(s_mine), quad_lane<1>(s_mine), quad_lane<2>(s_mine), quad_lane<3>(s_mine)};
+    const float r[4] = {quad_lane<0>(r_mine), quad_lane<1>(r_mine), quad_lane<2>(r_mine), quad_lane<3>(r_mine)};
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        uint32_t c[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t w0 = e ? hi[i][0] : lo[i][0], w1 = e ? hi[i][1] : lo[i][1];
+            c[i] = kv8_codes<FORMAT>(bf16_lo(w0), bf16_hi(w0), bf16_lo(w1), bf16_hi(w1), s[i], r[i]);
+        }
+        if (!is_v) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *reinterpret_cast<uint32_t*>(rec + in_lds(k_byte(p0 + i, c0 + 64 * e))) = c[i];
+        } else {
+            uint32_t v[4];
+            transpose_bytes(c, v);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) *reinterpret_cast<uint32_t*>(rec + in_lds(v_byte(p0, c0 + 64 * e + j))) = v[j];
+        }
+    }
+    if ((lane & 12) == 0)
+        *reinterpret_cast<uint16_t*>(rec + kLdsScales - kScaleBytes + k_scale_byte(p0 + l4) + 64 * is_v) = (uint16_t)(__builtin_bit_cast(uint32_t, s_mine) >> 16);
+    __syncthreads();
+    write_record(a.cache + (kh * a.records + record) * kKv8Record, rec, from, to);
+}
+
 CopyArgs copy_args(const llmi_kv8_copy_args& args) {
     CopyArgs a;
     const bool by_head = args.kv_layout == LLMI_KV_LAYOUT_HEAD_MAJOR;
@@ -290,6 +374,9 @@ int launch_kv8_load(const llmi_kv8_copy_args& args) {
     return check_launch();
 }
 
+// Tokens from which a record is put together by a workgroup: half a wavefront a row, which scatters V's bytes, has the shorter way. us, half a wavefront a row :
+// records, 32 Q / 8 KV heads: 2.3 : 4.3 with 1 token, 3.2 : 4.7 with 40, 5.95 : 5.94 with 300, 12.3 : 8.6 with 1001; 64 Q heads 16.7 : 11.6, 16 Q 11.5 : 8.0.
+constexpr int kManyRows = 384;
 int launch_qk_norm_rope_append_kv8(const llmi_qk_norm_rope_kv8_args& args) {
     const int64_t q_row = (int64_t)args.head_num * kHeadDim;
     RowsArgs a;
@@ -312,6 +399,15 @@ int launch_qk_norm_rope_append_kv8(const llmi_qk_norm_rope_kv8_args& args) {
     a.rows = args.row_num;
     a.head_num = args.head_num;
     a.eps = args.eps;
+    if (args.row_num >= kManyRows) {
+        // (at a position on the device the rows may begin anywhere in a record)
+        const int64_t records = args.pos_device ? (args.row_num + 30) / 32 + 1 : ((int64_t)args.pos + args.row_num - 1) / 32 - args.pos / 32 + 1;
+        a.record_groups = (uint32_t)(records * a.n_kv);
+        const dim3 grid((unsigned)args.row_num + a.record_groups);
+        if (args.format == LLMI_KV8_E4M3) hipLaunchKernelGGL((kv8_append_many_kernel<LLMI_KV8_E4M3>), grid, dim3(kCopyThreads), 0, static_cast<hipStream_t>(args.stream), a);
+        else hipLaunchKernelGGL((kv8_append_many_kernel<LLMI_KV8_INT8>), grid, dim3(kCopyThreads), 0, static_cast<hipStream_t>(args.stream), a);
+        return check_launch();
+    }
     const int per = kRowThreads / 32;
     const dim3 grid((unsigned)((args.head_num + 2 * a.n_kv + per - 1) / per), (unsigned)(args.row_num < 65535 ? args.row_num : 65535));
     const hipStream_t stream = static_cast<hipStream_t>(args.stream);

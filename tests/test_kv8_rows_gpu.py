@@ -194,6 +194,37 @@ def test_rows_in_place_from_slices_and_at_a_position_on_the_device(dev, how):
         assert same_bits(a[keep], b[keep])
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("pos,n,how", [
+    (0, 384, {}), (17, 500, dict(inplace=True)), (100, 449, dict(wide=True)), (64, 1001, dict(device_pos=31)), (64, 385, dict(device_pos=64)), (90, 416, dict(device_pos=-7)),
+    (31, 386, dict(device_pos=500)), (1, 383, {}), (5, 383, dict(device_pos=2)),
+])
+def test_rows_of_many_tokens(dev, pos, n, how, fmt):
+    """From some hundred tokens on records are put together by workgroups: the same bits as token by token, whole and at the edges."""
+    n_q, n_kv, msl = 12, 3, pos + n + 3
+    out, cache, before, at, ref = appended(dev, n_q, n_kv, msl, pos, n, fmt, seed=n, **how)
+    assert bool(((out.double() - ref["q"]).abs() <= 2.0 ** -8 * ref["q"].abs() + 1e-5).all())
+    kc, ks, vc, vs = C.unpack(cache)
+    codes, scale = C.quantise(ref["v"].transpose(0, 1), fmt)
+    assert torch.equal(vc[1, :, at:at + n], codes) and torch.equal(vs[1, :, at:at + n], scale)
+    keep = torch.ones(2, n_kv, kc.shape[2], dtype=torch.bool)
+    keep[1, :, at:at + n] = False
+    for a, b in zip(C.unpack(cache), C.unpack(before)):
+        assert same_bits(a[keep], b[keep])
+    # the same tokens in calls of a few
+    g = torch.Generator().manual_seed(n)
+    packed = torch.randn(n, (n_q + 2 * n_kv) * D + (40 if how.get("wide") else 0), generator=g).to(BF16).to(dev)
+    w = (1 + 0.1 * torch.randn(2 * D, generator=g)).to(BF16).to(dev)
+    sin, cos = (x.to(dev) for x in C.tables(msl))
+    few, q_few = before.to(dev), torch.zeros(n, n_q * D, dtype=BF16, device=dev)
+    for i in range(0, n, 100):
+        rows = packed[i:i + 100]
+        q, k, v = rows[:, :n_q * D], rows[:, n_q * D:(n_q + n_kv) * D], rows[:, (n_q + n_kv) * D:(n_q + 2 * n_kv) * D]
+        ops.qk_norm_rope_append_kv8(q_few[i:i + 100], k, v, few, w, sin, cos, row_num=rows.shape[0], layer_id=1, pos=at + i, kv_dim=n_kv * D, head_num=n_q, head_dim=D,
+                                    max_seq_len=msl, kv8_format=fmt, query_src=q)
+    assert torch.equal(few.cpu(), cache) and torch.equal(q_few.cpu().view(n, n_q, D), out)
+
+
 def test_what_the_front_end_refuses(dev):
     u8 = torch.zeros(2 * 8320, dtype=torch.uint8, device=dev)
     x = torch.zeros(64, D, dtype=BF16, device=dev)
