@@ -77,8 +77,8 @@ int validate_copy(const llmi_kv8_copy_args* a) {
     if (a->layer_num < 0) return LLMI_ERR_INVALID_ARG;
     if (a->first_pos < 0 || a->num_pos < 0 || a->first_pos > a->max_seq_len || a->num_pos > a->max_seq_len - a->first_pos) return LLMI_ERR_POS_RANGE;
     if (a->kv_layout != LLMI_KV_LAYOUT_POS_MAJOR && a->kv_layout != LLMI_KV_LAYOUT_HEAD_MAJOR) return LLMI_ERR_LAYOUT;
-    // (a workgroup per record and KV head; no such cache fits a GPU)
-    if (kv8_records(a->max_seq_len) * (a->kv_dim / 128) > INT32_MAX) return LLMI_ERR_INVALID_ARG;
+    // (a workgroup per record and KV head: no layer of a bf16 cache that fits a GPU has more)
+    if (kv8_records(a->max_seq_len) * (a->kv_dim / 128) > kKv8MostGroups) return LLMI_ERR_INVALID_ARG;
     if (!aligned(a->key_cache, 16) || !aligned(a->value_cache, 16) || !aligned(a->cache8, 16)) return LLMI_ERR_ALIGNMENT;
     return LLMI_OK;
 }

@@ -399,9 +399,9 @@ int launch_qk_norm_rope_append_kv8(const llmi_qk_norm_rope_kv8_args& args) {
     a.rows = args.row_num;
     a.head_num = args.head_num;
     a.eps = args.eps;
-    if (args.row_num >= kManyRows) {
-        // (at a position on the device the rows may begin anywhere in a record)
-        const int64_t records = args.pos_device ? (args.row_num + 30) / 32 + 1 : ((int64_t)args.pos + args.row_num - 1) / 32 - args.pos / 32 + 1;
+    // (at a position on the device the rows may begin anywhere in a record)
+    const int64_t records = args.pos_device ? ((int64_t)args.row_num + 30) / 32 + 1 : ((int64_t)args.pos + args.row_num - 1) / 32 - args.pos / 32 + 1;
+    if (args.row_num >= kManyRows && args.row_num + records * a.n_kv <= kKv8MostGroups) {
         a.record_groups = (uint32_t)(records * a.n_kv);
         const dim3 grid((unsigned)args.row_num + a.record_groups);
         if (args.format == LLMI_KV8_E4M3) hipLaunchKernelGGL((kv8_append_many_kernel<LLMI_KV8_E4M3>), grid, dim3(kCopyThreads), 0, static_cast<hipStream_t>(args.stream), a);

@@ -144,11 +144,14 @@ int launch_verify_tree(const llmi_verify_tree_args& args);
 int launch_kv_commit_tree(const llmi_kv_commit_tree_args& args);
 // The 8-bit cache (kv8.h, kv8_api.cpp).
 constexpr int kKv8Record = LLMI_KV8_RECORD_BYTES;
+constexpr int64_t kKv8MostGroups = (1 << 24) - 1;  // workgroups of 256 threads along a grid's x: their threads are counted with 32 bits
 inline int64_t kv8_records(int32_t max_seq_len) { return ((int64_t)max_seq_len + LLMI_KV8_RECORD_POSITIONS - 1) / LLMI_KV8_RECORD_POSITIONS; }
-// The splits that a KV head's records are dealt to where there may be `splits`: one for short contexts, else a record each at least.
+// The splits that a KV head's records are dealt to where there may be `splits` (measurements: kv8_api.cpp): one for short contexts, then a record each
+// up to 32, then three records each.
 constexpr int kKv8Single = 10;
 LLMI_HOST_DEVICE constexpr int kv8_active_splits(int64_t tiles, int splits) {
-    return tiles <= kKv8Single || splits < 2 ? 1 : tiles < splits ? (int)tiles : splits;
+    const int64_t most = tiles <= 32 ? tiles : tiles <= 96 ? 32 : tiles / 3;
+    return tiles <= kKv8Single || splits < 2 ? 1 : most < splits ? (int)most : splits;
 }
 // How the attention takes a call (rules and measurements: kv8_api.cpp): splits of a KV head, wavefronts of a workgroup (4 or 8), fewest splits at
 // which a KV head's query heads are joined by different workgroups.

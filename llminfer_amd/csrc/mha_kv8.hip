@@ -260,11 +260,14 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
             const float m_new = fmaxf(m_run, top);
             const float alpha = fast_exp2(m_run - m_new);
             m_run = m_new;
-            l_run *= alpha;
+            // (a wavefront's first record finds zeros)
+            if (__any(l_run != 0.0f)) {
+                l_run *= alpha;
 #pragma unroll
-            for (int b = 0; b < 8; ++b)
+                for (int b = 0; b < 8; ++b)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[b][e] *= alpha;
+                    for (int e = 0; e < 4; ++e) o[b][e] *= alpha;
+            }
         }
         u32x4 ph, pl;
 #pragma unroll

@@ -113,6 +113,7 @@ def test_rows_status_codes(over, status):
     (dict(key_cache=0), "NULL_POINTER"), (dict(cache8=0), "NULL_POINTER"), (dict(value_cache=0x1008), "ALIGNMENT"), (dict(layer_num=-1), "INVALID_ARG"), (dict(first_pos=-1), "POS_RANGE"),
     (dict(num_pos=-1), "POS_RANGE"), (dict(first_pos=4000, num_pos=97), "POS_RANGE"), (dict(first_pos=(1 << 31) - 1, num_pos=(1 << 31) - 1), "POS_RANGE"), (dict(kv_layout=2), "LAYOUT"),
     (dict(format=2), "INVALID_ARG"), (dict(head_dim=64), "HEAD_DIM"), (dict(kv_dim=64), "KV_DIM"), (dict(max_seq_len=-4), "INVALID_ARG"),
+    (dict(max_seq_len=(1 << 31) - 1), "INVALID_ARG"),
 ])
 def test_copy_status_codes(over, status):
     a = B.Kv8CopyArgs()

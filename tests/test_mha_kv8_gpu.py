@@ -60,6 +60,80 @@ def test_splits(dev, splits, fmt):
     assert all(torch.equal(x[1], tap) for x in again)
 
 
+@pytest.mark.parametrize("n_q,n_kv,keys,splits", [(256, 16, 3000, 0), (144, 9, 2500, 70), (144, 9, 2500, 3), (130, 10, 700, 0), (160, 160, 1100, 0), (300, 300, 800, 20), (192, 12, 9000, 256)])
+def test_more_heads_than_are_joined_by_workgroups_of_their_own(dev, n_q, n_kv, keys, splits):
+    """Over 128 query heads one workgroup joins all of a KV head's: a wavefront each, or all of them in turn where there are over 64 splits."""
+    g = torch.Generator().manual_seed(n_q + splits)
+    cache, k, v = C.filled(1, n_kv, keys, keys, C.E4M3, keys)
+    q = C.rows(g, n_q, outliers=False)
+    want = C.attention(q, k[0], v[0])
+    cache, ws = cache.to(dev), torch.full((n_q * 528 * 256 // 4 + 64,), math.nan, device=dev)
+    taps = []
+    for _ in range(2):
+        out, tap = decode(dev, q.to(dev), cache, n_kv, keys, keys - 1, C.E4M3, layer_id=0, num_splits=splits, ws=ws)
+        C.close(tap, *want, rounded=out)
+        taps.append(tap)
+    assert torch.equal(*taps)
+
+
+def test_offsets_past_32_bits(dev):
+    """A layer that starts past 4 GiB of the cache, and one KV head whose records alone pass 4 GiB."""
+    n_kv, msl, layers = 8, 131072, 17
+    per = ops.kv8_bytes(1, msl, n_kv * D, D)
+    assert per * (layers - 1) > 1 << 32
+    big = torch.empty(per * layers, dtype=torch.uint8, device=dev)
+    g = torch.Generator().manual_seed(1)
+    small, k, v = C.filled(1, n_kv, 700, 700, C.INT8, 8)
+    last = big[per * (layers - 1):].view(1, n_kv, msl // 32, C.RECORD)
+    last[:, :, :small.shape[2]] = small.to(dev)
+    q = C.rows(g, 16, outliers=False)
+    out, tap = decode(dev, q.to(dev), big, n_kv, msl, 699, C.INT8, layer_id=layers - 1)
+    C.close(tap, *C.attention(q, k[0], v[0]), rounded=out)
+    del big, last
+    # all codes 0 but the rows of one token at the end, whose score outweighs the others': its V row comes out
+    msl = (1 << 32) // 260 + 4000
+    cache = torch.zeros(ops.kv8_bytes(1, msl, D, D), dtype=torch.uint8, device=dev)
+    assert cache.numel() > 1 << 32
+    x = torch.randn(3, D, generator=g).to(BF16)
+    sin, cos, w = torch.zeros(msl, 64, device=dev), torch.ones(msl, 64, device=dev), torch.full((2 * D,), 3.0, dtype=BF16, device=dev)
+    kv = torch.stack([x[0], x[2]]).to(dev)
+    ops.mha_decode_append_kv8(kv[0], kv[0], kv[1], w, sin, cos, cache, torch.zeros(D, dtype=BF16, device=dev), workspace(dev, 1, msl), layer_id=0, pos=msl - 1, kv_dim=D, kv_mul=1, head_num=1,
+                              head_dim=D, max_seq_len=msl, kv8_format=C.INT8)
+    out, tap = decode(dev, (3 * kv[0]).view(1, D), cache, 1, msl, msl - 1, C.INT8, layer_id=0)
+    codes, scale = C.quantise(x[2].view(1, D), C.INT8)
+    row = C.stands_for(codes, scale, C.INT8)
+    # (score 3 x 3 |x|^2 / sqrt(128) = 100 above the others': 16.5 million weights of e^-100)
+    assert bool(((tap.double() - row).abs() <= 2.0 ** -15 * row.abs()).all())
+
+
+def test_two_graphs_that_share_a_workspace(dev):
+    """Captured calls of two models (other heads, lengths, codes) with one workspace, replayed in turn with eager calls between."""
+    g = torch.Generator().manual_seed(55)
+    ws = torch.full((ops.workspace_bytes(32, D, 8192) // 4,), math.nan, device=dev)
+    made = []
+    for n_q, n_kv, keys, fmt in ((32, 8, 4100, C.E4M3), (24, 2, 1800, C.INT8)):
+        cache, k, v = C.filled(1, n_kv, keys, keys, fmt, keys)
+        q, cache = C.rows(g, n_q, outliers=False), cache.to(dev)
+        q_dev, out, tap = q.to(dev), torch.zeros(n_q, D, dtype=BF16, device=dev), torch.zeros(n_q, D, device=dev)
+
+        def call(q_dev=q_dev, cache=cache, out=out, tap=tap, n_q=n_q, n_kv=n_kv, keys=keys, fmt=fmt):
+            ops.mha_decode_kv8(q_dev, cache, out, ws, output_f32=tap, layer_id=0, pos=keys - 1, kv_dim=n_kv * D, kv_mul=n_q // n_kv, head_num=n_q, head_dim=D, max_seq_len=keys,
+                               kv8_format=fmt)
+
+        call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call()
+        made.append((graph, call, out, tap, C.attention(q, k[0], v[0])))
+    for turn in range(6):
+        for graph, call, out, tap, want in made:
+            out.zero_(), tap.zero_()
+            graph.replay() if turn != 3 else call()
+            torch.cuda.synchronize()
+            C.close(tap.cpu(), *want, rounded=out.cpu())
+
+
 def test_without_a_workspace_and_with_little(dev):
     g = torch.Generator().manual_seed(3)
     keys, n_q, n_kv = 5000, 8, 2
