@@ -43,8 +43,14 @@ size_t split_bytes(const llmi_mha_kv8_args* a) { return (size_t)a->head_num * (1
 
 // A KV head's query heads are joined by different workgroups where those, which wait for each other, fit the chip with room to spare.
 constexpr int kMostJoining = 128;
+// Records up to which four workgroups of a KV head have 32 columns and all positions each: K's codes are read and multiplied four times, V's once, and
+// there is nothing to join. us, splits by the rule below : so, 32 Q / 8 KV heads E4M3: 2.69 : 2.45 at 21 positions, 2.94 : 2.56 at 128, 4.16 : 3.39 at 256, 4.54 : 3.83
+// at 320, 4.66 : 4.25 at 401, 4.67 : 4.35 at 512, 4.66 : 4.64 at 601, 4.73 : 5.19 at 701; with the new token 3.89 : 3.36 at 57, 5.06 : 4.47 at 300 (16 Q), 5.51 : 4.98
+// at 511. Whole numbers, whose conversion takes three times the instructions: 4.97 : 4.18 at 320, 4.86 : 5.08 at 401. (Sixteen wavefronts beyond eight records
+// 0.2 - 0.5 slower.)
+constexpr int kMostSliced = 18, kMostSlicedWhole = 12;
 
-// The workgroups a KV head's records are dealt to: one up to ten records (kKv8Single), then a record each up to one workgroup per compute unit. us by
+// The workgroups a KV head's records are dealt to beyond that: one up to ten records (kKv8Single), then a record each up to one workgroup per compute unit. us by
 // splits, 32 Q / 8 KV heads, E4M3: 4.54 : 4.83 : 4.71 with 1 : 5 : 10 at 301 positions, 5.24 : 4.95 : 4.73 with 1 : 5 : 13 at 401, 5.52 : 4.85 : 4.71 with
 // 1 : 8 : 16 at 512, 4.90 : 4.75 with 16 : 32 at 1024, 5.68 : 6.55 with 32 : 64 at 4096, 7.31 : 7.96 at 8192, 14.2 : 15.9 at 32768, 42.7 : 45.6 at 131001.
 // Eight wavefronts a workgroup where four would have more than a record each alone, more than five in a split (each wavefront has one record on
@@ -66,6 +72,18 @@ int make_form(const llmi_mha_kv8_args* a, int new_rows, Kv8Form* form) {
     }
     form->splits = (int)std::max<int64_t>(want, 1);
     form->waves = tiles > (form->splits == 1 ? 4 : 5 * (int64_t)form->splits) ? 8 : 4;
+    form->sliced = 0;
+    if (a->num_splits == 0) {
+        const int most = a->format == LLMI_KV8_E4M3 ? kMostSliced : kMostSlicedWhole;
+        if (a->pos_device) {  // (one workgroup size for all lengths up to the bound)
+            form->sliced = most;
+            if (tiles > 4) form->waves = 8;
+        } else if (tiles <= most) {
+            form->sliced = most;
+            form->splits = 1;
+            form->waves = tiles > 4 ? 8 : 4;
+        }
+    }
     form->spread_min = a->head_num <= kMostJoining ? 2 : INT32_MAX;
     return LLMI_OK;
 }

@@ -157,7 +157,9 @@ LLMI_HOST_DEVICE constexpr int kv8_active_splits(int64_t tiles, int splits) {
 // which a KV head's query heads are joined by different workgroups.
 struct Kv8Form {
     int splits, waves, spread_min;
+    int sliced;  // records up to which four workgroups of a KV head have 32 columns and all positions each (position on the host: 0 or its own)
 };
+constexpr int kKv8Slices = 4;
 int launch_mha_kv8(const llmi_mha_kv8_args& args, const llmi_mha_kv8_append_args* append, const Kv8Form& form);
 hipError_t poll_timeouts_kv8(unsigned int* n);
 int launch_qk_norm_rope_append_kv8(const llmi_qk_norm_rope_kv8_args& args);

@@ -42,6 +42,7 @@ struct Kv8Args {
     uint32_t tag;
     int32_t pos, group, n_q, splits, max_polls;
     int32_t run, longer;          // records per split, and how many splits take one more (position known on the host)
+    int32_t sliced;               // position read on the device: records up to which a workgroup has 32 columns and all of them
     int32_t spread_min;           // fewest splits at which a KV head's query heads are joined by different workgroups
     float scale_log2e;            // log2(e) / sqrt(128)
     // the new token's
@@ -53,78 +54,63 @@ struct Kv8Args {
     float eps;
 };
 
+// CHUNKS: the 1 KiB chunks of V's codes that a workgroup reads, all four or one.
+template <int CHUNKS>
 struct Record {
-    u32x4 k[4], v[4], ks, vs;  // codes, the lane's eight scales
+    u32x4 k[4], v[CHUNKS], ks, vs;  // codes, the lane's eight scales
 };
 
-// Streaming loads: nobody reads a record twice.
-constexpr int kStream = 2;
-// (a record that there is not: zeros, and nothing read)
-__device__ __forceinline__ Record load_record(const char* at, bool there, uint32_t lane) {
+// (a record that there is not: zeros, and nothing read). Whole records are streamed, nobody reads one twice; where four workgroups read the same K codes they are not.
+template <int CHUNKS>
+__device__ __forceinline__ Record<CHUNKS> load_record(const char* at, bool there, uint32_t lane, int chunk) {
     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(at), 0, there ? kKv8Record : 0, 0x00020000);
     auto load = [&](uint32_t lane_at, int offset) __attribute__((always_inline)) {
-        return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, lane_at, offset, kStream));
+        constexpr int kStream = 2;
+        return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, lane_at, offset, CHUNKS == 4 ? kStream : 0));
     };
-    Record y;
+    Record<CHUNKS> y;
 #pragma unroll
     for (int i = 0; i < 4; ++i) y.k[i] = load(lane * 16u, i * 1024);
     y.ks = load((lane >> 4) * 16u, kScaleBytes);
     y.vs = load((lane >> 4) * 16u, kScaleBytes + 64);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y.v[i] = load(lane * 16u, kVBytes + i * 1024);
+    for (int i = 0; i < CHUNKS; ++i) y.v[i] = load(lane * 16u, kVBytes + (chunk + i) * 1024);
     return y;
 }
 
-template <int FORMAT, int NW, bool APPEND>
-__global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
-    __shared__ __attribute__((aligned(16))) float parts[NW][kHeads][kHeadDim];
-    __shared__ float part_m[kHeads][NW], part_l[kHeads][NW];
-    __shared__ __attribute__((aligned(16))) float weights[NW][2][32];
-    __shared__ float fin[kHeads][2];
-    __shared__ bool arrived[NW];
-    __shared__ __attribute__((aligned(16))) uint16_t rows[APPEND ? kHeads : 1][kHeadDim];
-    __shared__ __attribute__((aligned(16))) uint8_t new_codes[APPEND ? 2 : 1][kHeadDim];
-    __shared__ float new_scale[2];
+template <int NW, int COLUMNS>
+struct Kv8Shared {
+    __attribute__((aligned(16))) float parts[NW][kHeads][COLUMNS];
+    __attribute__((aligned(16))) float weights[NW][2][32];
+    __attribute__((aligned(16))) uint16_t rows[kHeads][kHeadDim];  // the new token's query heads
+    __attribute__((aligned(16))) uint8_t new_codes[2][kHeadDim];
+    float part_m[kHeads][NW], part_l[kHeads][NW], fin[kHeads][2], new_scale[2];
+    bool arrived[NW];
+};
+
+// The new token's row `at` of a KV head: its query heads, then K and V.
+__device__ __forceinline__ void ask_row(const Kv8Args& a, NewRow& row, int kvh, int at, int p32) {
+    const bool is_new = at >= a.group;
+    const uint64_t new_row = reinterpret_cast<uint64_t>(at > a.group ? a.v_new : a.k_new) + (uint64_t)(uint32_t)(kvh * 256);
+    const uint64_t q_row = reinterpret_cast<uint64_t>(a.q) + (uint64_t)(uint32_t)((kvh * a.group + at) * 256);
+    load_row32(row, is_new ? new_row : q_row, reinterpret_cast<uint64_t>(a.norm_w) + (is_new ? 256u : 0u), p32);
+}
+
+// SLICED: the workgroup has 32 of the 128 columns and every position, split is which (nothing to join). Otherwise all columns and its split's run. `row`: what does
+// not depend on the position of the half wavefront's first new row has been asked for.
+template <int FORMAT, int NW, bool APPEND, bool SLICED, int COLUMNS>
+__device__ __forceinline__ void kv8_attend(const Kv8Args& a, Kv8Shared<NW, COLUMNS>& sm, NewRow& row, int pos, int active, int run, int longer) {
+    constexpr int kChunks = SLICED ? 1 : 4, kColumns = 32 * kChunks;
+    auto& parts = sm.parts;
+    auto& part_m = sm.part_m;
+    auto& part_l = sm.part_l;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
-    const int kvh = blockIdx.x, split = blockIdx.y;
-
-    // The new token's rows, half a wavefront each: the query heads, and (the last split files them) K and V behind them. What does not depend on the
-    // position is asked for in front of it, everything else in front of the records.
+    const int kvh = blockIdx.x, split = SLICED ? 0 : blockIdx.y, slice = SLICED ? blockIdx.y : 0;
     const int p32 = lane & 31;
     const int half = (int)(threadIdx.x >> 5);
     const int work_rows = a.group + 2;
-    NewRow row;
-    auto ask_row = [&](int at) __attribute__((always_inline)) {
-        const bool is_new = at >= a.group;
-        const uint64_t new_row = reinterpret_cast<uint64_t>(at > a.group ? a.v_new : a.k_new) + (uint64_t)(uint32_t)(kvh * 256);
-        const uint64_t q_row = reinterpret_cast<uint64_t>(a.q) + (uint64_t)(uint32_t)((kvh * a.group + at) * 256);
-        load_row32(row, is_new ? new_row : q_row, reinterpret_cast<uint64_t>(a.norm_w) + (is_new ? 256u : 0u), p32);
-    };
-    // (half wavefronts without a row take the last one again: a branch around the loads would make their wait one for all of the records' too)
-    if constexpr (APPEND) ask_row(min(half, work_rows - 1));
-    int pos = a.pos, active = a.splits, run = a.run, longer = a.longer;
-    if (a.pos_dev) {
-        // (constant address space: a scalar load; nothing in the launch writes the position)
-        const auto word = reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(a.pos_dev));
-        pos = max(0, min(*word, a.pos));
-        const int tiles = (int)(((int64_t)pos + (APPEND ? 0 : 1) + 31) >> 5);
-        active = kv8_active_splits(tiles, a.splits);
-        if (split >= active) return;
-        // (a quotient in two steps of 24 bits, then one up or down: two orders shorter than the compiler's division, and on the way to the first load)
-        const float inverse = 1.0f / (float)active;
-        run = (int)((float)tiles * inverse);
-        run += (int)((float)(tiles - run * active) * inverse);
-        longer = tiles - run * active;
-        if (longer < 0) {
-            --run;
-            longer += active;
-        } else if (longer >= active) {
-            ++run;
-            longer -= active;
-        }
-    }
     const int64_t keys = (int64_t)pos + (APPEND ? 0 : 1);  // positions that come from the cache
     const bool last = split == active - 1;
     // A split's records are a run of consecutive ones (runs differ by one at most), its wavefronts take them in turn.
@@ -135,7 +121,7 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
     const char* from = head + (int64_t)(first_tile + wave) * kKv8Record;
     const int count = wave < mine ? (mine - wave + NW - 1) / NW : 0;
     auto fetch = [&](int i) __attribute__((always_inline)) {
-        return load_record(from + (i < count ? (int64_t)i * (NW * kKv8Record) : 0), i < count, (uint32_t)lane);
+        return load_record<kChunks>(from + (i < count ? (int64_t)i * (NW * kKv8Record) : 0), i < count, (uint32_t)lane, slice);
     };
 
     // The query heads: step s of the first product has channels 64 (s/2) + 16 g + 8 (s%2) .. + 7 in lane group g. (Columns behind the group repeat its
@@ -150,7 +136,7 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
     auto ask_tables = [&]() __attribute__((always_inline)) { load_tables32(row, a.sin_cache + (int64_t)pos * 64, a.cos_cache + (int64_t)pos * 64, p32); };
     if constexpr (APPEND) ask_tables();
     asm volatile("" ::: "memory");
-    Record r = fetch(0);
+    Record<kChunks> r = fetch(0);
     if constexpr (APPEND) {
         auto finish_row = [&](int at) __attribute__((always_inline)) {
             const bool is_new = at >= a.group, is_v = at > a.group;
@@ -161,42 +147,43 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
                 hi = row.x[1];
             }
             if (!is_new) {
-                reinterpret_cast<uint32_t*>(rows[at])[p32] = lo;
-                reinterpret_cast<uint32_t*>(rows[at])[p32 + 32] = hi;
+                reinterpret_cast<uint32_t*>(sm.rows[at])[p32] = lo;
+                reinterpret_cast<uint32_t*>(sm.rows[at])[p32 + 32] = hi;
             } else if (last) {
                 float s;
                 const uint32_t codes = quantise_row32<FORMAT>(lo, hi, s);
-                file_row32(const_cast<char*>(head) + (int64_t)(pos >> 5) * kKv8Record, pos & 31, is_v, p32, codes, s);
-                reinterpret_cast<uint16_t*>(new_codes[is_v])[p32] = (uint16_t)codes;
-                reinterpret_cast<uint16_t*>(new_codes[is_v])[p32 + 32] = (uint16_t)(codes >> 16);
-                if (p32 == 0) new_scale[is_v] = s;
+                if (slice == 0) file_row32(const_cast<char*>(head) + (int64_t)(pos >> 5) * kKv8Record, pos & 31, is_v, p32, codes, s);
+                reinterpret_cast<uint16_t*>(sm.new_codes[is_v])[p32] = (uint16_t)codes;
+                reinterpret_cast<uint16_t*>(sm.new_codes[is_v])[p32 + 32] = (uint16_t)(codes >> 16);
+                if (p32 == 0) sm.new_scale[is_v] = s;
             }
         };
         if (half < work_rows) finish_row(half);
         // (apart from the first one: a loop's wait would be for its newest loads, the record's too)
         for (int at = half + 2 * NW; at < work_rows; at += 2 * NW) {
-            ask_row(at);
+            ask_row(a, row, kvh, at, p32);
             ask_tables();
             finish_row(at);
         }
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (the records stay on their way)
 #pragma unroll
-        for (int s = 0; s < 4; ++s) q[s] = *reinterpret_cast<const u32x4*>(rows[hq] + 64 * (s >> 1) + 16 * g + 8 * (s & 1));
+        for (int s = 0; s < 4; ++s) q[s] = *reinterpret_cast<const u32x4*>(sm.rows[hq] + 64 * (s >> 1) + 16 * g + 8 * (s & 1));
     }
     float m_run = -FLT_MAX, l_run = 0.0f;  // (a finite maximum: scores of -inf get weight 0, not NaN)
-    f32x4 o[8];
+    constexpr int kAccs = 2 * kChunks;  // b: columns 16 b .. + 15 of the workgroup's
+    f32x4 o[kAccs];
 #pragma unroll
-    for (int b = 0; b < 8; ++b) o[b] = f32x4{};
+    for (int b = 0; b < kAccs; ++b) o[b] = f32x4{};
 
     if constexpr (APPEND) {
         // The new token, as its codes stand for it, with weight 1: the wavefront that has the fewest records starts from it.
         if (last && wave == NW - 1) {
-            const float ks = new_scale[0], vs = new_scale[1];
+            const float ks = sm.new_scale[0], vs = sm.new_scale[1];
             f32x4 c{};
             // (all sixteen positions of the product are the new one)
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-                const u32x2 w = *reinterpret_cast<const u32x2*>(new_codes[0] + 64 * (s >> 1) + 16 * g + 8 * (s & 1));
+                const u32x2 w = *reinterpret_cast<const u32x2*>(sm.new_codes[0] + 64 * (s >> 1) + 16 * g + 8 * (s & 1));
                 c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kv8_operand<FORMAT>(w[0], w[1]), __builtin_bit_cast(bf16x8, q[s]), c, 0, 0, 0);
             }
             const float s = c[0] * (ks * a.scale_log2e);
@@ -204,8 +191,8 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
             const float w = fast_exp2(s - m_run);
             l_run = g == 0 ? w : 0.0f;
 #pragma unroll
-            for (int b = 0; b < 8; ++b) {
-                const uint32_t v = *reinterpret_cast<const uint32_t*>(new_codes[1] + 16 * b + 4 * g);
+            for (int b = 0; b < kAccs; ++b) {
+                const uint32_t v = *reinterpret_cast<const uint32_t*>(sm.new_codes[1] + 32 * slice + 16 * b + 4 * g);
                 const uint32_t v0 = kv8_pair<FORMAT, false>(v), v1 = kv8_pair<FORMAT, true>(v);
                 const float ws = w * vs;
                 o[b] = f32x4{bf16_lo(v0) * ws, bf16_hi(v0) * ws, bf16_lo(v1) * ws, bf16_hi(v1) * ws};
@@ -246,7 +233,7 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
                 const int bytes = min(max(left - 16 * u, 0), 4);
                 const uint32_t mask = bytes == 4 ? ~0u : (1u << (8 * bytes)) - 1u;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < kChunks; ++i) {
                     r.v[i][u] &= mask;
                     r.v[i][2 + u] &= mask;
                 }
@@ -264,7 +251,7 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
             if (__any(l_run != 0.0f)) {
                 l_run *= alpha;
 #pragma unroll
-                for (int b = 0; b < 8; ++b)
+                for (int b = 0; b < kAccs; ++b)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[b][e] *= alpha;
             }
@@ -280,7 +267,7 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
             pl[e] = pack_bf16(x0 - bf16_lo(w), x1 - bf16_hi(w));
         }
 #pragma unroll
-        for (int b = 0; b < 8; ++b) {
+        for (int b = 0; b < kAccs; ++b) {
             const bf16x8 x = kv8_operand<FORMAT>(r.v[b >> 1][2 * (b & 1)], r.v[b >> 1][2 * (b & 1) + 1]);
             o[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(bf16x8, ph), o[b], 0, 0, 0);
             o[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(bf16x8, pl), o[b], 0, 0, 0);
@@ -295,7 +282,7 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
     l_run = rows_sum(l_run);
     if (n < a.group) {
 #pragma unroll
-        for (int b = 0; b < 8; ++b) *reinterpret_cast<f32x4*>(&parts[wave][n][16 * b + 4 * g]) = o[b];
+        for (int b = 0; b < kAccs; ++b) *reinterpret_cast<f32x4*>(&parts[wave][n][16 * b + 4 * g]) = o[b];
         if (g == 0) {
             part_m[n][wave] = m_run;
             part_l[n][wave] = l_run;
@@ -306,6 +293,7 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
     const int64_t part_bytes = (int64_t)a.n_q * S * kHeadDim * (int64_t)sizeof(float);
     const __amdgpu_buffer_rsrc_t part_rsrc = __builtin_amdgcn_make_buffer_rsrc(a.ws, 0, (int)part_bytes, 0x00020000);
     auto write_out = [&](int hq, int c4, f32x4 x) __attribute__((always_inline)) {
+        c4 += 8 * slice;
         *reinterpret_cast<u32x2*>(a.out + (int64_t)hq * kHeadDim + 4 * c4) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
         if (a.out_f32) {
 #pragma unroll
@@ -316,13 +304,13 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
     // that the parts are read back by several compute units.
     const bool spread = active >= a.spread_min && active >= a.group;
     const int my_head = spread && active - 1 - split < a.group ? active - 1 - split : -1;
-    constexpr int kUnits = kHeads * 32 / (NW * 64);
+    constexpr int kPerHead = kColumns / 4, kUnits = (kHeads * kPerHead + NW * 64 - 1) / (NW * 64);
     float unit_m[kUnits], unit_l[kUnits];
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) {
         const int u = (int)threadIdx.x + i * NW * 64;
-        if (u >= a.group * 32) break;
-        const int h = u >> 5, c4 = u & 31, hq = kvh * a.group + h;
+        if (u >= a.group * kPerHead) break;
+        const int h = u / kPerHead, c4 = u % kPerHead, hq = kvh * a.group + h;
         float m = part_m[h][0];
 #pragma unroll
         for (int w = 1; w < NW; ++w) m = fmaxf(m, part_m[h][w]);
@@ -338,14 +326,14 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
         }
         unit_m[i] = m;
         unit_l[i] = sum;
-        if (active == 1) {
+        if (SLICED || active == 1) {
             const float r = 1.0f / sum;
             write_out(hq, c4, f32x4{x[0] * r, x[1] * r, x[2] * r, x[3] * r});
         } else {
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), part_rsrc, (uint32_t)(((hq * S + split) * kHeadDim + 4 * c4) * 4), 0, kCacheDevice);
         }
     }
-    if (active == 1) return;
+    if (SLICED || active == 1) return;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (a head's 32 columns are half a wavefront's: no barrier)
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) {
@@ -354,8 +342,8 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
         const int h = u >> 5;
         if ((u & 31) != 0) continue;
         if (spread ? h == my_head : last) {
-            fin[h][0] = unit_m[i];
-            fin[h][1] = unit_l[i];
+            sm.fin[h][0] = unit_m[i];
+            sm.fin[h][1] = unit_l[i];
         } else {
             unsigned long long* to = a.arrivals + ((int64_t)(kvh * a.group + h) * S + split) * 2;
             const unsigned long long tag = a.tag;
@@ -382,8 +370,8 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
         float m = -FLT_MAX, l = 0.0f;
         const bool mine_is = lane < n && s0 + lane == split, polls = lane < n && !mine_is;
         if (mine_is) {
-            m = fin[h][0];
-            l = fin[h][1];
+            m = sm.fin[h][0];
+            l = sm.fin[h][1];
         }
         y.in = false;
         for (int spin = 0; spin < a.max_polls && !y.in; ++spin) {
@@ -411,14 +399,14 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
         }
         y.m = wave_max(m);
         const float f = lane < n ? fast_exp2(m - y.m) : 0.0f;
-        weights[wave][lane & 1][lane >> 1] = f;  // (a half wavefront's side by side)
+        sm.weights[wave][lane & 1][lane >> 1] = f;  // (a half wavefront's side by side)
         y.sum = wave_sum(f * l);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_wave_barrier();
         f32x4 w[kBatch / 4];
         auto weigh = [&](int j0) __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 0; j < kBatch / 4; ++j) w[j] = *reinterpret_cast<const f32x4*>(&weights[wave][part][j0 + 4 * j]);
+            for (int j = 0; j < kBatch / 4; ++j) w[j] = *reinterpret_cast<const f32x4*>(&sm.weights[wave][part][j0 + 4 * j]);
         };
         auto add = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -460,7 +448,7 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
         if (lane == 0) {
             part_m[0][wave] = y.m;
             part_l[0][wave] = y.sum;
-            arrived[wave] = y.in;
+            sm.arrived[wave] = y.in;
         }
         __syncthreads();
         if (threadIdx.x < 32) {
@@ -477,7 +465,7 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
             }
             bool in = true;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) in = in && arrived[w];
+            for (int w = 0; w < NW; ++w) in = in && sm.arrived[w];
             if (!in && lane == 0) atomicAdd(&g_poll_timeouts, 1u);
             const float r = in ? 1.0f / sum : __builtin_bit_cast(float, 0x7fc00000u);
             write_out(kvh * a.group + h, c4, f32x4{x[0] * r, x[1] * r, x[2] * r, x[3] * r});
@@ -486,10 +474,56 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
     }
 }
 
+enum class Kv8Kind { split, sliced, device };  // device: which of them the position read at run time decides
+
+template <int FORMAT, int NW, bool APPEND, Kv8Kind KIND>
+__global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
+    __shared__ Kv8Shared<NW, KIND == Kv8Kind::sliced ? 32 : kHeadDim> sm;
+    // The new token's rows, half a wavefront each: the query heads, and (the last split files them) K and V behind them. What does not depend on the
+    // position is asked for in front of it, everything else in front of the records. (Half wavefronts without a row take the last one again: a branch around
+    // the loads would make their wait one for all of the records' too.)
+    NewRow row;
+    if constexpr (APPEND) ask_row(a, row, blockIdx.x, min((int)(threadIdx.x >> 5), a.group + 1), threadIdx.x & 31);
+    int pos = a.pos, active = a.splits, run = a.run, longer = a.longer;
+    if constexpr (KIND == Kv8Kind::device) {
+        // (constant address space: a scalar load; nothing in the launch writes the position)
+        const auto word = reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(a.pos_dev));
+        pos = max(0, min(*word, a.pos));
+        const int tiles = (int)(((int64_t)pos + (APPEND ? 0 : 1) + 31) >> 5), split = (int)blockIdx.y;
+        if (tiles <= a.sliced) {
+            if (split < kKv8Slices) kv8_attend<FORMAT, NW, APPEND, true>(a, sm, row, pos, 1, tiles, 0);
+            return;
+        }
+        active = kv8_active_splits(tiles, a.splits);
+        if (split >= active) return;
+        // (a quotient in two steps of 24 bits, then one up or down: shorter than the compiler's division, and on the way to the first load)
+        const float inverse = 1.0f / (float)active;
+        run = (int)((float)tiles * inverse);
+        run += (int)((float)(tiles - run * active) * inverse);
+        longer = tiles - run * active;
+        if (longer < 0) {
+            --run;
+            longer += active;
+        } else if (longer >= active) {
+            ++run;
+            longer -= active;
+        }
+    }
+    kv8_attend<FORMAT, NW, APPEND, KIND == Kv8Kind::sliced>(a, sm, row, pos, active, run, longer);
+}
+
+template <int FORMAT, bool APPEND, Kv8Kind KIND>
+void launch(const Kv8Args& a, int n_kv, const Kv8Form& form, hipStream_t stream) {
+    const dim3 grid(n_kv, KIND == Kv8Kind::sliced ? kKv8Slices : KIND == Kv8Kind::device && a.sliced > 0 && a.splits < kKv8Slices ? kKv8Slices : a.splits);
+    if (form.waves == 8) hipLaunchKernelGGL((mha_kv8_kernel<FORMAT, 8, APPEND, KIND>), grid, dim3(8 * 64), 0, stream, a);
+    else hipLaunchKernelGGL((mha_kv8_kernel<FORMAT, 4, APPEND, KIND>), grid, dim3(4 * 64), 0, stream, a);
+}
+
 template <int FORMAT, bool APPEND>
-void launch(const Kv8Args& a, int n_kv, int waves, hipStream_t stream) {
-    if (waves == 8) hipLaunchKernelGGL((mha_kv8_kernel<FORMAT, 8, APPEND>), dim3(n_kv, a.splits), dim3(8 * 64), 0, stream, a);
-    else hipLaunchKernelGGL((mha_kv8_kernel<FORMAT, 4, APPEND>), dim3(n_kv, a.splits), dim3(4 * 64), 0, stream, a);
+void launch(const Kv8Args& a, int n_kv, const Kv8Form& form, hipStream_t stream) {
+    if (a.pos_dev) launch<FORMAT, APPEND, Kv8Kind::device>(a, n_kv, form, stream);
+    else if (form.sliced > 0) launch<FORMAT, APPEND, Kv8Kind::sliced>(a, n_kv, form, stream);
+    else launch<FORMAT, APPEND, Kv8Kind::split>(a, n_kv, form, stream);
 }
 
 }  // namespace
@@ -514,6 +548,7 @@ int launch_mha_kv8(const llmi_mha_kv8_args& m, const llmi_mha_kv8_append_args* a
     a.run = tiles / form.splits;
     a.longer = tiles % form.splits;
     a.spread_min = form.spread_min;
+    a.sliced = form.sliced;
     a.scale_log2e = 1.4426950408889634f / sqrtf((float)kHeadDim);
     if (form.splits > 1) {
         a.ws = static_cast<float*>(m.workspace);
@@ -530,8 +565,8 @@ int launch_mha_kv8(const llmi_mha_kv8_args& m, const llmi_mha_kv8_append_args* a
     }
     const hipStream_t stream = static_cast<hipStream_t>(m.stream);
     const bool e4m3 = m.format == LLMI_KV8_E4M3;
-    if (append) e4m3 ? launch<LLMI_KV8_E4M3, true>(a, n_kv, form.waves, stream) : launch<LLMI_KV8_INT8, true>(a, n_kv, form.waves, stream);
-    else e4m3 ? launch<LLMI_KV8_E4M3, false>(a, n_kv, form.waves, stream) : launch<LLMI_KV8_INT8, false>(a, n_kv, form.waves, stream);
+    if (append) e4m3 ? launch<LLMI_KV8_E4M3, true>(a, n_kv, form, stream) : launch<LLMI_KV8_INT8, true>(a, n_kv, form, stream);
+    else e4m3 ? launch<LLMI_KV8_E4M3, false>(a, n_kv, form, stream) : launch<LLMI_KV8_INT8, false>(a, n_kv, form, stream);
     return check_launch();
 }
 
