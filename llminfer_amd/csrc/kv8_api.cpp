@@ -26,6 +26,13 @@ int validate_dims(int32_t head_dim, int32_t kv_dim, int32_t max_seq_len, int32_t
     return LLMI_OK;
 }
 
+// The output is written while other workgroups may still read the inputs.
+bool apart(const llmi_mha_kv8_args* a, const void* input, size_t bytes) {
+    const uintptr_t from = reinterpret_cast<uintptr_t>(input), out = reinterpret_cast<uintptr_t>(a->output), tap = reinterpret_cast<uintptr_t>(a->output_f32);
+    const size_t n = (size_t)a->head_num * 256;
+    return (from + bytes <= out || out + n <= from) && (!tap || from + bytes <= tap || tap + 2 * n <= from);
+}
+
 int validate(const llmi_mha_kv8_args* a) {
     if (!a) return LLMI_ERR_NULL_POINTER;
     if (!a->query || !a->cache8 || !a->output) return LLMI_ERR_NULL_POINTER;
@@ -36,6 +43,7 @@ int validate(const llmi_mha_kv8_args* a) {
     if (!aligned(a->query, 16) || !aligned(a->cache8, 16) || !aligned(a->output, 16) || !aligned(a->workspace, 16) || !aligned(a->output_f32, 4) ||
         !aligned(a->pos_device, 4))
         return LLMI_ERR_ALIGNMENT;
+    if (!apart(a, a->query, (size_t)a->head_num * 256)) return LLMI_ERR_INVALID_ARG;
     return LLMI_OK;
 }
 
@@ -175,6 +183,7 @@ int llmi_hip_mha_decode_append_kv8(const llmi_mha_kv8_append_args* a) {
     if (!aligned(a->key_new, 16) || !aligned(a->value_new, 16) || !aligned(a->norm_weight, 16) || !aligned(a->sin_cache, 16) || !aligned(a->cos_cache, 16))
         return LLMI_ERR_ALIGNMENT;
     if (!(a->eps >= 0.0f)) return LLMI_ERR_INVALID_ARG;
+    if (!apart(&a->mha, a->key_new, (size_t)a->mha.kv_dim * 2) || !apart(&a->mha, a->value_new, (size_t)a->mha.kv_dim * 2)) return LLMI_ERR_INVALID_ARG;
     return launch_mha_kv8(a->mha, a, form);
 }
 

@@ -46,7 +46,7 @@ def test_sizes(layers, msl, kv_dim, head_dim, want):
 
 def mha(**over):
     a = B.MhaKv8Args()
-    a.query = a.cache8 = a.output = 0x1000
+    a.query, a.cache8, a.output = 0x10000, 0x1000, 1 << 40
     a.workspace, a.workspace_bytes = 0x2000, 512 << 20
     a.layer_id, a.pos, a.kv_dim, a.kv_mul, a.head_num, a.head_dim, a.max_seq_len = 0, 4000, 1024, 4, 32, 128, 4096
     for k, v in over.items():
@@ -61,12 +61,14 @@ def plan(a):
 
 MHA_REFUSED = [
     (dict(pos=4096), "POS_RANGE"), (dict(pos=-1), "POS_RANGE"), (dict(query=0), "NULL_POINTER"), (dict(cache8=0), "NULL_POINTER"), (dict(output=0), "NULL_POINTER"),
-    (dict(query=0x1008), "ALIGNMENT"), (dict(cache8=0x1008), "ALIGNMENT"), (dict(output=0x1004), "ALIGNMENT"), (dict(workspace=0x2008), "ALIGNMENT"),
+    (dict(query=0x10008), "ALIGNMENT"), (dict(cache8=0x1008), "ALIGNMENT"), (dict(output=0x20004), "ALIGNMENT"), (dict(workspace=0x2008), "ALIGNMENT"),
     (dict(output_f32=0x1002), "ALIGNMENT"), (dict(pos_device=0x1002), "ALIGNMENT"), (dict(head_dim=64), "HEAD_DIM"), (dict(kv_dim=1000), "KV_DIM"),
     (dict(kv_dim=0), "KV_DIM"), (dict(kv_dim=-128), "KV_DIM"), (dict(head_num=31), "HEAD_GROUP"), (dict(kv_mul=17, head_num=136), "HEAD_GROUP"), (dict(kv_mul=0, head_num=0), "HEAD_GROUP"),
     (dict(num_splits=257), "INVALID_ARG"), (dict(num_splits=-1), "INVALID_ARG"), (dict(max_seq_len=0), "INVALID_ARG"), (dict(layer_id=-1), "INVALID_ARG"),
     (dict(format=2), "INVALID_ARG"), (dict(format=-1), "INVALID_ARG"), (dict(kv_dim=128 * 65536, kv_mul=1, head_num=65536), "INVALID_ARG"),
     (dict(num_splits=16, workspace_bytes=16 * 32 * 528 + 15), "WORKSPACE"), (dict(num_splits=2, workspace=0), "WORKSPACE"),
+    (dict(output=0x10000), "INVALID_ARG"), (dict(output=0x10000 + 32 * 256 - 16), "INVALID_ARG"), (dict(output=0x10000 - 16), "INVALID_ARG"),
+    (dict(output_f32=0x10000 - 4), "INVALID_ARG"), (dict(output_f32=0x10000 + 32 * 256 - 4), "INVALID_ARG"),
 ]
 
 
@@ -82,7 +84,7 @@ def test_attention_status_codes(over, status):
 @pytest.mark.parametrize("over,status", [
     (dict(key_new=0), "NULL_POINTER"), (dict(value_new=0), "NULL_POINTER"), (dict(norm_weight=0), "NULL_POINTER"), (dict(sin_cache=0), "NULL_POINTER"),
     (dict(cos_cache=0), "NULL_POINTER"), (dict(key_new=0x1008), "ALIGNMENT"), (dict(cos_cache=0x1004), "ALIGNMENT"), (dict(eps=-1.0), "INVALID_ARG"),
-    (dict(eps=float("nan")), "INVALID_ARG"),
+    (dict(eps=float("nan")), "INVALID_ARG"), (dict(key_new=1 << 40), "INVALID_ARG"), (dict(value_new=(1 << 40) + 32 * 256 - 16), "INVALID_ARG"),
 ])
 def test_append_status_codes(over, status):
     t = B.MhaKv8AppendArgs(mha=mha(), key_new=0x1000, value_new=0x1000, norm_weight=0x1000, sin_cache=0x1000, cos_cache=0x1000, eps=1e-6)
@@ -123,6 +125,13 @@ def test_copy_status_codes(over, status):
         setattr(a, k, v)
     assert B.lib().llmi_hip_kv8_store(ctypes.byref(a)) == B.STATUS[status]
     assert B.lib().llmi_hip_kv8_load(ctypes.byref(a)) == B.STATUS[status]
+
+
+def test_neighbours_do_not_overlap():
+    """Output right behind or in front of an input (the plan makes no HIP call)."""
+    for out in (0x10000 + 32 * 256, 0x10000 - 32 * 256):
+        assert plan(mha(output=out))[0] == 0
+    assert plan(mha(output_f32=0x10000 - 32 * 512))[0] == 0
 
 
 def test_null_arguments():
