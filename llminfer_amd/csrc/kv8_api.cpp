@@ -92,6 +92,9 @@ int make_form(const llmi_mha_kv8_args* a, int new_rows, Kv8Form* form) {
             form->waves = tiles > 4 ? 8 : 4;
         }
     }
+    // (the new token's query heads, half a wavefront each, all but one wavefront's: six in one pass with four. us with 4 : 8, 64 Q heads: 3.70 : 3.46 at 127
+    // positions, 5.74 : 5.95 at 1024, 6.15 : 6.17 at 2000, 7.61 : 7.05 at 4099)
+    if (new_rows && a->kv_mul > 6 && (form->sliced || tiles >= 3 * (int64_t)form->splits)) form->waves = 8;
     form->spread_min = a->head_num <= kMostJoining ? 2 : INT32_MAX;
     return LLMI_OK;
 }

@@ -84,7 +84,8 @@ struct Kv8Shared {
     __attribute__((aligned(16))) float weights[NW][2][32];
     __attribute__((aligned(16))) uint16_t rows[kHeads][kHeadDim];  // the new token's query heads
     __attribute__((aligned(16))) uint8_t new_codes[2][kHeadDim];
-    float part_m[kHeads][NW], part_l[kHeads][NW], fin[kHeads][2], new_scale[2];
+    float part_m[kHeads][NW], part_l[kHeads][NW], fin[kHeads][2];
+    int rows_done;  // of the new token's query heads
     bool arrived[NW];
 };
 
@@ -95,6 +96,9 @@ __device__ __forceinline__ void ask_row(const Kv8Args& a, NewRow& row, int kvh, 
     const uint64_t q_row = reinterpret_cast<uint64_t>(a.q) + (uint64_t)(uint32_t)((kvh * a.group + at) * 256);
     load_row32(row, is_new ? new_row : q_row, reinterpret_cast<uint64_t>(a.norm_w) + (is_new ? 256u : 0u), p32);
 }
+
+// A lane's value, for all of them.
+__device__ __forceinline__ float row_scalar(float x, int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane)); }
 
 // SLICED: the workgroup has 32 of the 128 columns and every position, split is which (nothing to join). Otherwise all columns and its split's run. `row`: what does
 // not depend on the position of the half wavefront's first new row has been asked for.
@@ -110,7 +114,6 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args& a, Kv8Shared<NW, COLUM
     const int kvh = blockIdx.x, split = SLICED ? 0 : blockIdx.y, slice = SLICED ? blockIdx.y : 0;
     const int p32 = lane & 31;
     const int half = (int)(threadIdx.x >> 5);
-    const int work_rows = a.group + 2;
     const int64_t keys = (int64_t)pos + (APPEND ? 0 : 1);  // positions that come from the cache
     const bool last = split == active - 1;
     // A split's records are a run of consecutive ones (runs differ by one at most), its wavefronts take them in turn.
@@ -134,38 +137,40 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args& a, Kv8Shared<NW, COLUM
         for (int s = 0; s < 4; ++s) q[s] = *reinterpret_cast<const u32x4*>(src + 64 * (s >> 1) + 16 * g + 8 * (s & 1));
     }
     auto ask_tables = [&]() __attribute__((always_inline)) { load_tables32(row, a.sin_cache + (int64_t)pos * 64, a.cos_cache + (int64_t)pos * 64, p32); };
+    uint32_t new_lo = 0u, new_hi = 0u, codes = 0u;
+    float scale = 0.0f;
+    const bool takes_new = wave == NW - 1;
     if constexpr (APPEND) ask_tables();
     asm volatile("" ::: "memory");
     Record<kChunks> r = fetch(0);
     if constexpr (APPEND) {
-        auto finish_row = [&](int at) __attribute__((always_inline)) {
-            const bool is_new = at >= a.group, is_v = at > a.group;
-            uint32_t lo, hi;
-            norm_rope_regs32(row, p32, a.eps, lo, hi);
-            if (is_v) {
-                lo = row.x[0];
-                hi = row.x[1];
-            }
-            if (!is_new) {
-                reinterpret_cast<uint32_t*>(sm.rows[at])[p32] = lo;
-                reinterpret_cast<uint32_t*>(sm.rows[at])[p32 + 32] = hi;
-            } else if (last) {
-                float s;
-                const uint32_t codes = quantise_row32<FORMAT>(lo, hi, s);
-                if (slice == 0) file_row32(const_cast<char*>(head) + (int64_t)(pos >> 5) * kKv8Record, pos & 31, is_v, p32, codes, s);
-                reinterpret_cast<uint16_t*>(sm.new_codes[is_v])[p32] = (uint16_t)codes;
-                reinterpret_cast<uint16_t*>(sm.new_codes[is_v])[p32 + 32] = (uint16_t)(codes >> 16);
-                if (p32 == 0) sm.new_scale[is_v] = s;
-            }
+        auto put_row = [&](int at) __attribute__((always_inline)) {
+            reinterpret_cast<uint32_t*>(sm.rows[at])[p32] = new_lo;
+            reinterpret_cast<uint32_t*>(sm.rows[at])[p32 + 32] = new_hi;
+            // (a wavefront's LDS instructions are done in order)
+            asm volatile("" ::: "memory");
+            if (p32 == 0) __hip_atomic_fetch_add(&sm.rows_done, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
         };
-        if (half < work_rows) finish_row(half);
-        // (apart from the first one: a loop's wait would be for its newest loads, the record's too)
-        for (int at = half + 2 * NW; at < work_rows; at += 2 * NW) {
-            ask_row(a, row, kvh, at, p32);
-            ask_tables();
-            finish_row(at);
+        if (half < a.group || takes_new) norm_rope_regs32(row, p32, a.eps, new_lo, new_hi);
+        if (!takes_new) {
+            if (half < a.group) put_row(half);
+            // (apart from the first one: a loop's wait would be for its newest loads, the record's too)
+            for (int at = half + 2 * (NW - 1); at < a.group; at += 2 * (NW - 1)) {
+                ask_row(a, row, kvh, at, p32);
+                ask_tables();
+                norm_rope_regs32(row, p32, a.eps, new_lo, new_hi);
+                put_row(at);
+            }
+        } else if (last) {
+            const bool is_v = lane >= 32;
+            codes = quantise_row32<FORMAT>(is_v ? row.x[0] : new_lo, is_v ? row.x[1] : new_hi, scale);
+            reinterpret_cast<uint16_t*>(sm.new_codes[is_v])[p32] = (uint16_t)codes;
+            reinterpret_cast<uint16_t*>(sm.new_codes[is_v])[p32 + 32] = (uint16_t)(codes >> 16);
         }
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (the records stay on their way)
+        // The query heads are waited for by their number, not at a barrier: nobody waits for K and V but the wavefront that has them. (Those that finish
+        // rows wait for nothing.)
+        while (__builtin_amdgcn_readfirstlane(__hip_atomic_load(&sm.rows_done, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP)) < a.group) {}
+        asm volatile("" ::: "memory");
 #pragma unroll
         for (int s = 0; s < 4; ++s) q[s] = *reinterpret_cast<const u32x4*>(sm.rows[hq] + 64 * (s >> 1) + 16 * g + 8 * (s & 1));
     }
@@ -177,8 +182,8 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args& a, Kv8Shared<NW, COLUM
 
     if constexpr (APPEND) {
         // The new token, as its codes stand for it, with weight 1: the wavefront that has the fewest records starts from it.
-        if (last && wave == NW - 1) {
-            const float ks = sm.new_scale[0], vs = sm.new_scale[1];
+        if (last && takes_new) {
+            const float ks = row_scalar(scale, 0), vs = row_scalar(scale, 32);
             f32x4 c{};
             // (all sixteen positions of the product are the new one)
 #pragma unroll
@@ -289,6 +294,9 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args& a, Kv8Shared<NW, COLUM
         }
     }
     __syncthreads();
+    // (here, where nobody waits for this wavefront any more; ahead of the records their waits would be for these stores too)
+    if (APPEND && last && takes_new && slice == 0)
+        file_row32(const_cast<char*>(head) + (int64_t)(pos >> 5) * kKv8Record, pos & 31, lane >= 32, p32, codes, scale);
     const int S = a.splits;
     const int64_t part_bytes = (int64_t)a.n_q * S * kHeadDim * (int64_t)sizeof(float);
     const __amdgpu_buffer_rsrc_t part_rsrc = __builtin_amdgcn_make_buffer_rsrc(a.ws, 0, (int)part_bytes, 0x00020000);
@@ -479,11 +487,18 @@ enum class Kv8Kind { split, sliced, device };  // device: which of them the posi
 template <int FORMAT, int NW, bool APPEND, Kv8Kind KIND>
 __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
     __shared__ Kv8Shared<NW, KIND == Kv8Kind::sliced ? 32 : kHeadDim> sm;
-    // The new token's rows, half a wavefront each: the query heads, and (the last split files them) K and V behind them. What does not depend on the
-    // position is asked for in front of it, everything else in front of the records. (Half wavefronts without a row take the last one again: a branch around
-    // the loads would make their wait one for all of the records' too.)
+    // The new token's rows, half a wavefront each: the query heads, in the last wavefront K and V (which the last split files). What does not depend on the
+    // position is asked for in front of it, everything else in front of the records. (Half wavefronts without a row take a head again: a branch around
+    // the loads would make their wait one for all of the records' too.) Only the wavefront that has K and V waits for their quantisation; one barrier for all rows,
+    // K and V quantised by a third wavefront ahead of it : this, us: 3.32 : 3.17 at 57 positions (16 Q), 4.46 : 4.36 at 300, 5.00 : 5.13 at 511 (32 Q), 5.19 : 5.06 at
+    // 1024, 6.08 : 5.83 at 4095, 14.87 : 14.64 at 32768; position on the device 5.97 : 5.83 at 1000, 6.97 : 6.90 at 4099.
     NewRow row;
-    if constexpr (APPEND) ask_row(a, row, blockIdx.x, min((int)(threadIdx.x >> 5), a.group + 1), threadIdx.x & 31);
+    if constexpr (APPEND) {
+        const int half = (int)(threadIdx.x >> 5), behind = half - 2 * (NW - 1);
+        ask_row(a, row, blockIdx.x, behind >= 0 ? a.group + behind : min(half, a.group - 1), threadIdx.x & 31);
+        if (threadIdx.x == 0) sm.rows_done = 0;
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    }
     int pos = a.pos, active = a.splits, run = a.run, longer = a.longer;
     if constexpr (KIND == Kv8Kind::device) {
         // (constant address space: a scalar load; nothing in the launch writes the position)
