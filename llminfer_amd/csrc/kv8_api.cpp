@@ -55,7 +55,7 @@ constexpr int kMostJoining = 128;
 // there is nothing to join. us, splits by the rule below : so, 32 Q / 8 KV heads E4M3: 2.69 : 2.45 at 21 positions, 2.94 : 2.56 at 128, 4.16 : 3.39 at 256, 4.54 : 3.83
 // at 320, 4.66 : 4.25 at 401, 4.67 : 4.35 at 512, 4.66 : 4.64 at 601, 4.73 : 5.19 at 701; with the new token 3.89 : 3.36 at 57, 5.06 : 4.47 at 300 (16 Q), 5.51 : 4.98
 // at 511. Whole numbers, whose conversion takes three times the instructions: 4.97 : 4.18 at 320, 4.86 : 5.08 at 401. (Sixteen wavefronts beyond eight records
-// 0.2 - 0.5 slower.)
+// 0.2 - 0.65 slower.)
 constexpr int kMostSliced = 18, kMostSlicedWhole = 12;
 
 // The workgroups a KV head's records are dealt to beyond that: one up to ten records (kKv8Single), then a record each up to one workgroup per compute unit. us by

@@ -13,9 +13,17 @@
 // which enters the product as the sum of two bf16 numbers (2^-16 of it lost at most). Maximum, sum and accumulators are fp32; the accumulators are
 // rescaled only where a maximum has grown by more than 2^8.
 //
-// Records are dealt to the splits (workgroups of a KV head) and their wavefronts in turn. The workgroup of the last split joins the others inside the launch:
-// every split leaves its partial outputs and, once they are acknowledged, a record {tag | maximum} {tag | sum} per head in the workspace, past the
-// caches; the last one, which is dispatched behind the others, waits for those (bounded) and adds the parts up.
+// Two forms (rules and measurements: kv8_api.cpp):
+//   sliced  Short contexts: four workgroups a KV head, each with 32 of the columns and every position. K's codes are read (through the L2) and multiplied four
+//           times, V's once; nothing is handed from workgroup to workgroup, which costs a call 1.8 us otherwise (a record a wavefront: 2.9 in one workgroup, 4.7 joined).
+//   split   A KV head's records are dealt to up to 256 workgroups in contiguous runs, a workgroup's wavefronts take them in turn, one record of each on its way
+//           (more in flight on a compute unit come back later, not faster). Every split leaves its partial outputs and, once they are acknowledged, a
+//           record {tag | maximum} {tag | sum} per head in the workspace, past the caches; the last one (or the last ones, a head each), which are
+//           dispatched behind the others, wait for those (bounded) and add the parts up.
+// What bounds it: the launch and a trip to memory up to some hundred positions (32 Q / 8 KV heads, E4M3, captured: 2.5 us at 58, 4.4 at 512), the hand-over up to some
+// thousand (4.8 at 1024, 5.7 at 4096), then memory: 14.5 us at 32768 (68 MB), 42 - 44.5 by card at 131001 with 64 Q heads (272 MB, 6.2 TB/s with everything, 6.9 beyond
+// the 4.8). Over the bf16 cache the same calls took 7.0 at 4096, 23.6 and 82.4 beside them.
+// Whole-number codes take three instructions for two values where E4M3's take one, E4M3 : whole numbers 6.8 : 7.2 at 6008 positions, 44.1 : 44.6 at 131001.
 
 #include <hip/hip_runtime.h>
 #include <float.h>
@@ -60,7 +68,8 @@ struct Record {
     u32x4 k[4], v[CHUNKS], ks, vs;  // codes, the lane's eight scales
 };
 
-// (a record that there is not: zeros, and nothing read). Whole records are streamed, nobody reads one twice; where four workgroups read the same K codes they are not.
+// (a record that there is not: zeros, and nothing read). Whole records are streamed past the caches, nobody reads one twice: 14.45 us at 32768 positions, without the hint
+// 16.0; 44.6 : 48.7 at 131001. Where four workgroups read the same K codes they are not.
 template <int CHUNKS>
 __device__ __forceinline__ Record<CHUNKS> load_record(const char* at, bool there, uint32_t lane, int chunk) {
     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(at), 0, there ? kKv8Record : 0, 0x00020000);

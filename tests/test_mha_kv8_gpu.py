@@ -161,6 +161,33 @@ def test_position_on_the_device(dev, fmt):
         C.close(tap, *C.attention(q.cpu(), k[0, :, :keys], v[0, :, :keys]), rounded=out)
 
 
+@pytest.mark.parametrize("n_q,n_kv,msl,fmt", [(8, 1, 30000, C.E4M3), (22, 2, 9000, C.INT8), (48, 8, 2500, C.E4M3)])
+def test_one_captured_launch_at_every_length(dev, n_q, n_kv, msl, fmt):
+    """A launch captured for the window, replayed at positions all over it: one workgroup's share, slices, splits of every number; the workspace is not cleared between."""
+    g = torch.Generator().manual_seed(msl)
+    cache, k, v = C.filled(1, n_kv, msl, msl, fmt, n_q)
+    q, ws, cache = C.rows(g, n_q, outliers=False), workspace(dev, n_q, msl), cache.to(dev)
+    q_dev, word = q.to(dev), torch.zeros(1, dtype=torch.int32, device=dev)
+    out, tap = torch.zeros(n_q, D, dtype=BF16, device=dev), torch.zeros(n_q, D, device=dev)
+
+    def call():
+        ops.mha_decode_kv8(q_dev, cache, out, ws, output_f32=tap, layer_id=0, pos=msl - 1, pos_device=word, kv_dim=n_kv * D, kv_mul=n_q // n_kv, head_num=n_q, head_dim=D, max_seq_len=msl,
+                           kv8_format=fmt)
+
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    edges = [32 * t + x for t in (1, 4, 12, 13, 18, 19, 31, 32, 33, 96, 97) for x in (-1, 0)]
+    for pos in [p for p in edges if p < msl] + torch.randint(0, msl, (25,), generator=g).tolist() + [msl - 1]:
+        word.fill_(pos)
+        out.fill_(math.nan), tap.fill_(math.nan)
+        graph.replay()
+        torch.cuda.synchronize()
+        C.close(tap.cpu(), *C.attention(q, k[0, :, :pos + 1], v[0, :, :pos + 1]), rounded=out.cpu())
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_scores_far_apart(dev, fmt):
     """One position far above the others, anywhere; scales from the smallest to large ones; weights that underflow."""
