@@ -225,6 +225,51 @@ def test_rows_of_many_tokens(dev, pos, n, how, fmt):
     assert torch.equal(few.cpu(), cache) and torch.equal(q_few.cpu().view(n, n_q, D), out)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("n", [5, 400])
+def test_captured_on_a_side_stream(dev, n, fmt):
+    """A range stored, rows filed behind it at a position on the device, both read back: one graph, replayed with other inputs and positions, other work between."""
+    n_q, n_kv, msl = 6, 3, 900
+    g = torch.Generator().manual_seed(n)
+    dims = dict(kv_dim=n_kv * D, head_dim=D, max_seq_len=msl, kv8_format=fmt)
+    w = (1 + 0.1 * torch.randn(2 * D, generator=g)).to(BF16).to(dev)
+    sin, cos = (x.to(dev) for x in C.tables(msl))
+    kc, vc = (torch.zeros(2, msl, n_kv * D, dtype=BF16, device=dev) for _ in range(2))
+    packed, word = torch.zeros(n, (n_q + 2 * n_kv) * D, dtype=BF16, device=dev), torch.zeros(1, dtype=torch.int32, device=dev)
+
+    def buffers():
+        cache = torch.zeros(ops.kv8_bytes(2, msl, n_kv * D, D), dtype=torch.uint8, device=dev)
+        return cache, torch.zeros(n, n_q * D, dtype=BF16, device=dev), torch.zeros_like(kc), torch.zeros_like(vc)
+
+    def call(cache, q, k_back, v_back, bound, at):
+        rows = packed.split([n_q * D, n_kv * D, n_kv * D], dim=1)
+        ops.kv8_store(kc, vc, cache, layer_num=2, num_pos=77, **dims)
+        ops.qk_norm_rope_append_kv8(q, rows[1], rows[2], cache, w, sin, cos, row_num=n, layer_id=1, pos=bound, head_num=n_q, query_src=rows[0], pos_device=at, **dims)
+        ops.kv8_load(cache, k_back, v_back, layer_num=2, num_pos=msl, **dims)
+
+    mine = buffers()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        call(*mine, msl - n, word)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        call(*mine, msl - n, word)
+    for at in (77, 0, 31, 450, msl - n):
+        for x in (kc, vc, packed):
+            x.copy_(torch.randn(x.shape, generator=g).to(BF16))
+        word.fill_(at)
+        for x in mine:
+            x.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = buffers()
+        call(*want, at, None)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(mine, want)), at
+
+
 def test_what_the_front_end_refuses(dev):
     u8 = torch.zeros(2 * 8320, dtype=torch.uint8, device=dev)
     x = torch.zeros(64, D, dtype=BF16, device=dev)
