@@ -50,7 +50,7 @@ struct Kv8Args {
     uint32_t tag;
     int32_t pos, group, n_q, splits, max_polls;
     int32_t run, longer;          // records per split, and how many splits take one more (position known on the host)
-    int32_t sliced;               // position read on the device: records up to which a workgroup has 32 columns and all of them
+    int32_t sliced;               // position read on the device: records up to which a workgroup has 32 columns and all of them; 0: at no number
     int32_t spread_min;           // fewest splits at which a KV head's query heads are joined by different workgroups
     float scale_log2e;            // log2(e) / sqrt(128)
     // the new token's
@@ -514,7 +514,8 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
         const auto word = reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(a.pos_dev));
         pos = max(0, min(*word, a.pos));
         const int tiles = (int)(((int64_t)pos + (APPEND ? 0 : 1) + 31) >> 5), split = (int)blockIdx.y;
-        if (tiles <= a.sliced) {
+        // (a chosen number of splits: 0, and fewer workgroups than slices, perhaps; a step at position 0, with no record, is one split's then)
+        if (a.sliced > 0 && tiles <= a.sliced) {
             if (split < kKv8Slices) kv8_attend<FORMAT, NW, APPEND, true>(a, sm, row, pos, 1, tiles, 0);
             return;
         }
