@@ -26,11 +26,20 @@ int validate_dims(int32_t head_dim, int32_t kv_dim, int32_t max_seq_len, int32_t
     return LLMI_OK;
 }
 
-// The output is written while other workgroups may still read the inputs.
-bool apart(const llmi_mha_kv8_args* a, const void* input, size_t bytes) {
-    const uintptr_t from = reinterpret_cast<uintptr_t>(input), out = reinterpret_cast<uintptr_t>(a->output), tap = reinterpret_cast<uintptr_t>(a->output_f32);
-    const size_t n = (size_t)a->head_num * 256;
-    return (from + bytes <= out || out + n <= from) && (!tap || from + bytes <= tap || tap + 2 * n <= from);
+// Bytes of memory from an address on (none: nowhere), up to the end of the address space at most.
+struct Range {
+    uintptr_t from, to;
+};
+Range range(const void* p, size_t bytes) {
+    const uintptr_t from = reinterpret_cast<uintptr_t>(p);
+    return p ? Range{from, bytes > UINTPTR_MAX - from ? UINTPTR_MAX : from + bytes} : Range{0, 0};
+}
+bool apart(Range a, Range b) { return a.to <= b.from || b.to <= a.from; }
+
+// The 8-bit cache up to and with a layer (later layers' place is not known to be the cache's). No memory is as large as one whose size passes 64 bits.
+Range cache_range(const void* cache8, int32_t layers, int32_t max_seq_len, int32_t kv_dim) {
+    const size_t n = llmi_hip_kv8_bytes(layers, max_seq_len, kv_dim, 128);
+    return range(cache8, n ? n : SIZE_MAX);
 }
 
 int validate(const llmi_mha_kv8_args* a) {
@@ -43,7 +52,8 @@ int validate(const llmi_mha_kv8_args* a) {
     if (!aligned(a->query, 16) || !aligned(a->cache8, 16) || !aligned(a->output, 16) || !aligned(a->workspace, 16) || !aligned(a->output_f32, 4) ||
         !aligned(a->pos_device, 4))
         return LLMI_ERR_ALIGNMENT;
-    if (!apart(a, a->query, (size_t)a->head_num * 256)) return LLMI_ERR_INVALID_ARG;
+    const Range query = range(a->query, (size_t)a->head_num * 256);
+    if (!apart(query, range(a->output, (size_t)a->head_num * 256)) || !apart(query, range(a->output_f32, (size_t)a->head_num * 512))) return LLMI_ERR_INVALID_ARG;
     return LLMI_OK;
 }
 
@@ -97,6 +107,29 @@ int make_form(const llmi_mha_kv8_args* a, int new_rows, Kv8Form* form) {
     if (new_rows && a->kv_mul > 6 && (form->sliced || tiles >= 3 * (int64_t)form->splits)) form->waves = 8;
     form->spread_min = a->head_num <= kMostJoining ? 2 : INT32_MAX;
     return LLMI_OK;
+}
+
+// Whether what a call writes is apart from what it reads, and each thing written from the others: workgroups write while others still read.
+bool writes_apart(const llmi_mha_kv8_args* a, const llmi_mha_kv8_append_args* append, int splits) {
+    if (a->layer_id == INT32_MAX) return false;
+    const size_t heads = (size_t)a->head_num * 256, new_row = (size_t)a->kv_dim * 2, table = ((size_t)a->pos + 1) * 256;
+    const Range none{0, 0}, cache = cache_range(a->cache8, a->layer_id + 1, a->max_seq_len, a->kv_dim);
+    const Range writes[] = {range(a->output, heads), range(a->output_f32, 2 * heads), splits > 1 ? range(a->workspace, split_bytes(a) * (size_t)splits) : none, append ? cache : none};
+    const Range reads[] = {range(a->query, heads),
+                           range(a->pos_device, 4),
+                           append ? none : cache,
+                           append ? range(append->key_new, new_row) : none,
+                           append ? range(append->value_new, new_row) : none,
+                           append ? range(append->norm_weight, 512) : none,
+                           append ? range(append->sin_cache, table) : none,
+                           append ? range(append->cos_cache, table) : none};
+    for (const Range& w : writes) {
+        for (const Range& r : reads)
+            if (!apart(w, r)) return false;
+        for (const Range* x = writes; x != &w; ++x)
+            if (!apart(w, *x)) return false;
+    }
+    return true;
 }
 
 int validate_copy(const llmi_kv8_copy_args* a) {
@@ -175,6 +208,7 @@ int llmi_hip_mha_kv8_plan(const llmi_mha_kv8_args* args, llmi_mha_plan* plan) {
 int llmi_hip_mha_decode_kv8(const llmi_mha_kv8_args* args) {
     Kv8Form form;
     if (int rc = make_form(args, 0, &form)) return rc;
+    if (!writes_apart(args, nullptr, form.splits)) return LLMI_ERR_INVALID_ARG;
     return launch_mha_kv8(*args, nullptr, form);
 }
 
@@ -186,7 +220,7 @@ int llmi_hip_mha_decode_append_kv8(const llmi_mha_kv8_append_args* a) {
     if (!aligned(a->key_new, 16) || !aligned(a->value_new, 16) || !aligned(a->norm_weight, 16) || !aligned(a->sin_cache, 16) || !aligned(a->cos_cache, 16))
         return LLMI_ERR_ALIGNMENT;
     if (!(a->eps >= 0.0f)) return LLMI_ERR_INVALID_ARG;
-    if (!apart(&a->mha, a->key_new, (size_t)a->mha.kv_dim * 2) || !apart(&a->mha, a->value_new, (size_t)a->mha.kv_dim * 2)) return LLMI_ERR_INVALID_ARG;
+    if (!writes_apart(&a->mha, a, form.splits)) return LLMI_ERR_INVALID_ARG;
     return launch_mha_kv8(a->mha, a, form);
 }
 

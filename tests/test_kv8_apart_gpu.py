@@ -1,0 +1,68 @@
+"""Buffers that lie side by side, cut out of one: the calls for an 8-bit KV cache take them, and write nothing beside what is theirs."""
+import pytest
+import torch
+
+from llminfer_amd import ops
+
+import kv8_cases as C
+
+pytestmark = pytest.mark.gpu
+D, BF16 = C.D, C.BF16
+
+
+class Slab:
+    """One allocation, handed out piece by piece with nothing between."""
+
+    def __init__(self, dev, size):
+        self.bytes, self.used = torch.full((size,), 0x5A, dtype=torch.uint8, device=dev), 0
+
+    def take(self, shape, dtype, like=None):
+        n = torch.Size(shape).numel() * torch.empty(0, dtype=dtype).element_size()
+        assert n % 16 == 0 and self.used + n <= self.bytes.numel()
+        x = self.bytes[self.used:self.used + n].view(dtype).view(shape)
+        self.used += n
+        return x if like is None else x.copy_(like)
+
+    def check(self):
+        assert bool((self.bytes[self.used:] == 0x5A).all())
+
+
+@pytest.mark.parametrize("keys", [70, 3000])
+@pytest.mark.parametrize("order", [1, -1])
+def test_attention(dev, keys, order):
+    n_q, n_kv, msl, splits = 8, 2, keys + 30, 5 if keys > 2000 else 0
+    g = torch.Generator().manual_seed(keys)
+    cache, k, v = C.filled(2, n_kv, msl, keys, C.E4M3, keys)
+    q = C.rows(g, n_q, outliers=False)
+    new = torch.randn((n_q + 2 * n_kv) * D, generator=g).to(BF16)
+    w = (1 + 0.1 * torch.randn(2 * D, generator=g)).to(BF16)
+    sin, cos = C.tables(msl)
+    slab = Slab(dev, cache.numel() + n_q * 528 * max(splits, 1) + 4 * msl * D + (1 << 16))
+    made = {}
+    pieces = [("out", (n_q, D), BF16, None), ("q", (n_q, D), BF16, q), ("tap", (n_q, D), torch.float32, None), ("ws", (n_q * 132 * max(splits, 1),), torch.float32, None),
+              ("cache", cache.shape, torch.uint8, cache), ("new", new.shape, BF16, new), ("word", (4,), torch.int32, torch.tensor([keys - 1, 0, 0, 0], dtype=torch.int32)),
+              ("out2", (n_q, D), BF16, None), ("w", w.shape, BF16, w), ("sin", sin.shape, torch.float32, sin), ("cos", cos.shape, torch.float32, cos), ("pad", (4,), torch.float32, None)]
+    for name, shape, dtype, like in pieces[::order]:
+        made[name] = slab.take(shape, dtype, like)
+    # (a workspace has 16 bytes more than its partial results take: here they are its neighbour's)
+    ws = torch.as_strided(made["ws"], (made["ws"].numel() + 4,), (1,)) if splits else None
+    dims = dict(layer_id=1, kv_dim=n_kv * D, kv_mul=n_q // n_kv, head_num=n_q, head_dim=D, max_seq_len=msl, num_splits=splits)
+    want = C.attention(q, k[1], v[1])
+    for at in (dict(pos=keys - 1), dict(pos=msl - 1, pos_device=made["word"][:1])):
+        made["out"].zero_(), made["tap"].zero_()
+        ops.mha_decode_kv8(made["q"], made["cache"], made["out"], ws, output_f32=made["tap"], **at, **dims)
+        C.close(made["tap"].cpu(), *want, rounded=made["out"].cpu())
+    made["word"].fill_(keys)
+    parts = made["new"].split([n_q * D, n_kv * D, n_kv * D])
+    alone = [x.clone() for x in (*parts, made["w"], made["sin"], made["cos"], made["cache"])]
+    out, enough = torch.zeros(n_q, D, dtype=BF16, device=dev), torch.zeros(1 << 18, device=dev)
+    ops.mha_decode_append_kv8(*alone, out, enough, pos=keys, **dims)
+    for at in (dict(pos=keys), dict(pos=msl - 1, pos_device=made["word"][:1])):
+        made["out2"].zero_()
+        ops.mha_decode_append_kv8(*parts, made["w"], made["sin"], made["cos"], made["cache"], made["out2"], ws, **at, **dims)
+        assert torch.equal(made["cache"], alone[-1])
+        if "pos_device" not in at:
+            assert torch.equal(made["out2"], out)
+    assert torch.equal(made["q"].cpu(), q) and torch.equal(made["new"].cpu(), new) and torch.equal(made["w"].cpu(), w)
+    assert torch.equal(made["sin"].cpu(), sin) and torch.equal(made["cos"].cpu(), cos)
+    slab.check()
