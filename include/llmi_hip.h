@@ -486,7 +486,9 @@ typedef struct llmi_qk_norm_rope_kv8_args {
 } llmi_qk_norm_rope_kv8_args;
 
 /* llmi_hip_qk_norm_rope_append for consecutive tokens and an 8-bit cache: K rows are normalised, rotated and rounded to bf16 as there (what the bf16
- * cache would hold; the bits of llmi_hip_mha_decode_append), then quantised; V rows are quantised as they are. One launch, no allocation. */
+ * cache would hold; the bits of llmi_hip_mha_decode_append), then quantised; V rows are quantised as they are. One launch, no allocation.
+ * The queries may take their raw rows' place (same address and stride). Else what is written -- the query rows, the cache up to and with the layer -- must not overlap what is
+ * read, nor one another (LLMI_ERR_INVALID_ARG); rows of the same stride may interleave, slices of one buffer, rows of different strides may not. */
 int llmi_hip_qk_norm_rope_append_kv8(const llmi_qk_norm_rope_kv8_args* args);
 
 typedef struct llmi_mha_kv8_args {

@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <initializer_list>
 
 #include "llmi_hip.h"
 #include "llmi_internal.h"
@@ -132,6 +133,45 @@ bool writes_apart(const llmi_mha_kv8_args* a, const llmi_mha_kv8_append_args* ap
     return true;
 }
 
+// Rows of the same length, `stride` bytes from one to the next: tokens' slices of a projection's result, or (one of them) anything.
+struct Rows {
+    const void* first;
+    size_t width, stride;
+    int32_t count;
+};
+Range span(const Rows& r) {
+    size_t n;
+    return range(r.first, __builtin_mul_overflow((size_t)(r.count - 1), r.stride, &n) || __builtin_add_overflow(n, r.width, &n) ? SIZE_MAX : n);
+}
+// Exact for rows of the same stride, as many of each, and for one row against others; rows of different strides are apart if their spans are.
+bool apart(const Rows& a, const Rows& b) {
+    const Range x = span(a), y = span(b);
+    if (apart(x, y)) return true;
+    if (a.count == 1 || (b.count == 1 ? y.from < x.from : a.stride != b.stride)) return false;
+    const size_t behind = y.from >= x.from ? (y.from - x.from) % a.stride : (a.stride - (x.from - y.from) % a.stride) % a.stride;
+    return behind >= a.width && b.width <= a.stride && behind <= a.stride - b.width;
+}
+
+// Whether what the rows' call writes, queries and cache, is apart from what it reads. (Queries in their raw rows' place are not: a row is read and written by the same lanes.)
+bool writes_apart(const llmi_qk_norm_rope_kv8_args* a) {
+    if (a->layer_id == INT32_MAX) return false;
+    const size_t heads = (size_t)a->head_num * 256, kv = (size_t)a->kv_dim * 2, table = ((size_t)a->pos + (size_t)a->row_num) * 256;
+    const auto rows = [&](const void* p, size_t width, int64_t stride) { return Rows{p, width, a->row_num > 1 && stride ? (size_t)stride * 2 : width, a->row_num}; };
+    const auto whole = [](Range r) { return Rows{reinterpret_cast<const void*>(r.from), r.to - r.from, r.to - r.from, 1}; };
+    const Rows query = rows(a->query, heads, a->query_stride), src = rows(a->query_src, heads, a->query_src_stride);
+    const Rows cache = whole(cache_range(a->cache8, a->layer_id + 1, a->max_seq_len, a->kv_dim));
+    const Rows reads[] = {rows(a->key_new, kv, a->key_new_stride), rows(a->value_new, kv, a->value_new_stride), whole(range(a->norm_weight, 512)), whole(range(a->sin_cache, table)),
+                          whole(range(a->cos_cache, table))};
+    for (const Rows& r : {query, src, reads[0], reads[1]})
+        if (span(r).to == UINTPTR_MAX) return false;  // (no memory holds them)
+    for (const Rows& r : reads)
+        if (!apart(query, r) || !apart(r, cache)) return false;
+    if (a->query_src && !(a->query_src == a->query && src.stride == query.stride) && !apart(query, src)) return false;
+    if (a->query_src && !apart(src, cache)) return false;
+    if (a->pos_device && (!apart(query, whole(range(a->pos_device, 4))) || !apart(span(cache), range(a->pos_device, 4)))) return false;
+    return apart(query, cache);
+}
+
 int validate_copy(const llmi_kv8_copy_args* a) {
     if (!a) return LLMI_ERR_NULL_POINTER;
     if (!a->key_cache || !a->value_cache || !a->cache8) return LLMI_ERR_NULL_POINTER;
@@ -186,6 +226,7 @@ int llmi_hip_qk_norm_rope_append_kv8(const llmi_qk_norm_rope_kv8_args* a) {
         if (strides[i] < least[i] && a->row_num > 1) return LLMI_ERR_INVALID_ARG;
     }
     if (!aligned(a->pos_device, 4)) return LLMI_ERR_ALIGNMENT;
+    if (!writes_apart(a)) return LLMI_ERR_INVALID_ARG;
     return launch_qk_norm_rope_append_kv8(*a);
 }
 

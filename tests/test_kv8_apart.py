@@ -55,3 +55,55 @@ def test_a_cache_past_any_address():
         a = mha(at, False)
         a.layer_id, a.max_seq_len = layer, msl
         assert B.lib().llmi_hip_mha_decode_kv8(ctypes.byref(a)) == REFUSED
+
+
+# The rows' call: three tokens whose projections lie in one buffer, a token's query, key and value behind one another.
+N, PACKED = 3, (N_Q + 2 * N_KV) * 256
+ROWS = {n: ((i + 20) << 32, size) for i, (n, size) in enumerate((
+    ("query", N * N_Q * 256), ("query_src", 2 * PACKED + N_Q * 256), ("cache8", CACHE), ("pos_device", 4), ("norm_weight", 512), ("sin_cache", (POS + N) * 256), ("cos_cache", (POS + N) * 256)))}
+ROWS["key_new"] = (ROWS["query_src"][0] + N_Q * 256, 2 * PACKED + N_KV * 256)
+ROWS["value_new"] = (ROWS["key_new"][0] + N_KV * 256, 2 * PACKED + N_KV * 256)
+
+
+def append_rows(at, **more):
+    a = B.QkNormRopeKv8Args(layer_id=LAYER, pos=POS, row_num=N, kv_dim=N_KV * 128, head_num=N_Q, head_dim=128, max_seq_len=MSL, eps=1e-6, query_src_stride=PACKED // 2,
+                            key_new_stride=PACKED // 2, value_new_stride=PACKED // 2)
+    for name, value in {**at, **more}.items():
+        setattr(a, name, value)
+    return B.lib().llmi_hip_qk_norm_rope_append_kv8(ctypes.byref(a))
+
+
+def test_rows():
+    """Dense query rows, and the cache, over each of the things that are read; over one another."""
+    for write in ("query", "cache8"):
+        for other in ROWS:
+            if other == write:
+                continue
+            for place in over(ROWS, write, other):
+                at = {n: x[0] for n, x in ROWS.items()}
+                if other == "query_src" and place == at["query_src"]:
+                    at["query_src"] += 16  # (in its place: below)
+                at[write] = place
+                assert append_rows(at) == REFUSED, (write, other, hex(place))
+
+
+@pytest.mark.parametrize("shift", [16, 256, N_Q * 256 - 16, N_Q * 256, (N_Q + N_KV) * 256, PACKED - 16, PACKED - N_Q * 256 + 16, -16, -N_Q * 256 + 16, 16 - PACKED])
+def test_rows_of_the_packed_buffer(shift):
+    """Query rows with the packed rows' stride whose place in them is another one's: a neighbouring head's, the key's, the value's, past the row's end."""
+    at = {n: x[0] for n, x in ROWS.items()}
+    at["query"] = at["query_src"] + shift
+    assert append_rows(at, query_stride=PACKED // 2) == REFUSED
+
+
+def test_rows_in_place():
+    """In the raw rows' place only with their stride; one row in another one's place not at all; a stride that has no end."""
+    at = {n: x[0] for n, x in ROWS.items()}
+    at["query"] = at["query_src"]
+    assert append_rows(at) == REFUSED  # (dense over packed)
+    assert append_rows(at, query_stride=PACKED) == REFUSED
+    at["query"] = at["query_src"] + PACKED
+    assert append_rows(at, query_stride=PACKED // 2) == REFUSED
+    at["query"], at["query_src"] = at["query_src"], 0
+    assert append_rows(at, query_stride=PACKED // 2 - 8) == REFUSED  # (runs into the keys)
+    at = {n: x[0] for n, x in ROWS.items()}
+    assert append_rows({**at, "query": at["cos_cache"] - (1 << 20)}, query_stride=(1 << 62)) == REFUSED

@@ -66,3 +66,32 @@ def test_attention(dev, keys, order):
     assert torch.equal(made["q"].cpu(), q) and torch.equal(made["new"].cpu(), new) and torch.equal(made["w"].cpu(), w)
     assert torch.equal(made["sin"].cpu(), sin) and torch.equal(made["cos"].cpu(), cos)
     slab.check()
+
+
+@pytest.mark.parametrize("n", [1, 3, 400])
+@pytest.mark.parametrize("how", ["behind", "in place", "named in place", "dense"])
+def test_rows(dev, how, n):
+    """Query rows in the packed buffer: behind a token's value, in the raw rows' place (told or not), or dense right behind the buffer."""
+    n_q, n_kv, msl = 6, 3, n + 50
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(n, (2 * n_q + 2 * n_kv) * D, generator=g).to(BF16)
+    w, (sin, cos) = (1 + 0.1 * torch.randn(2 * D, generator=g)).to(BF16), C.tables(msl)
+    cache = C.garbage(2, n_kv, msl, n)
+    dims = dict(row_num=n, layer_id=1, pos=20, kv_dim=n_kv * D, head_num=n_q, head_dim=D, max_seq_len=msl)
+    alone = [y.to(dev) for y in (x[:, :n_q * D].contiguous(), x[:, n_q * D:(n_q + n_kv) * D].contiguous(), x[:, (n_q + n_kv) * D:(n_q + 2 * n_kv) * D].contiguous(), cache, w, sin, cos)]
+    want = torch.zeros(n, n_q * D, dtype=BF16, device=dev)
+    ops.qk_norm_rope_append_kv8(want, *alone[1:], query_src=alone[0], **dims)
+    slab = Slab(dev, cache.numel() + x.numel() * 4 + 4 * msl * D + (1 << 14))
+    cache8, packed = slab.take(cache.shape, torch.uint8, cache), slab.take(x.shape, BF16, x)
+    out = slab.take((n, n_q * D), BF16)
+    word = slab.take((4,), torch.int32, torch.tensor([20, 0, 0, 0], dtype=torch.int32))
+    tables = slab.take(w.shape, BF16, w), slab.take(sin.shape, torch.float32, sin), slab.take(cos.shape, torch.float32, cos)
+    raw, k, v, behind = packed.split([n_q * D, n_kv * D, n_kv * D, n_q * D], dim=1)
+    query, src = {"behind": (behind, raw), "in place": (raw, None), "named in place": (raw, raw), "dense": (out, raw)}[how]
+    ops.qk_norm_rope_append_kv8(query, k, v, cache8, *tables, query_src=src, pos_device=word[:1], **dims)
+    assert torch.equal(query, want) and torch.equal(cache8, alone[3])
+    kept = x.to(dev)
+    assert torch.equal(k, kept[:, n_q * D:(n_q + n_kv) * D]) and torch.equal(v, kept[:, (n_q + n_kv) * D:(n_q + 2 * n_kv) * D])
+    if how in ("behind", "dense"):
+        assert torch.equal(raw, kept[:, :n_q * D])
+    slab.check()
