@@ -456,9 +456,10 @@ typedef struct llmi_kv8_copy_args {
     void* stream;
 } llmi_kv8_copy_args;
 
-/* Rows of a bf16 cache into the 8-bit one (a prompt that was prefilled in bf16, say). Every other position of both stays as it is. */
+/* Rows of a bf16 cache into the 8-bit one (a prompt that was prefilled in bf16, say). Every other position of both stays as it is. In both directions the
+ * 8-bit cache must not overlap the bf16 one (LLMI_ERR_INVALID_ARG): nothing is quantised in place. */
 int llmi_hip_kv8_store(const llmi_kv8_copy_args* args);
-/* Back: code * s, rounded to bf16 once. Every other position of both stays as it is. */
+/* Back: code * s, rounded to bf16 once. Every other position of both stays as it is. K and V are two caches that do not overlap (LLMI_ERR_INVALID_ARG). */
 int llmi_hip_kv8_load(const llmi_kv8_copy_args* args);
 
 typedef struct llmi_qk_norm_rope_kv8_args {

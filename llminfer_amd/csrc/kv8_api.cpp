@@ -185,6 +185,14 @@ int validate_copy(const llmi_kv8_copy_args* a) {
     return LLMI_OK;
 }
 
+// Whether the three caches of a copy are apart (the two that are read may be one).
+bool caches_apart(const llmi_kv8_copy_args* a, bool load) {
+    size_t rows = (size_t)a->max_seq_len * (size_t)a->kv_dim * 2;
+    if (__builtin_mul_overflow(rows, (size_t)a->layer_num, &rows)) return false;
+    const Range k = range(a->key_cache, rows), v = range(a->value_cache, rows), cache = cache_range(a->cache8, a->layer_num, a->max_seq_len, a->kv_dim);
+    return apart(k, cache) && apart(v, cache) && (!load || apart(k, v));
+}
+
 }  // namespace
 }  // namespace llmi
 
@@ -201,11 +209,15 @@ size_t llmi_hip_kv8_bytes(int32_t layer_num, int32_t max_seq_len, int32_t kv_dim
 
 int llmi_hip_kv8_store(const llmi_kv8_copy_args* args) {
     if (int rc = validate_copy(args)) return rc;
+    if (args->layer_num == 0 || args->num_pos == 0) return LLMI_OK;
+    if (!caches_apart(args, false)) return LLMI_ERR_INVALID_ARG;
     return launch_kv8_store(*args);
 }
 
 int llmi_hip_kv8_load(const llmi_kv8_copy_args* args) {
     if (int rc = validate_copy(args)) return rc;
+    if (args->layer_num == 0 || args->num_pos == 0) return LLMI_OK;
+    if (!caches_apart(args, true)) return LLMI_ERR_INVALID_ARG;
     return launch_kv8_load(*args);
 }
 

@@ -357,7 +357,6 @@ void launch_copy(const CopyArgs& a, hipStream_t stream, int format, bool past, C
 }  // namespace
 
 int launch_kv8_store(const llmi_kv8_copy_args& args) {
-    if (args.layer_num == 0 || args.num_pos == 0) return LLMI_OK;
     const CopyArgs a = copy_args(args);
     const hipStream_t stream = static_cast<hipStream_t>(args.stream);
     launch_copy(a, stream, args.format, streams(args, 2 * 256), kv8_store_kernel<LLMI_KV8_E4M3, false>, kv8_store_kernel<LLMI_KV8_E4M3, true>, kv8_store_kernel<LLMI_KV8_INT8, false>,
@@ -366,7 +365,6 @@ int launch_kv8_store(const llmi_kv8_copy_args& args) {
 }
 
 int launch_kv8_load(const llmi_kv8_copy_args& args) {
-    if (args.layer_num == 0 || args.num_pos == 0) return LLMI_OK;
     const CopyArgs a = copy_args(args);
     const hipStream_t stream = static_cast<hipStream_t>(args.stream);
     launch_copy(a, stream, args.format, streams(args, 2 * 130), kv8_load_kernel<LLMI_KV8_E4M3, false>, kv8_load_kernel<LLMI_KV8_E4M3, true>, kv8_load_kernel<LLMI_KV8_INT8, false>,

@@ -107,3 +107,21 @@ def test_rows_in_place():
     assert append_rows(at, query_stride=PACKED // 2 - 8) == REFUSED  # (runs into the keys)
     at = {n: x[0] for n, x in ROWS.items()}
     assert append_rows({**at, "query": at["cos_cache"] - (1 << 20)}, query_stride=(1 << 62)) == REFUSED
+
+
+@pytest.mark.parametrize("call,also", [("llmi_hip_kv8_store", False), ("llmi_hip_kv8_load", True)])
+def test_copies(call, also):
+    """Caches of three layers over one another, by a little or altogether; nothing to copy is no overlap."""
+    call, rows = getattr(B.lib(), call), 3 * MSL * N_KV * 256
+    places = {"key_cache": (1 << 36, rows), "value_cache": (2 << 36, rows), "cache8": (3 << 36, ops.kv8_bytes(3, MSL, N_KV * 128, 128))}
+    for one, other in (("key_cache", "cache8"), ("cache8", "key_cache"), ("value_cache", "cache8"), ("cache8", "value_cache")) + ((("key_cache", "value_cache"), ("value_cache", "key_cache")) if also else ()):
+        for place in over(places, one, other):
+            a = B.Kv8CopyArgs(layer_num=3, first_pos=7, num_pos=10, kv_dim=N_KV * 128, head_dim=128, max_seq_len=MSL)
+            for name, (where, _) in places.items():
+                setattr(a, name, where)
+            setattr(a, one, place)
+            assert call(ctypes.byref(a)) == REFUSED, (one, other, hex(place))
+            a.num_pos = 0
+            assert call(ctypes.byref(a)) == 0
+    a = B.Kv8CopyArgs(layer_num=(1 << 31) - 1, num_pos=1, kv_dim=1 << 20, head_dim=128, max_seq_len=1 << 16, key_cache=1 << 30, value_cache=1 << 62, cache8=1 << 20)
+    assert call(ctypes.byref(a)) == REFUSED  # (sizes that no memory has)

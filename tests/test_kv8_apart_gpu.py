@@ -95,3 +95,34 @@ def test_rows(dev, how, n):
     if how in ("behind", "dense"):
         assert torch.equal(raw, kept[:, :n_q * D])
     slab.check()
+
+
+@pytest.mark.parametrize("layout", [0, 1])
+@pytest.mark.parametrize("order", [1, -1])
+def test_copies(dev, order, layout):
+    layers, heads, msl = 2, 3, 48
+    g = torch.Generator().manual_seed(4)
+    k, v = (C.rows(g, layers, heads, msl) for _ in range(2))
+    laid = [(x if layout else x.transpose(1, 2)).contiguous() for x in (k, v)]
+    slab = Slab(dev, 4 * k.numel() + C.records(msl) * C.RECORD * layers * heads + 64)
+    pieces = [("k", laid[0].shape, BF16, laid[0]), ("cache", (layers, heads, C.records(msl), C.RECORD), torch.uint8, C.garbage(layers, heads, msl, 2)), ("v", laid[1].shape, BF16, laid[1])]
+    made = {n: slab.take(shape, dtype, like) for n, shape, dtype, like in pieces[::order]}
+    dims = dict(layer_num=layers, num_pos=msl, kv_dim=heads * D, head_dim=D, max_seq_len=msl, kv_layout=layout)
+    ops.kv8_store(made["k"], made["v"], made["cache"], **dims)
+    assert torch.equal(made["k"].cpu(), laid[0]) and torch.equal(made["v"].cpu(), laid[1])
+    kc, ks, vc, vs = C.unpack(made["cache"].cpu())
+    for codes, scale, rows in ((kc, ks, k), (vc, vs, v)):
+        q, s = C.quantise(rows, C.E4M3)
+        assert torch.equal(codes[:, :, :msl], q) and torch.equal(scale[:, :, :msl], s)
+    keep = made["cache"].clone()
+    made["k"].zero_(), made["v"].zero_()
+    ops.kv8_load(made["cache"], made["k"], made["v"], **dims)
+    assert torch.equal(made["cache"], keep)
+    for got, codes, scale in ((made["k"], kc, ks), (made["v"], vc, vs)):
+        ref = C.stands_for(codes, scale, C.E4M3)[:, :, :msl].float().to(BF16)
+        assert torch.equal(got.cpu(), (ref if layout else ref.transpose(1, 2)).contiguous())
+    slab.check()
+    # (what is read may be one cache)
+    ops.kv8_store(made["k"], made["k"], made["cache"], **dims)
+    kc, ks, vc, vs = C.unpack(made["cache"].cpu())
+    assert torch.equal(kc[:, :, :msl], vc[:, :, :msl]) and torch.equal(ks[:, :, :msl], vs[:, :, :msl])
