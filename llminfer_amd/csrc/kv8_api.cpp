@@ -69,9 +69,8 @@ constexpr int kMostJoining = 128;
 // 0.2 - 0.65 slower.)
 constexpr int kMostSliced = 18, kMostSlicedWhole = 12;
 
-// The workgroups a KV head's records are dealt to beyond that: one up to ten records (kKv8Single), then a record each up to one workgroup per compute unit. us by
-// splits, 32 Q / 8 KV heads, E4M3: 4.54 : 4.83 : 4.71 with 1 : 5 : 10 at 301 positions, 5.24 : 4.95 : 4.73 with 1 : 5 : 13 at 401, 5.52 : 4.85 : 4.71 with
-// 1 : 8 : 16 at 512, 4.90 : 4.75 with 16 : 32 at 1024, 5.68 : 6.55 with 32 : 64 at 4096, 7.31 : 7.96 at 8192, 14.2 : 15.9 at 32768, 42.7 : 45.6 at 131001.
+// The workgroups a KV head's records are dealt to beyond that: a record each up to 32, then three records each, up to one workgroup per compute unit. us by
+// splits, 32 Q / 8 KV heads, E4M3: 4.90 : 4.75 with 16 : 32 at 1024 positions, 5.68 : 6.55 with 32 : 64 at 4096, 7.31 : 7.96 at 8192, 14.2 : 15.9 at 32768, 42.7 : 45.6 at 131001.
 // Eight wavefronts a workgroup where four would have more than a record each alone, more than five in a split (each wavefront has one record on
 // its way; more in flight on a compute unit are slower: two a wavefront 43.9 : 42.4 us at 131001, 15.3 : 14.2 at 32768, three 18.6). us with 4 : 8: 3.08 : 3.16 at
 // 128 positions, 4.61 : 4.19 at 256, 5.48 : 4.54 at 301 (one split); 5.73 : 5.81 at 4096, 7.02 : 6.64 at 6008, 15.7 : 14.3 at 32768, 46.2 : 42.4 at 131001, whole
@@ -81,28 +80,17 @@ int make_form(const llmi_mha_kv8_args* a, int new_rows, Kv8Form* form) {
     const int64_t keys = (int64_t)a->pos + 1 - new_rows, tiles = (keys + 31) / 32;
     // (partial outputs are addressed with 31 bits)
     const size_t room = a->workspace ? std::min(a->workspace_bytes > 16 ? a->workspace_bytes - 16 : 0, (size_t)INT32_MAX) / split_bytes(a) : 0;
-    int64_t want = a->num_splits;
-    if (want == 0) {
-        want = std::min<int64_t>({std::max(256 / (a->kv_dim / 128), 1), kMaxSplits, (int64_t)room});
-        want = kv8_active_splits(tiles, (int)want);
+    if (a->num_splits > 0) {
+        form->splits = kv8_chosen_splits(tiles, a->num_splits);
+        if (form->splits > 1 && (size_t)form->splits > room) return LLMI_ERR_WORKSPACE;
+        form->sliced = 0;
     } else {
-        want = std::min(want, tiles);
-        if (want > 1 && (size_t)want > room) return LLMI_ERR_WORKSPACE;
-    }
-    form->splits = (int)std::max<int64_t>(want, 1);
-    form->waves = tiles > (form->splits == 1 ? 4 : 5 * (int64_t)form->splits) ? 8 : 4;
-    form->sliced = 0;
-    if (a->num_splits == 0) {
         const int most = a->format == LLMI_KV8_E4M3 ? kMostSliced : kMostSlicedWhole;
-        if (a->pos_device) {  // (one workgroup size for all lengths up to the bound)
-            form->sliced = most;
-            if (tiles > 4) form->waves = 8;
-        } else if (tiles <= most) {
-            form->sliced = most;
-            form->splits = 1;
-            form->waves = tiles > 4 ? 8 : 4;
-        }
+        form->sliced = tiles <= most || a->pos_device ? most : 0;
+        form->splits = tiles <= most ? 1 : kv8_active_splits(tiles, (int)std::min<int64_t>({std::max(256 / (a->kv_dim / 128), 1), kMaxSplits, (int64_t)room}));
     }
+    // (with slices at some lengths up to the bound their workgroup size is all lengths')
+    form->waves = tiles > (form->sliced || form->splits == 1 ? 4 : 5 * (int64_t)form->splits) ? 8 : 4;
     // (the new token's query heads, half a wavefront each, all but one wavefront's: six in one pass with four. us with 4 : 8, 64 Q heads: 3.70 : 3.46 at 127
     // positions, 5.74 : 5.95 at 1024, 6.15 : 6.17 at 2000, 7.61 : 7.05 at 4099)
     if (new_rows && a->kv_mul > 6 && (form->sliced || tiles >= 3 * (int64_t)form->splits)) form->waves = 8;

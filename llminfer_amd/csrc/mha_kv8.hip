@@ -519,7 +519,7 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
             if (split < kKv8Slices) kv8_attend<FORMAT, NW, APPEND, true>(a, sm, row, pos, 1, tiles, 0);
             return;
         }
-        active = kv8_active_splits(tiles, a.splits);
+        active = a.sliced > 0 ? kv8_active_splits(tiles, a.splits) : kv8_chosen_splits(tiles, a.splits);
         if (split >= active) return;
         // (a quotient in two steps of 24 bits, then one up or down: shorter than the compiler's division, and on the way to the first load)
         const float inverse = 1.0f / (float)active;

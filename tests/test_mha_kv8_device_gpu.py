@@ -116,3 +116,26 @@ def test_a_captured_step_from_the_first_token_on(dev, splits):
         keys, values = (C.stands_for(c, s, C.E4M3)[0, :, :pos + 1] for c, s in ((kc, ks), (vc, vs)))
         C.close(tap.cpu(), *C.attention(normed.cpu().view(n_q, D), keys, values), rounded=out.cpu())
         assert torch.equal(eager, graphed), pos
+
+
+@pytest.mark.parametrize("n_q,n_kv", HEADS)
+@pytest.mark.parametrize("keys,splits", [(200, 2), (200, 4), (310, 10), (330, 10), (600, 3), (4000, 70), (4000, 256), (9000, 200)])
+def test_a_chosen_number_is_the_same_on_both_sides(dev, keys, splits, n_q, n_kv):
+    """The position on the device or on the host: a chosen number of splits deals the records alike, so sums of the same order, the same bits."""
+    g = torch.Generator().manual_seed(keys + splits)
+    cache = C.filled(1, n_kv, keys + 1, keys, C.E4M3, keys)[0].to(dev)
+    q = C.rows(g, n_q, outliers=False).to(dev)
+    x = torch.randn((n_q + 2 * n_kv) * D, generator=g).to(BF16).to(dev).split([n_q * D, n_kv * D, n_kv * D])
+    w, (sin, cos) = torch.ones(2 * D, dtype=BF16, device=dev), (y.to(dev) for y in C.tables(keys + 1))
+    ws = torch.full((n_q * 132 * splits + 4,), math.nan, device=dev)
+    dims = dict(layer_id=0, kv_dim=n_kv * D, kv_mul=n_q // n_kv, head_num=n_q, head_dim=D, max_seq_len=keys + 1, num_splits=splits)
+    taps = []
+    for where in (dict(pos=keys - 1), dict(pos=keys - 1, pos_device=torch.tensor([keys - 1], dtype=torch.int32, device=dev))):
+        out, tap = unwritten(dev, n_q)
+        ops.mha_decode_kv8(q, cache, out, ws, output_f32=tap, **where, **dims)
+        out2, tap2 = unwritten(dev, n_q)
+        where = {n: y + 1 for n, y in where.items()}
+        ops.mha_decode_append_kv8(*x, w, sin, cos, cache.clone(), out2, ws, output_f32=tap2, **where, **dims)
+        taps.append((tap, tap2))
+    assert bool(torch.isfinite(taps[0][0]).all()) and bool(torch.isfinite(taps[0][1]).all())
+    assert torch.equal(taps[0][0], taps[1][0]) and torch.equal(taps[0][1], taps[1][1])
