@@ -11,7 +11,7 @@
 //   O^T  lane L: head L%16, channel 16 b + 4 (L/16) + r in register r of accumulator b = 0..7
 // so that the probabilities never leave their lane. Codes become bf16 on the way (exact); K's scale multiplies the score, V's the probability,
 // which enters the product as the sum of two bf16 numbers (2^-16 of it lost at most). Maximum, sum and accumulators are fp32; the accumulators are
-// rescaled only where a maximum has grown by more than 2^8.
+// rescaled only where a maximum has grown by more than 2^8, so a weight is up to 2^8 and sums over V stay in range for values up to 10^36 / positions.
 //
 // Two forms (rules and measurements: kv8_api.cpp):
 //   sliced  Short contexts: four workgroups a KV head, each with 32 of the columns and every position. K's codes are read (through the L2) and multiplied four
