@@ -495,7 +495,7 @@ int llmi_hip_qk_norm_rope_append_kv8(const llmi_qk_norm_rope_kv8_args* args);
 typedef struct llmi_mha_kv8_args {
     const void* query;        /* device, bf16 [head_num*128]                                          */
     void* cache8;             /* device, base of the 8-bit cache (all layers)                         */
-    void* workspace;          /* device, 16-byte aligned; may be NULL: one workgroup per KV head then */
+    void* workspace;          /* device, 16-byte aligned; may be NULL: one workgroup per KV head then, four for short contexts */
     size_t workspace_bytes;   /* llmi_hip_mha_workspace_bytes() is enough for any length              */
     void* output;             /* device, bf16 [head_num*128]                                          */
     float* output_f32;        /* optional device fp32 [head_num*128]: the result before its rounding  */
@@ -507,7 +507,7 @@ typedef struct llmi_mha_kv8_args {
     int32_t head_dim;         /* must be 128                                                          */
     int32_t max_seq_len;
     int32_t format;           /* LLMI_KV8_*                                                           */
-    int32_t num_splits;       /* 0 = auto; otherwise the workgroups a KV head's positions are dealt to at most */
+    int32_t num_splits;       /* 0 = auto; otherwise the workgroups a KV head's positions are dealt to, one for each record of 32 at most */
     void* stream;
     const int32_t* pos_device; /* optional, device int32: the position read at run time, clamped to 0..pos; `pos` sizes the launch */
 } llmi_mha_kv8_args;
@@ -521,7 +521,10 @@ typedef struct llmi_mha_kv8_args {
  * pos (LLMI_ERR_INVALID_ARG; the plan looks at the query and the outputs only).
  * Allocates nothing; safe under stream capture; the workspace needs no initialisation, and two calls that share one must not overlap in time. */
 int llmi_hip_mha_decode_kv8(const llmi_mha_kv8_args* args);
-/* What it would launch (no HIP call): as llmi_hip_mha_plan; group_pad is 16. */
+/* What llmi_hip_mha_decode_kv8 would launch (no HIP call), as llmi_hip_mha_plan; rows_per_split is a multiple of 32, group_pad is 16. Short contexts are single-pass:
+ * the four workgroups of a KV head that have a quarter of the columns each are no splits, have nothing to join and need no workspace. With pos_device it is the launch for positions
+ * 0..pos; at a shorter one fewer splits, or four slices, are at work. llmi_hip_mha_decode_append_kv8 reads a position less from the cache, and takes eight wavefronts for groups of more
+ * than six query heads where this says four, perhaps; it needs no more workspace. */
 int llmi_hip_mha_kv8_plan(const llmi_mha_kv8_args* args, llmi_mha_plan* plan);
 
 typedef struct llmi_mha_kv8_append_args {
