@@ -62,15 +62,19 @@ size_t split_bytes(const llmi_mha_kv8_args* a) { return (size_t)a->head_num * (1
 
 // A KV head's query heads are joined by different workgroups where those, which wait for each other, fit the chip with room to spare.
 constexpr int kMostJoining = 128;
-// Records up to which four workgroups of a KV head have 32 columns and all positions each: K's codes are read and multiplied four times, V's once, and
-// there is nothing to join. us, splits by the rule below : so, 32 Q / 8 KV heads E4M3: 2.69 : 2.45 at 21 positions, 2.94 : 2.56 at 128, 4.16 : 3.39 at 256, 4.54 : 3.83
+// Records up to which a KV head is not split, and KV heads up to which four workgroups have 32 of its columns and all positions each there: K's codes are read and multiplied
+// four times, V's once, and there is nothing to join. us, splits by the rule below : so, 32 Q / 8 KV heads E4M3: 2.69 : 2.45 at 21 positions, 2.94 : 2.56 at 128, 4.16 : 3.39 at 256, 4.54 : 3.83
 // at 320, 4.66 : 4.25 at 401, 4.67 : 4.35 at 512, 4.66 : 4.64 at 601, 4.73 : 5.19 at 701; with the new token 3.89 : 3.36 at 57, 5.06 : 4.47 at 300 (16 Q), 5.51 : 4.98
 // at 511. Whole numbers, whose conversion takes three times the instructions: 4.97 : 4.18 at 320, 4.86 : 5.08 at 401. (Sixteen wavefronts beyond eight records
-// 0.2 - 0.65 slower.)
-constexpr int kMostSliced = 18, kMostSlicedWhole = 12;
+// 0.2 - 0.65 slower.) Other KV heads, a record each : slices : one workgroup, at 58, 301 and 576 positions: 1 (16 Q) 8.40 : 2.71 : 3.34, 8.58 : 4.06 : 5.21, 5.54 : 4.95 : 6.49; 3 4.36 : 2.45 : 2.73,
+// 4.24 : 3.77 : 4.37, 4.66 : 4.65 : 5.66; 32 4.57 : 2.78 : 3.10, 4.77 : 3.95 : 4.83, 5.03 : 5.47 : 6.06; 64 4.73 : 2.95 : 3.24, 5.23 : 4.65 : 4.96, 6.68 : 5.89 : 6.23. With more there are more slices than compute
+// units, and one workgroup reads K once: 80 4.77 : 3.33 : 3.27, 5.51 : 5.87 : 5.02, 6.50 : 7.50 : 6.34; 128 4.87 : 3.47 : 3.36, 6.83 : 6.21 : 5.13, 7.45 : 8.88 : 6.67; 512 slices : one workgroup 6.71 : 4.55, 18.1 : 9.7, 30.3 : 14.5.
+constexpr int kMostSingle = 18, kMostSingleWhole = 12;
+constexpr int kMostSlicedHeads = 64;
 
 // The workgroups a KV head's records are dealt to beyond that: a record each up to 32, then three records each, up to one workgroup per compute unit. us by
 // splits, 32 Q / 8 KV heads, E4M3: 4.90 : 4.75 with 16 : 32 at 1024 positions, 5.68 : 6.55 with 32 : 64 at 4096, 7.31 : 7.96 at 8192, 14.2 : 15.9 at 32768, 42.7 : 45.6 at 131001.
+constexpr int kRecordEach = 32;
 // Eight wavefronts a workgroup where four would have more than a record each alone, more than five in a split (each wavefront has one record on
 // its way; more in flight on a compute unit are slower: two a wavefront 43.9 : 42.4 us at 131001, 15.3 : 14.2 at 32768, three 18.6). us with 4 : 8: 3.08 : 3.16 at
 // 128 positions, 4.61 : 4.19 at 256, 5.48 : 4.54 at 301 (one split); 5.73 : 5.81 at 4096, 7.02 : 6.64 at 6008, 15.7 : 14.3 at 32768, 46.2 : 42.4 at 131001, whole
@@ -80,15 +84,14 @@ int make_form(const llmi_mha_kv8_args* a, int new_rows, Kv8Form* form) {
     const int64_t keys = (int64_t)a->pos + 1 - new_rows, tiles = (keys + 31) / 32;
     // (partial outputs are addressed with 31 bits)
     const size_t room = a->workspace ? std::min(a->workspace_bytes > 16 ? a->workspace_bytes - 16 : 0, (size_t)INT32_MAX) / split_bytes(a) : 0;
-    if (a->num_splits > 0) {
-        form->splits = kv8_chosen_splits(tiles, a->num_splits);
-        if (form->splits > 1 && (size_t)form->splits > room) return LLMI_ERR_WORKSPACE;
-        form->sliced = 0;
-    } else {
-        const int most = a->format == LLMI_KV8_E4M3 ? kMostSliced : kMostSlicedWhole;
-        form->sliced = tiles <= most || a->pos_device ? most : 0;
-        form->splits = tiles <= most ? 1 : kv8_active_splits(tiles, (int)std::min<int64_t>({std::max(256 / (a->kv_dim / 128), 1), kMaxSplits, (int64_t)room}));
-    }
+    // (a chosen number: a record each)
+    const bool chosen = a->num_splits > 0;
+    form->single = chosen ? 1 : a->format == LLMI_KV8_E4M3 ? kMostSingle : kMostSingleWhole;
+    form->each = chosen ? INT32_MAX : kRecordEach;
+    form->sliced = !chosen && a->kv_dim / 128 <= kMostSlicedHeads && (a->pos_device || tiles <= form->single);
+    const int most = chosen ? a->num_splits : (int)std::max<size_t>(std::min<size_t>({(size_t)std::max(256 / (a->kv_dim / 128), 1), (size_t)kMaxSplits, room}), 1);
+    form->splits = kv8_active_splits((int)tiles, most, form->single, form->each);
+    if (form->splits > 1 && (size_t)form->splits > room) return LLMI_ERR_WORKSPACE;
     // (with slices at some lengths up to the bound their workgroup size is all lengths')
     form->waves = tiles > (form->sliced || form->splits == 1 ? 4 : 5 * (int64_t)form->splits) ? 8 : 4;
     // (the new token's query heads, half a wavefront each, all but one wavefront's: six in one pass with four. us with 4 : 8, 64 Q heads: 3.70 : 3.46 at 127

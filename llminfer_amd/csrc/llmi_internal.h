@@ -146,21 +146,18 @@ int launch_kv_commit_tree(const llmi_kv_commit_tree_args& args);
 constexpr int kKv8Record = LLMI_KV8_RECORD_BYTES;
 constexpr int64_t kKv8MostGroups = (1 << 24) - 1;  // workgroups of 256 threads along a grid's x: their threads are counted with 32 bits
 inline int64_t kv8_records(int32_t max_seq_len) { return ((int64_t)max_seq_len + LLMI_KV8_RECORD_POSITIONS - 1) / LLMI_KV8_RECORD_POSITIONS; }
-// The splits that a KV head's records are dealt to where there may be `splits` and nobody has chosen (measurements: kv8_api.cpp): a record each up
-// to 32, then three records each.
-LLMI_HOST_DEVICE constexpr int kv8_active_splits(int64_t tiles, int splits) {
-    const int64_t most = tiles <= 32 ? tiles : tiles <= 96 ? 32 : tiles / 3;
-    return splits < 2 || tiles < 2 ? 1 : most < splits ? (int)most : splits;
+// The splits that a KV head's records are dealt to where there may be `splits` (measurements: kv8_api.cpp): one up to `single` records, a record each up to
+// `each`, then 32, or three records each where those are more.
+LLMI_HOST_DEVICE constexpr int kv8_active_splits(int tiles, int splits, int single, int each) {
+    const int third = tiles / 3, most = tiles <= single ? 1 : tiles <= each ? tiles : third > 32 ? third : 32;
+    return most < splits ? most : splits;
 }
-// ... where the caller has: a record each up to that number.
-LLMI_HOST_DEVICE constexpr int kv8_chosen_splits(int64_t tiles, int splits) { return tiles < 1 ? 1 : tiles < splits ? (int)tiles : splits; }
 // How the attention takes a call (rules and measurements: kv8_api.cpp): splits of a KV head, wavefronts of a workgroup (4 or 8), fewest splits at
 // which a KV head's query heads are joined by different workgroups.
 struct Kv8Form {
     int splits, waves, spread_min;
-    // Records up to which four workgroups of a KV head have 32 columns and all positions each. Position on the host: 0 where the call is not so. On the
-    // device: 0 where the caller has chosen the splits.
-    int sliced;
+    int single, each;  // kv8_active_splits
+    int sliced;        // up to `single` records four workgroups of a KV head have 32 columns and all positions each, not one everything
 };
 constexpr int kKv8Slices = 4;
 int launch_mha_kv8(const llmi_mha_kv8_args& args, const llmi_mha_kv8_append_args* append, const Kv8Form& form);

@@ -50,7 +50,8 @@ struct Kv8Args {
     uint32_t tag;
     int32_t pos, group, n_q, splits, max_polls;
     int32_t run, longer;          // records per split, and how many splits take one more (position known on the host)
-    int32_t sliced;               // position read on the device: records up to which a workgroup has 32 columns and all of them; 0: at no number
+    int32_t single, each;         // position read on the device: kv8_active_splits
+    int32_t sliced;               // ... records up to which a workgroup has 32 columns and all of them, -1 where the launch is not for that
     int32_t spread_min;           // fewest splits at which a KV head's query heads are joined by different workgroups
     float scale_log2e;            // log2(e) / sqrt(128)
     // the new token's
@@ -514,12 +515,12 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
         const auto word = reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(a.pos_dev));
         pos = max(0, min(*word, a.pos));
         const int tiles = (int)(((int64_t)pos + (APPEND ? 0 : 1) + 31) >> 5), split = (int)blockIdx.y;
-        // (a chosen number of splits: 0, and fewer workgroups than slices, perhaps; a step at position 0, with no record, is one split's then)
-        if (a.sliced > 0 && tiles <= a.sliced) {
+        // (only where the launch has workgroups for the slices: a chosen number of splits, or many KV heads, go the other way, a step without a record too)
+        if (tiles <= a.sliced) {
             if (split < kKv8Slices) kv8_attend<FORMAT, NW, APPEND, true>(a, sm, row, pos, 1, tiles, 0);
             return;
         }
-        active = a.sliced > 0 ? kv8_active_splits(tiles, a.splits) : kv8_chosen_splits(tiles, a.splits);
+        active = kv8_active_splits(tiles, a.splits, a.single, a.each);
         if (split >= active) return;
         // (a quotient in two steps of 24 bits, then one up or down: shorter than the compiler's division, and on the way to the first load)
         const float inverse = 1.0f / (float)active;
@@ -539,7 +540,7 @@ __global__ __launch_bounds__(NW * 64, 2) void mha_kv8_kernel(Kv8Args a) {
 
 template <int FORMAT, bool APPEND, Kv8Kind KIND>
 void launch(const Kv8Args& a, int n_kv, const Kv8Form& form, hipStream_t stream) {
-    const dim3 grid(n_kv, KIND == Kv8Kind::sliced ? kKv8Slices : KIND == Kv8Kind::device && a.sliced > 0 && a.splits < kKv8Slices ? kKv8Slices : a.splits);
+    const dim3 grid(n_kv, KIND == Kv8Kind::sliced ? kKv8Slices : KIND == Kv8Kind::device && form.sliced && a.splits < kKv8Slices ? kKv8Slices : a.splits);
     if (form.waves == 8) hipLaunchKernelGGL((mha_kv8_kernel<FORMAT, 8, APPEND, KIND>), grid, dim3(8 * 64), 0, stream, a);
     else hipLaunchKernelGGL((mha_kv8_kernel<FORMAT, 4, APPEND, KIND>), grid, dim3(4 * 64), 0, stream, a);
 }
@@ -547,7 +548,7 @@ void launch(const Kv8Args& a, int n_kv, const Kv8Form& form, hipStream_t stream)
 template <int FORMAT, bool APPEND>
 void launch(const Kv8Args& a, int n_kv, const Kv8Form& form, hipStream_t stream) {
     if (a.pos_dev) launch<FORMAT, APPEND, Kv8Kind::device>(a, n_kv, form, stream);
-    else if (form.sliced > 0) launch<FORMAT, APPEND, Kv8Kind::sliced>(a, n_kv, form, stream);
+    else if (form.sliced) launch<FORMAT, APPEND, Kv8Kind::sliced>(a, n_kv, form, stream);
     else launch<FORMAT, APPEND, Kv8Kind::split>(a, n_kv, form, stream);
 }
 
@@ -573,7 +574,9 @@ int launch_mha_kv8(const llmi_mha_kv8_args& m, const llmi_mha_kv8_append_args* a
     a.run = tiles / form.splits;
     a.longer = tiles % form.splits;
     a.spread_min = form.spread_min;
-    a.sliced = form.sliced;
+    a.single = form.single;
+    a.each = form.each;
+    a.sliced = form.sliced ? form.single : -1;
     a.scale_log2e = 1.4426950408889634f / sqrtf((float)kHeadDim);
     if (form.splits > 1) {
         a.ws = static_cast<float*>(m.workspace);

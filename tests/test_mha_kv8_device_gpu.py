@@ -139,3 +139,33 @@ def test_a_chosen_number_is_the_same_on_both_sides(dev, keys, splits, n_q, n_kv)
         taps.append((tap, tap2))
     assert bool(torch.isfinite(taps[0][0]).all()) and bool(torch.isfinite(taps[0][1]).all())
     assert torch.equal(taps[0][0], taps[1][0]) and torch.equal(taps[0][1], taps[1][1])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("n_q,n_kv", [(64, 64), (130, 65), (130, 130)])
+def test_many_kv_heads(dev, n_q, n_kv, fmt):
+    """More KV heads than a chip has workgroups for four each: one workgroup where fewer heads have slices. Steps with the position on the host and on the device."""
+    g = torch.Generator().manual_seed(n_q)
+    bound = 1300
+    msl = bound + 1
+    sin, cos = (x.to(dev) for x in C.tables(msl))
+    w = (1 + 0.1 * torch.randn(2 * D, generator=g)).to(BF16).to(dev)
+    q, k, v = (x.to(dev) for x in torch.randn((n_q + 2 * n_kv) * D, generator=g).to(BF16).split([n_q * D, n_kv * D, n_kv * D]))
+    ws = torch.full((ops.workspace_bytes(n_q, D, msl) // 4,), math.nan, device=dev)
+    dims = dict(layer_id=0, kv_dim=n_kv * D, head_num=n_q, head_dim=D, max_seq_len=msl, kv8_format=fmt)
+    full = C.filled(1, n_kv, msl, bound, fmt, n_q)[0].to(dev)
+    for at in (0, 1, 40, 384, 385, 576, 577, bound):
+        filed, normed = full.clone(), torch.zeros(1, n_q * D, dtype=BF16, device=dev)
+        ops.qk_norm_rope_append_kv8(normed, k[None], v[None], filed, w, sin, cos, row_num=1, query_src=q[None], pos=at, **dims)
+        kc, ks, vc, vs = C.unpack(filed.cpu())
+        keys, values = (C.stands_for(c, s, fmt)[0, :, :at + 1] for c, s in ((kc, ks), (vc, vs)))
+        want = C.attention(normed.cpu().view(n_q, D), keys, values)
+        for where in (dict(pos=at), dict(pos=bound, pos_device=torch.tensor([at], dtype=torch.int32, device=dev))):
+            out, tap = unwritten(dev, n_q)
+            mine = full.clone()
+            ops.mha_decode_append_kv8(q, k, v, w, sin, cos, mine, out, ws, output_f32=tap, kv_mul=n_q // n_kv, **where, **dims)
+            C.close(tap.cpu(), *want, rounded=out.cpu())
+            assert torch.equal(mine, filed)
+            out, tap = unwritten(dev, n_q)
+            ops.mha_decode_kv8(normed.view(-1), filed, out, ws, output_f32=tap, kv_mul=n_q // n_kv, **where, **dims)
+            C.close(tap.cpu(), *want, rounded=out.cpu())
