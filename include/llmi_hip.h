@@ -512,8 +512,8 @@ typedef struct llmi_mha_kv8_args {
     const int32_t* pos_device; /* optional, device int32: the position read at run time, clamped to 0..pos; `pos` sizes the launch */
 } llmi_mha_kv8_args;
 
-/* llmi_hip_mha_decode over an 8-bit cache: K and V are what the codes stand for, scores, maxima, sums and accumulators fp32, a weight times V's
- * scale enters the sum over V as the sum of two bf16 numbers (2^-16 of it lost at most). The sums are divided by their weights at the end, and a weight is up to
+/* llmi_hip_mha_decode over an 8-bit cache: K and V are what the codes stand for, scores, weights, maxima, sums and accumulators fp32 (a weight times V's
+ * scale enters the sum over V as the sum of three bf16 numbers, which hold all its bits). The sums are divided by their weights at the end, and a weight is up to
  * 2^8 (the maximum it is taken against is followed only when it has grown by more): values up to 10^36 / positions never leave fp32's range on the way, larger ones may come
  * out as infinities or NaN. One launch; where it is split, one or some workgroups of a
  * KV head wait (bounded: llmi_hip_set_poll_limit) for the others. What is written -- output, output_f32, the part of the

@@ -10,11 +10,13 @@
 //   P^T  lane L: those eight, place 8 (L/16) + 4 t + r          V^T  lane L: channel 16 b + L%16, the same positions: eight bytes of the record
 //   O^T  lane L: head L%16, channel 16 b + 4 (L/16) + r in register r of accumulator b = 0..7
 // so that the probabilities never leave their lane. Codes become bf16 on the way (exact); K's scale multiplies the score, V's the probability,
-// which enters the product as the sum of two bf16 numbers (2^-16 of it lost at most). Maximum, sum and accumulators are fp32; the accumulators are
+// which enters the product as the sum of three bf16 numbers: all bits that it has in fp32. (Of two numbers 2^-17 of it is lost, and results are 2e-6 from 64 bits where these are 1 - 3e-7; us, two : three,
+// 2.42 : 2.47 at 58 positions (16 Q), 4.67 : 4.73 at 1024, 5.60 : 5.70 at 4096, 14.4 : 14.6 at 32768, 44.4 : 44.7 at 131001, whole numbers 6.93 : 7.09 at 6008, with the new token 4.36 : 4.46 at 300.)
+// Maximum, sum and accumulators are fp32; the accumulators are
 // rescaled only where a maximum has grown by more than 2^8, so a weight is up to 2^8 and sums over V stay in range for values up to 10^36 / positions.
 //
 // Two forms (rules and measurements: kv8_api.cpp):
-//   sliced  Short contexts: four workgroups a KV head, each with 32 of the columns and every position. K's codes are read (through the L2) and multiplied four
+//   sliced  Short contexts of up to 64 KV heads: four workgroups a KV head, each with 32 of the columns and every position. K's codes are read (through the L2) and multiplied four
 //           times, V's once; nothing is handed from workgroup to workgroup, which costs a call 1.8 us otherwise (a record a wavefront: 2.9 in one workgroup, 4.7 joined).
 //   split   A KV head's records are dealt to up to 256 workgroups in contiguous runs, a workgroup's wavefronts take them in turn, one record of each on its way
 //           (more in flight on a compute unit come back later, not faster). Every split leaves its partial outputs and, once they are acknowledged, a
@@ -23,7 +25,8 @@
 // What bounds it: the launch and a trip to memory up to some hundred positions (32 Q / 8 KV heads, E4M3, captured: 2.5 us at 58, 4.4 at 512), the hand-over up to some
 // thousand (4.8 at 1024, 5.7 at 4096), then memory: 14.5 us at 32768 (68 MB), 42 - 44.5 by card at 131001 with 64 Q heads (272 MB, 6.2 TB/s with everything, 6.9 beyond
 // the 4.8). Over the bf16 cache the same calls took 7.0 at 4096, 23.6 and 82.4 beside them.
-// Whole-number codes take three instructions for two values where E4M3's take one, E4M3 : whole numbers 6.8 : 7.2 at 6008 positions, 44.1 : 44.6 at 131001.
+// Whole-number codes take three instructions for two values where E4M3's take one, E4M3 : whole numbers 6.8 : 7.2 at 6008 positions, 44.1 : 44.6 at 131001; with
+// the new token 3.17 : 3.29 at 57 (16 Q), 5.06 : 5.30 at 1024, 6.34 : 6.66 at 4099, 14.57 : 14.96 at 32768.
 
 #include <hip/hip_runtime.h>
 #include <float.h>
@@ -271,7 +274,7 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args& a, Kv8Shared<NW, COLUM
                     for (int e = 0; e < 4; ++e) o[b][e] *= alpha;
             }
         }
-        u32x4 ph, pl;
+        u32x4 ph, pm, pl;  // a weight's three numbers, all of its bits together
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float p0 = fast_exp2(c[2 * e] - m_run), p1 = fast_exp2(c[2 * e + 1] - m_run);
@@ -279,12 +282,16 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args& a, Kv8Shared<NW, COLUM
             const float x0 = p0 * vs[2 * e], x1 = p1 * vs[2 * e + 1];
             const uint32_t w = pack_bf16(x0, x1);
             ph[e] = w;
-            pl[e] = pack_bf16(x0 - bf16_lo(w), x1 - bf16_hi(w));
+            const float y0 = x0 - bf16_lo(w), y1 = x1 - bf16_hi(w);
+            const uint32_t z = pack_bf16(y0, y1);
+            pm[e] = z;
+            pl[e] = pack_bf16(y0 - bf16_lo(z), y1 - bf16_hi(z));
         }
 #pragma unroll
         for (int b = 0; b < kAccs; ++b) {
             const bf16x8 x = kv8_operand<FORMAT>(r.v[b >> 1][2 * (b & 1)], r.v[b >> 1][2 * (b & 1) + 1]);
             o[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(bf16x8, ph), o[b], 0, 0, 0);
+            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(bf16x8, pm), o[b], 0, 0, 0);
             o[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(bf16x8, pl), o[b], 0, 0, 0);
         }
     };
