@@ -76,8 +76,9 @@ constexpr int kMostSlicedHeads = 64;
 // splits, 32 Q / 8 KV heads, E4M3: 4.90 : 4.75 with 16 : 32 at 1024 positions, 5.68 : 6.55 with 32 : 64 at 4096, 7.31 : 7.96 at 8192, 14.2 : 15.9 at 32768, 42.7 : 45.6 at 131001.
 constexpr int kRecordEach = 32;
 // Eight wavefronts a workgroup where four would have more than a record each alone, more than five in a split (each wavefront has one record on
-// its way; more in flight on a compute unit are slower: two a wavefront 43.9 : 42.4 us at 131001, 15.3 : 14.2 at 32768, three 18.6). us with 4 : 8: 3.08 : 3.16 at
-// 128 positions, 4.61 : 4.19 at 256, 5.48 : 4.54 at 301 (one split); 5.73 : 5.81 at 4096, 7.02 : 6.64 at 6008, 15.7 : 14.3 at 32768, 46.2 : 42.4 at 131001, whole
+// its way; more in flight on a compute unit are slower: two a wavefront 43.9 : 42.4 us at 131001, 15.3 : 14.2 at 32768, three 18.6). us with 4 : 8: slices 3.10 : 3.15 at
+// 160 positions, 3.53 : 3.48 at 256, 4.35 : 3.96 at 301, 5.79 : 4.68 at 576, whole numbers 4.76 : 4.20 at 301, with the new token 3.74 : 3.71 at 160 (16 Q 3.74 : 3.62), 4.84 : 4.38 at 300; one workgroup 3.08 : 3.16 at
+// 128, 4.61 : 4.19 at 256, 5.48 : 4.54 at 301; splits 5.73 : 5.81 at 4096, 7.02 : 6.64 at 6008, 15.7 : 14.3 at 32768, 46.2 : 42.4 at 131001, whole
 // numbers, 64 Q heads 6.16 : 6.33 at 4096, 7.59 : 7.25 at 6008, 51.8 : 44.0 at 131001.
 int make_form(const llmi_mha_kv8_args* a, int new_rows, Kv8Form* form) {
     if (int rc = validate(a)) return rc;

@@ -22,11 +22,11 @@
 //           (more in flight on a compute unit come back later, not faster). Every split leaves its partial outputs and, once they are acknowledged, a
 //           record {tag | maximum} {tag | sum} per head in the workspace, past the caches; the last one (or the last ones, a head each), which are
 //           dispatched behind the others, wait for those (bounded) and add the parts up.
-// What bounds it: the launch and a trip to memory up to some hundred positions (32 Q / 8 KV heads, E4M3, captured: 2.5 us at 58, 4.4 at 512), the hand-over up to some
-// thousand (4.8 at 1024, 5.7 at 4096), then memory: 14.5 us at 32768 (68 MB), 42 - 44.5 by card at 131001 with 64 Q heads (272 MB, 6.2 TB/s with everything, 6.9 beyond
-// the 4.8). Over the bf16 cache the same calls took 7.0 at 4096, 23.6 and 82.4 beside them.
-// Whole-number codes take three instructions for two values where E4M3's take one, E4M3 : whole numbers 6.8 : 7.2 at 6008 positions, 44.1 : 44.6 at 131001; with
-// the new token 3.17 : 3.29 at 57 (16 Q), 5.06 : 5.30 at 1024, 6.34 : 6.66 at 4099, 14.57 : 14.96 at 32768.
+// What bounds it: the launch and a trip to memory up to some hundred positions (32 Q / 8 KV heads, E4M3, captured: 2.6 us at 58, 4.6 at 512), the hand-over up to some
+// thousand (4.9 at 1024, 5.8 at 4096), then memory: 14.8 us at 32768 (68 MB), 42 - 45 by card at 131001 with 64 Q heads (272 MB, 6.2 TB/s with everything, 6.9 beyond
+// the 4.9). Over the bf16 cache the same calls took 7.0 at 4096, 23.6 and 87.2 beside them.
+// Whole-number codes take three instructions for two values where E4M3's take one, E4M3 : whole numbers 6.9 : 7.3 at 6008 positions, 44.2 : 45.2 at 131001; with
+// the new token 3.20 : 3.33 at 57 (16 Q), 5.20 : 5.41 at 1024, 6.56 : 6.96 at 4099, 14.8 : 15.5 at 32768.
 
 #include <hip/hip_runtime.h>
 #include <float.h>
