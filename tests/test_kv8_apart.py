@@ -123,5 +123,5 @@ def test_copies(call, also):
             assert call(ctypes.byref(a)) == REFUSED, (one, other, hex(place))
             a.num_pos = 0
             assert call(ctypes.byref(a)) == 0
-    a = B.Kv8CopyArgs(layer_num=(1 << 31) - 1, num_pos=1, kv_dim=1 << 20, head_dim=128, max_seq_len=1 << 16, key_cache=1 << 30, value_cache=1 << 62, cache8=1 << 20)
+    a = B.Kv8CopyArgs(layer_num=(1 << 31) - 1, num_pos=1, kv_dim=1 << 20, head_dim=128, max_seq_len=1 << 15, key_cache=1 << 30, value_cache=1 << 62, cache8=1 << 20)
     assert call(ctypes.byref(a)) == REFUSED  # (sizes that no memory has)
